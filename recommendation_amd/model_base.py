@@ -144,13 +144,10 @@ def get_checkpoint_state(directory):
 # Lifetime of captured graphs.
 # What went wrong before: a process that captured many models in turn died with SIGSEGV inside hipGraphLaunch at a
 # replay of a freshly captured graph, whenever executables of earlier models had been destroyed - also when they were
-# destroyed with the device idle before and after.  The native stack (tools/repro/segv_trace.c) ends four frames below
-# at::cuda::CUDAGraph::replay inside libamdhip64, in a loop that walks an array of stream objects by an index with no
-# bound and dereferences the element (mov 0x1a8(%rax),%rdi with %rax = array[i]): the launch of an executable with
-# parallel branches picks its extra streams from a runtime-wide pool, and destroying another executable with
-# branches leaves that pool shorter than the survivor needs.  A graph with a single chain of nodes needs no extra
-# stream and never enters that loop.  So captured steps are single-chain graphs (the side stream is switched off
-# while capturing), and their executables can be destroyed.
+# destroyed with the device idle before and after.  The native stack (tools/repro/segv_trace.c) ends inside
+# hipGraphLaunch, below at::cuda::CUDAGraph::replay, and only executables with parallel branches were ever hit.
+# So captured steps are single-chain graphs (the side stream is switched off while capturing), and their
+# executables can be destroyed.
 # A graph owns no memory here (_capture asserts that nothing is allocated while
 # capturing; every buffer it points at belongs to its model or the session).  A graph executable is never destroyed
 # by the garbage collector: a model that is closed or collected hands its graphs - together with the static input
@@ -618,8 +615,8 @@ class CTRModel(GraphOwner):
             step0 = self.global_step
             self._indirect = (step_w, lr_w)
             # The captured step is one chain of launches: no second stream inside a graph.  An executable with
-            # parallel branches takes streams from a pool inside the HIP runtime when it is launched, and destroying
-            # another such executable shrinks that pool under it (see the note above _capture).
+            # parallel branches must not be launched after another such executable was destroyed (see the note above
+            # _capture).
             side_was = self.session.side_enabled
             self.session.side_enabled = False
             try:
