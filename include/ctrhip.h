@@ -39,6 +39,11 @@ int ctr_version(void);
 /* Host copy of the device dropout hash (24 random bits). */
 uint32_t ctr_keep_hash24(uint64_t seed, uint64_t stream_id, uint64_t index);
 
+/* Element types of the operators that take more than fp32 (the `dtype` arguments). */
+#define CTR_F32 0
+#define CTR_BF16 1
+#define CTR_F16 2
+
 /* Dropout descriptor: threshold == 0 or >= 2^24 with scale == 1 means "off". */
 typedef struct {
   uint64_t seed;
@@ -775,6 +780,71 @@ int ctr_allreduce_sum_f32(ctr_comm_t* comm, float* buf, int64_t n, void* stream)
 int ctr_all2all(ctr_comm_t* comm, const void* send, void* recv, int64_t bytes_per_peer, void* stream);
 int ctr_all2allv(ctr_comm_t* comm, const void* send, const int64_t* send_offset, const int64_t* send_bytes,
                  void* recv, const int64_t* recv_offset, const int64_t* recv_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------
+ * Attention towers over behaviour sequences: the general forms beside DIN's own attention (DIN/DIN.py:169-196), its
+ * inference-mode batch norm (DIN/DIN.py:45,53) and the optimizers.  fp32, bf16 and fp16 tensors (dtype); parameters,
+ * statistics and their gradients are fp32.
+ *
+ * Multi-head cross attention.  q, out: [B, Tq, H, D]; k, v: [B, Tk, Hkv, D], Hkv divides H and query head h uses key
+ * head h / (H / Hkv).  Any strides >= 0 with the last axis contiguous, every row on a 16-byte boundary; D a multiple of
+ * 8 up to 128.
+ *   s = scale q k^T over the keys t < sl[b] (clamped to [0, Tk]; NULL: all) with mask[b * mask_ld + t] != 0 (NULL: all)
+ *   out = softmax(s) v;  lse[b, h, i] = log sum_t exp(s) (optional; the backward needs it)
+ * What the memory of a key that is left out holds (NaN and infinities too) does not reach any result.  A query row
+ * without keys, or whose scores are all -infinity, gives zeros and lse = -infinity.  Valid fp32 values of 2^127 (2 - 2^-8)
+ * and above, infinities among them, give NaN where they enter.
+ * _bwd: dq, dk, dv (all overwritten, zeros for keys that are left out) from dout and the forward's q, k, v, out, lse,
+ * sl, mask; dk / dv are summed over the query heads that share a key head.  Outputs share no memory with an input or
+ * with each other.  All sums in a fixed order.
+ * ---------------------------------------------------------------------------------- */
+typedef struct {
+  int B, Tq, Tk, H, Hkv, D, dtype;
+  float scale;             /* > 0 */
+  const int32_t* sl;       /* [B], optional */
+  const uint8_t* mask;     /* rows of mask_ld bytes, optional */
+  int64_t mask_ld;
+} ctr_attn_t;
+typedef struct {
+  void* p;
+  int64_t stride_b, stride_t, stride_h; /* elements */
+} ctr_heads_t;
+size_t ctr_cross_attn_fwd_workspace_bytes(const ctr_attn_t* shape);
+int ctr_cross_attn_fwd(const ctr_attn_t* shape, const ctr_heads_t* q, const ctr_heads_t* k, const ctr_heads_t* v,
+                       const ctr_heads_t* out, float* lse_out, void* workspace, size_t workspace_bytes, void* stream);
+size_t ctr_cross_attn_bwd_workspace_bytes(const ctr_attn_t* shape);
+int ctr_cross_attn_bwd(const ctr_attn_t* shape, const ctr_heads_t* dout, const ctr_heads_t* q, const ctr_heads_t* k,
+                       const ctr_heads_t* v, const ctr_heads_t* out, const float* lse, const ctr_heads_t* dq,
+                       const ctr_heads_t* dk, const ctr_heads_t* dv, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/* Layer norm over the columns of a [rows, cols] view (any leading dimension >= cols, any alignment):
+ *   y = (x - mean) rstd gamma + beta,  rstd = 1 / sqrt(var + eps),  var = mean of (x - mean)^2
+ * gamma / beta [cols] optional (1 and 0).  mean_out, rstd_out [rows]: kept for the backward (optional).  y may be x.
+ * _bwd: with g = dy gamma and xh = (x - mean) rstd,  dx = rstd (g - mean(g) - xh mean(g xh)) (added to dx's content
+ * when accumulate_dx: the residual branch's gradient), dgamma = sum_rows dy xh, dbeta = sum_rows dy (either optional,
+ * overwritten; workspace only for them).  dx may be dy or x. */
+int ctr_layer_norm_fwd(const void* x, int64_t x_ld, int64_t rows, int cols, int dtype, const float* gamma,
+                       const float* beta, float eps, void* y, int64_t y_ld, float* mean_out, float* rstd_out,
+                       void* stream);
+size_t ctr_layer_norm_bwd_workspace_bytes(int64_t rows, int cols);
+int ctr_layer_norm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, const float* mean, const float* rstd,
+                       int64_t rows, int cols, int dtype, const float* gamma, void* dx, int64_t dx_ld,
+                       int accumulate_dx, float* dgamma, float* dbeta, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/* Global gradient norm over n tensors, and clipping by it (tf.clip_by_global_norm):
+ *   norm = sqrt(sum of all squares);  out = g * max_norm / max(norm, max_norm);  every out NaN if norm is not finite
+ * The lists are HOST arrays of device addresses, element counts and dtypes; they are read during the call only (a
+ * captured graph keeps its own copy).  Contiguous tensors of any alignment; a count may be 0.  out_host[i] may be
+ * grads_host[i] (in place; nothing is written then when the norm is within the bound); tensors must not overlap
+ * otherwise.  norm_out [1] (optional for ctr_clip_grads): the norm before clipping.  Squares are summed in fp64. */
+size_t ctr_grad_norm_workspace_bytes(int n_tensors);
+int ctr_grad_norm(const void* const* grads_host, const int64_t* counts_host, const int* dtypes_host, int n_tensors,
+                  float* norm_out, void* workspace, size_t workspace_bytes, void* stream);
+int ctr_clip_grads(const void* const* grads_host, void* const* out_host, const int64_t* counts_host,
+                   const int* dtypes_host, int n_tensors, float max_norm, float* norm_out, void* workspace,
+                   size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------
  * Input text of the Criteo display-advertising sets -> the arrays a step is fed with (host code, no GPU).

@@ -44,6 +44,17 @@ class Epilogue(C.Structure):
                 ('b_amax_floor', C.c_float), ('c_amax_out', C.c_void_p)]
 
 
+class AttnShape(C.Structure):
+    _fields_ = [('B', C.c_int), ('Tq', C.c_int), ('Tk', C.c_int), ('H', C.c_int), ('Hkv', C.c_int), ('D', C.c_int),
+                ('dtype', C.c_int), ('scale', C.c_float), ('sl', C.c_void_p), ('mask', C.c_void_p),
+                ('mask_ld', C.c_int64)]
+
+
+class Heads(C.Structure):
+    _fields_ = [('p', C.c_void_p), ('stride_b', C.c_int64), ('stride_t', C.c_int64), ('stride_h', C.c_int64)]
+
+
+F32, BF16, F16 = 0, 1, 2     # CTR_F32 / CTR_BF16 / CTR_F16
 OPT_GRAD_ONLY, OPT_ADAM, OPT_ADAGRAD, OPT_SGD, OPT_FTRL = 0, 1, 2, 3, 4
 COMM_ID_BYTES = 128          # CTR_COMM_ID_BYTES
 LOSS_SIGMOID_LOGLOSS, LOSS_IDENTITY_LOGLOSS, LOSS_SIGMOID_SCE_PROB, LOSS_SCE_LOGIT, LOSS_PROB_SCE = 0, 1, 2, 3, 4
@@ -164,6 +175,16 @@ SIGNATURES = {
     'ctr_dice_bwd_sum': (i, [vp, i64, i, i, vp, f, vp, i64, vp, i64, vp, vp]),
     'ctr_dsigmoid_apply': (i, [vp, i64, vp, i64, i, i, vp]),
     'ctr_mean_positive_diff': (i, [vp, vp, i, vp, vp]),
+    'ctr_cross_attn_fwd_workspace_bytes': (sz, [vp]),
+    'ctr_cross_attn_fwd': (i, [vp] * 6 + [vp, sz, vp]),
+    'ctr_cross_attn_bwd_workspace_bytes': (sz, [vp]),
+    'ctr_cross_attn_bwd': (i, [vp] * 10 + [vp, sz, vp]),
+    'ctr_layer_norm_fwd': (i, [vp, i64, i64, i, i, vp, vp, f, vp, i64, vp, vp, vp]),
+    'ctr_layer_norm_bwd_workspace_bytes': (sz, [i64, i]),
+    'ctr_layer_norm_bwd': (i, [vp, i64, vp, i64, vp, vp, i64, i, i, vp, vp, i64, i, vp, vp, vp, sz, vp]),
+    'ctr_grad_norm_workspace_bytes': (sz, [i]),
+    'ctr_grad_norm': (i, [vp, vp, vp, i, vp, vp, sz, vp]),
+    'ctr_clip_grads': (i, [vp, vp, vp, vp, i, f, vp, vp, sz, vp]),
     'ctr_copy2d': (i, [vp, i64, vp, i64, i, i, i, vp]),
     'ctr_mul2d': (i, [vp, i64, vp, i64, vp, i64, i, i, vp]),
     'ctr_dropout_apply': (i, [vp, i64, i, i, DP, vp]),

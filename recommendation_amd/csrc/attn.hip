@@ -1,0 +1,905 @@
+// Multi-head cross attention, forward and backward: Tq query rows attend to the Tk states of another sequence.
+//   s = scale q k^T over the keys t < sl[b] that mask[b] leaves;  p = softmax(s);  out = p v;  lse = log sum exp s
+//   delta = sum_d dout out;  ds = p (dout v^T - delta);  dq = scale ds k;  dk = scale ds^T q;  dv = p^T dout
+// H query heads share Hkv key heads in groups of G = H / Hkv.  The Tq * G query rows of one (sample, key head) form one
+// list (row r = query r / G, head r % G of the group), so a key tile is fetched once for the whole group and the sums
+// of dk / dv over the group fall out of the row loop.
+//
+// All products run on 32x32x16 matrix instructions.  The forward and the dq pass keep scores transposed (keys down,
+// query rows across): a lane owns one query row, so the running maximum, the sum and the rescaling are per-lane
+// scalars, and its 16 scores of a 32-key strip are already the second operand of the product with V (or K) once that
+// operand's rows are taken in the same order (kf_key below), which the transposing LDS read delivers.  The dk / dv pass
+// is the mirror image: a lane owns one key, the strip runs over query rows.
+// fp32 tensors are split into three bf16 terms (24 significant bits) and every product is the six largest of the nine
+// term products; the sums are fp32 in all types.  For 16-bit tensors p and ds are rounded to the tensors' type before
+// the second product (half a step each, independent over the keys that are summed, like the rounding of v and k
+// themselves); fp16's narrow exponent is met by a power of two on p (2^14) and a running one per row on ds.
+// A key behind sl[b] or off in the mask is staged as zeros and its p is set to zero, so nothing that its memory holds
+// reaches a result.  A row without keys gives zeros, lse = -inf and no gradient.  No float atomics: same bits every run.
+#include "types.h"
+
+namespace ctr {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
+
+// T: the tensors' type; NP: 16-bit terms per value; BIAS: log2 of the factor on p
+template <class T> struct Terms;
+template <> struct Terms<bf16_t> { static constexpr int NP = 1; static constexpr float BIAS = 0.f; };
+template <> struct Terms<f16_t> { static constexpr int NP = 1; static constexpr float BIAS = 14.f; };
+template <> struct Terms<float> { static constexpr int NP = 3; static constexpr float BIAS = 0.f; };
+
+// eight 16-bit values per term: one operand of a matrix instruction
+template <class T> struct Frag { s16x8 t[Terms<T>::NP]; };
+
+template <class T>
+__device__ static inline f32x16 mfma1(s16x8 a, s16x8 b, f32x16 c) {
+  if constexpr (__is_same(T, f16_t))
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <class T>
+__device__ static inline f32x16 mfma(const Frag<T>& a, const Frag<T>& b, f32x16 c) {
+  if constexpr (Terms<T>::NP == 1) {
+    return mfma1<T>(a.t[0], b.t[0], c);
+  } else {                                              // smallest products first
+    c = mfma1<T>(a.t[2], b.t[0], c);
+    c = mfma1<T>(a.t[0], b.t[2], c);
+    c = mfma1<T>(a.t[1], b.t[1], c);
+    c = mfma1<T>(a.t[1], b.t[0], c);
+    c = mfma1<T>(a.t[0], b.t[1], c);
+    return mfma1<T>(a.t[0], b.t[0], c);
+  }
+}
+
+__device__ static inline unsigned pack_bf16(float a, float b) {
+  const f32x2 v = {a, b};
+  return __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
+}
+// eight fp32 values -> operand (fp32: x = hi + mid + lo, each the bf16 nearest to what is left)
+template <class T>
+__device__ static inline Frag<T> make_frag(const float* f) {
+  Frag<T> r;
+  if constexpr (Terms<T>::NP == 1) {
+    r.t[0] = __builtin_bit_cast(s16x8, Packet<T>::pack(f));
+  } else {
+    unsigned w[3][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float a = f[2 * i], b = f[2 * i + 1];
+#pragma unroll
+      for (int t = 0; t < 3; ++t) {
+        const unsigned h = pack_bf16(a, b);
+        w[t][i] = h;
+        a -= __uint_as_float(h << 16);
+        b -= __uint_as_float(h & 0xffff0000u);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 3; ++t) r.t[t] = __builtin_bit_cast(s16x8, make_uint4(w[t][0], w[t][1], w[t][2], w[t][3]));
+  }
+  return r;
+}
+
+// Eight consecutive elements as they lie in memory (16 bytes of a 16-bit type, 32 of fp32).
+template <class T> struct Raw { uint4 w[sizeof(T) / 2]; };
+template <class T>
+__device__ static inline Raw<T> raw_load(const T* p) {
+  Raw<T> r;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = reinterpret_cast<const uint4*>(p)[i];
+  return r;
+}
+template <class T>
+__device__ static inline Raw<T> raw_zero() {
+  Raw<T> r;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = make_uint4(0, 0, 0, 0);
+  return r;
+}
+template <class T>
+__device__ static inline void raw_floats(const Raw<T>& r, float* f) {
+  if constexpr (sizeof(T) == 2) {
+    Packet<T>::unpack(r.w[0], f);
+  } else {
+    Packet<float>::unpack(r.w[0], f);
+    Packet<float>::unpack(r.w[1], f + 4);
+  }
+}
+template <class T>
+__device__ static inline Frag<T> raw_frag(const Raw<T>& r) {
+  Frag<T> o;
+  if constexpr (sizeof(T) == 2) {
+    o.t[0] = __builtin_bit_cast(s16x8, r.w[0]);
+  } else {
+    float f[8];
+    raw_floats<T>(r, f);
+    o = make_frag<T>(f);
+  }
+  return o;
+}
+
+// A tile of ROWS x DP values in LDS, one plane per term.  16 bytes of padding per row spread the rows over the banks.
+template <class T, int ROWS, int DP>
+struct Tile {
+  static constexpr int LD = DP + 8, NP = Terms<T>::NP, PLANE = ROWS * LD;
+  short v[NP * PLANE];
+  __device__ inline void put(int row, int col, const Frag<T>& f) {
+#pragma unroll
+    for (int t = 0; t < NP; ++t) *reinterpret_cast<s16x8*>(&v[t * PLANE + row * LD + col]) = f.t[t];
+  }
+  // first operand, rows r0 .. r0+31 down, columns col .. col+15 along the sum
+  __device__ inline Frag<T> rows(int r0, int col) const {
+    const int lane = threadIdx.x & 63;
+    Frag<T> f;
+#pragma unroll
+    for (int t = 0; t < NP; ++t)
+      f.t[t] = *reinterpret_cast<const s16x8*>(&v[t * PLANE + (r0 + (lane & 31)) * LD + col + (lane >> 5) * 8]);
+    return f;
+  }
+  // first operand, columns col .. col+31 down, rows r0 .. r0+15 along the sum in the order in which a lane holds the
+  // scores of 16 rows: element j of half h is row r0 + 4h + j (j < 4), r0 + 8 + 4h + j - 4 (j >= 4).  The transposing
+  // read takes, per 16 lanes, four rows of sixteen 16-bit values (four to a lane) and returns a column to each lane.
+  __device__ inline Frag<T> cols(int r0, int col) const {
+    const int lane = threadIdx.x & 63, i = lane & 15;
+    const int at = (r0 + 4 * (lane >> 5) + (i >> 2)) * LD + col + ((lane >> 4) & 1) * 16 + (i & 3) * 4;
+    Frag<T> f;
+#pragma unroll
+    for (int t = 0; t < NP; ++t) {
+      typedef __attribute__((address_space(3))) s16x4 lds4;
+      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(&v[t * PLANE + at]));
+      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(&v[t * PLANE + at + 8 * LD]));
+      f.t[t] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    return f;
+  }
+};
+// row of register r of a 32x32 product, before the 4 * (lane >> 5)
+__device__ static constexpr int acc_row(int r) { return (r & 3) + 8 * (r >> 2); }
+
+struct View4 {                                         // [B, T, heads, D]; strides in elements, the last is 1
+  const void* p;
+  int64_t b, t, h;
+};
+
+struct Attn {
+  View4 q, k, v, out, dout, dq, dk, dv;
+  float* lse;                                          // [B, H, Tq]
+  float* delta;                                        // [B, H, Tq]
+  const int32_t* sl;
+  const uint8_t* mask;
+  int64_t mask_ld;
+  int B, Tq, Tk, Hkv, G, D;
+  float scale, scale2;                                 // scale2 = scale * log2(e)
+  int rows, row_tiles, key_tiles, splits, per_split;
+  float *part, *part_lse;                              // [splits][B H Tq][D], [splits][B H Tq]
+};
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+__device__ static inline float minus_inf() { return -__builtin_inff(); }
+
+// Blocks that share a key head are neighbours in the logical order; the hardware deals consecutive blocks to the eight
+// dies in turn, so die d takes the d-th eighth of the logical order and its L2 holds only that eighth's keys.
+__device__ static inline int die_order(int id, int n) {
+  const int per = n >> 3, rem = n & 7, die = id & 7;
+  return die * per + min(die, rem) + (id >> 3);
+}
+
+__device__ static inline int key_count(const Attn& a, int b) {
+  if (!a.sl) return a.Tk;
+  return min(max(a.sl[b], 0), a.Tk);
+}
+
+struct RowAt { int t, h; };
+__device__ static inline RowAt row_at(const Attn& a, int r, int hk) {
+  if (a.G == 1) return {r, hk};
+  const int t = r / a.G;
+  return {t, hk * a.G + (r - t * a.G)};
+}
+template <class T>
+__device__ static inline const T* row_ptr(const View4& w, int b, const RowAt& ra) {
+  return (const T*)w.p + (int64_t)b * w.b + (int64_t)ra.t * w.t + (int64_t)ra.h * w.h;
+}
+__device__ static inline int64_t row_id(const Attn& a, int b, const RowAt& ra) {
+  return ((int64_t)b * (a.Hkv * a.G) + ra.h) * a.Tq + ra.t;
+}
+
+// max over a lane and its partner 32 lanes away
+__device__ static inline float half_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+  return fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
+}
+
+// The 32 rows from r0 of a row list as second operands: lane holds row r0 + (lane & 31)
+template <class T, int DP>
+__device__ static inline void load_row_frags(const T* p, bool ok, int D, Frag<T>* f) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    const int d = s * 16 + (lane >> 5) * 8;
+    f[s] = raw_frag<T>(ok && d < D ? raw_load(p + d) : raw_zero<T>());
+  }
+}
+
+// A lane's 16 values of one 32-column strip (columns acc_row(r) + 4 * half) to its row, four at a time
+template <class T>
+__device__ static inline void store_strip(T* row, int col0, int D, const f32x16& acc, float by) {
+  const int h4 = 4 * ((threadIdx.x & 63) >> 5);
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int d = col0 + 8 * g + h4;
+    if (d < D) {
+      const float a0 = acc[4 * g] * by, a1 = acc[4 * g + 1] * by, a2 = acc[4 * g + 2] * by, a3 = acc[4 * g + 3] * by;
+      if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(row + d) = make_float4(a0, a1, a2, a3);
+      } else if constexpr (__is_same(T, bf16_t)) {
+        *reinterpret_cast<uint2*>(row + d) = make_uint2(pack_bf16(a0, a1), pack_bf16(a2, a3));
+      } else {
+        const f16x2 x = {(f16_t)a0, (f16_t)a1}, y = {(f16_t)a2, (f16_t)a3};
+        *reinterpret_cast<uint2*>(row + d) = make_uint2(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y));
+      }
+    }
+  }
+}
+
+// Registers of a thread on the way from memory to a pair of tiles: ROWS rows of DP values of two views, dealt to THREADS
+template <class T, int ROWS, int DP, int THREADS>
+struct Stage {
+  static constexpr int PER = DP / 8, N = (ROWS * PER + THREADS - 1) / THREADS;
+  Raw<T> a[N], b[N];
+  bool on[N];
+  // keys k0 + row < k1 of one (sample, head); a masked key is read and dropped
+  __device__ inline void keys(const Attn& p, const T* ka, const T* kb, const uint8_t* mask, int k0, int k1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = threadIdx.x + i * THREADS, row = c / PER, d = (c - row * PER) * 8, key = k0 + row;
+      const bool in = row < ROWS && key < k1 && d < p.D;
+      a[i] = in ? raw_load(ka + (int64_t)key * p.k.t + d) : raw_zero<T>();
+      b[i] = in ? raw_load(kb + (int64_t)key * p.v.t + d) : raw_zero<T>();
+      on[i] = in && (!mask || mask[key]);
+    }
+  }
+  // rows r0 + row of the row list
+  __device__ inline void list(const Attn& p, int b_, int hk, int r0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = threadIdx.x + i * THREADS, row = c / PER, d = (c - row * PER) * 8, r = r0 + row;
+      const bool in = row < ROWS && r < p.rows && d < p.D;
+      const RowAt ra = row_at(p, in ? r : 0, hk);
+      a[i] = in ? raw_load(row_ptr<T>(p.q, b_, ra) + d) : raw_zero<T>();
+      b[i] = in ? raw_load(row_ptr<T>(p.dout, b_, ra) + d) : raw_zero<T>();
+      on[i] = true;
+    }
+  }
+  __device__ inline void put(Tile<T, ROWS, DP>& ta, Tile<T, ROWS, DP>& tb) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = threadIdx.x + i * THREADS, row = c / PER, d = (c - row * PER) * 8;
+      if (row < ROWS) {
+        ta.put(row, d, raw_frag<T>(on[i] ? a[i] : raw_zero<T>()));
+        tb.put(row, d, raw_frag<T>(on[i] ? b[i] : raw_zero<T>()));
+      }
+    }
+  }
+};
+
+// Bit i: key k0 + i may be attended to (the same in every lane)
+__device__ static inline uint64_t key_bits(const uint8_t* mask, int k0, int k1, int n) {
+  const int lane = threadIdx.x & 63, key = k0 + lane;
+  return __ballot(lane < n && key < k1 && (!mask || mask[key]));
+}
+
+// ---- forward -------------------------------------------------------------------------------------------------------
+// A wave owns QT x 32 query rows; the NW waves of a block share each tile of KT keys.
+template <class T, int DP, int NW, int QT, int KT>
+__global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(Attn a) {
+  constexpr int NS = KT / 32, NK = DP / 16, ND = DP / 32;
+  __shared__ Tile<T, KT, DP> kt, vt;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int id = die_order(blockIdx.x, gridDim.x);
+  const int split = id % a.splits;
+  id /= a.splits;
+  const int tile = id % a.row_tiles, bh = id / a.row_tiles, b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const int k0 = split * a.per_split, k1 = min(key_count(a, b), k0 + a.per_split);
+  const int r0 = (tile * NW + wave) * QT * 32;
+  const bool busy = r0 < a.rows;
+  const T* kp = (const T*)a.k.p + (int64_t)b * a.k.b + (int64_t)hk * a.k.h;
+  const T* vp = (const T*)a.v.p + (int64_t)b * a.v.b + (int64_t)hk * a.v.h;
+  const uint8_t* mask = a.mask ? a.mask + (int64_t)b * a.mask_ld : nullptr;
+
+  Frag<T> qf[QT][NK];
+  f32x16 o[QT][ND];
+  float m[QT], l[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = r0 + t * 32 + (lane & 31);
+    load_row_frags<T, DP>(row_ptr<T>(a.q, b, row_at(a, r < a.rows ? r : 0, hk)), r < a.rows, a.D, qf[t]);
+    m[t] = minus_inf();
+    l[t] = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[t][d] = f32x16{};
+  }
+
+  Stage<T, KT, DP, NW * 64> next;
+  if (k0 < k1) next.keys(a, kp, vp, mask, k0, k1);
+  for (int kb = k0; kb < k1; kb += KT) {
+    __syncthreads();                                   // every wave is done with the tile before this one
+    next.put(kt, vt);
+    const uint64_t bits = key_bits(mask, kb, k1, KT);
+    if (kb + KT < k1) next.keys(a, kp, vp, mask, kb + KT, k1);
+    __syncthreads();
+    if (!busy || bits == 0) continue;
+    f32x16 s[QT][NS];
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t) s[t][i] = f32x16{};
+#pragma unroll
+      for (int c = 0; c < NK; ++c) {
+        const Frag<T> kf = kt.rows(i * 32, c * 16);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) s[t][i] = mfma<T>(kf, qf[t][c], s[t][i]);
+      }
+    }
+    const bool all = bits == (KT == 64 ? ~0ull : ((1ull << (KT & 63)) - 1));
+    if (!all) {
+      const uint64_t mine = bits >> (4 * (lane >> 5));
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const bool on = (mine >> (i * 32 + acc_row(r))) & 1;
+#pragma unroll
+          for (int t = 0; t < QT; ++t) s[t][i][r] = on ? s[t][i][r] : minus_inf();
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      float top = m[t];
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][i][r]);
+      top = half_max(top);
+      const float base = top == minus_inf() ? 0.f : top;          // nothing seen yet: every p below is 2^-inf = 0
+      const float shift = Terms<T>::BIAS - base * a.scale2;
+      const float fade = __builtin_amdgcn_exp2f((m[t] - base) * a.scale2);
+      m[t] = top;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[t][i][r] = __builtin_amdgcn_exp2f(fmaf(s[t][i][r], a.scale2, shift));
+          sum += s[t][i][r];
+        }
+      l[t] = fmaf(l[t], fade, sum);
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[t][d][r] *= fade;
+    }
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        Frag<T> pf[QT];
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          float f[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = s[t][i][c * 8 + j];
+          pf[t] = make_frag<T>(f);
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const Frag<T> vf = vt.cols(i * 32 + c * 16, d * 32);
+#pragma unroll
+          for (int t = 0; t < QT; ++t) o[t][d] = mfma<T>(vf, pf[t], o[t][d]);
+        }
+      }
+  }
+  if (!busy) return;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = r0 + t * 32 + (lane & 31);
+    const float sum = half_swap_sum(l[t], l[t]);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (r >= a.rows) continue;
+    const RowAt ra = row_at(a, r, hk);
+    const int64_t rid = row_id(a, b, ra);
+    const float lse = sum == 0.f ? minus_inf() : m[t] * a.scale + (logf(sum) - Terms<T>::BIAS * LN2);
+    if (a.splits == 1) {
+      T* dst = const_cast<T*>(row_ptr<T>(a.out, b, ra));
+#pragma unroll
+      for (int d = 0; d < ND; ++d) store_strip<T>(dst, d * 32, a.D, o[t][d], inv);
+      if (a.lse && lane < 32) a.lse[rid] = lse;
+    } else {
+      const int64_t at = (int64_t)split * ((int64_t)a.B * a.Hkv * a.rows) + rid;
+      float* dst = a.part + at * a.D;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) store_strip<float>(dst, d * 32, a.D, o[t][d], inv);
+      if (lane < 32) a.part_lse[at] = lse;
+    }
+  }
+}
+
+// Joins the splits: out = sum_i w_i out_i, w_i = exp(lse_i - max) / sum; a thread per four columns of a row
+template <class T>
+__global__ __launch_bounds__(256) void attn_join_kernel(Attn a, int64_t n_rows) {
+  const int quads = a.D / 4;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= n_rows * quads) return;
+  const int64_t rid = id / quads;
+  const int d = (int)(id - rid * quads) * 4;
+  float top = minus_inf();
+  for (int i = 0; i < a.splits; ++i) top = fmaxf(top, a.part_lse[i * n_rows + rid]);
+  const float base = top == minus_inf() ? 0.f : top;
+  float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < a.splits; ++i) {
+    const float w = expf(a.part_lse[i * n_rows + rid] - base);
+    const float4 v = *reinterpret_cast<const float4*>(a.part + (i * n_rows + rid) * a.D + d);
+    sum += w;
+    acc[0] = fmaf(w, v.x, acc[0]);
+    acc[1] = fmaf(w, v.y, acc[1]);
+    acc[2] = fmaf(w, v.z, acc[2]);
+    acc[3] = fmaf(w, v.w, acc[3]);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int H = a.Hkv * a.G;
+  const int64_t bhead = rid / a.Tq;
+  const RowAt ra = {(int)(rid - bhead * a.Tq), (int)(bhead % H)};
+  T* dst = const_cast<T*>(row_ptr<T>(a.out, (int)(bhead / H), ra)) + d;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) dst[j] = (T)(acc[j] * inv);
+  if (a.lse && d == 0) a.lse[rid] = sum == 0.f ? minus_inf() : base + logf(sum);
+}
+
+// ---- backward ------------------------------------------------------------------------------------------------------
+// fp16: keeps ds * factor below 2^15 with a power of two per lane that only ever shrinks; the accumulators follow it
+template <int ND>
+__device__ static inline float fit_f16(const f32x16& ds, float factor, f32x16* acc) {
+  float top = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(ds[r]));
+  top = half_max(top);
+  const bool over = top * factor > 16384.f;
+  if (__any(over)) {
+    const float next = over ? ldexpf(1.f, 13 - ilogbf(fminf(top, 3.0e38f))) : factor;
+    const float by = next / factor;
+    factor = next;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[d][r] *= by;
+  }
+  return factor;
+}
+constexpr float F16_FACTOR0 = 1.2676506e30f;           // 2^100: the first strip with a gradient sets the factor
+
+// dq, and delta for the dk / dv pass.  A wave owns 32 query rows.
+template <class T, int DP, int NW, int KT>
+__global__ __launch_bounds__(NW * 64) void attn_dq_kernel(Attn a) {
+  constexpr int NS = KT / 32, NK = DP / 16, ND = DP / 32;
+  constexpr bool F16 = __is_same(T, f16_t);
+  __shared__ Tile<T, KT, DP> kt, vt;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int id = die_order(blockIdx.x, gridDim.x);
+  const int split = id % a.splits;
+  id /= a.splits;
+  const int tile = id % a.row_tiles, bh = id / a.row_tiles, b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const int k0 = split * a.per_split, k1 = min(key_count(a, b), k0 + a.per_split);
+  const int r0 = (tile * NW + wave) * 32;
+  const bool busy = r0 < a.rows;
+  const T* kp = (const T*)a.k.p + (int64_t)b * a.k.b + (int64_t)hk * a.k.h;
+  const T* vp = (const T*)a.v.p + (int64_t)b * a.v.b + (int64_t)hk * a.v.h;
+  const uint8_t* mask = a.mask ? a.mask + (int64_t)b * a.mask_ld : nullptr;
+
+  const int r = r0 + (lane & 31);
+  const bool in = r < a.rows;
+  const RowAt ra = row_at(a, in ? r : 0, hk);
+  const int64_t rid = row_id(a, b, ra);
+  Frag<T> qf[NK], gf[NK];
+  load_row_frags<T, DP>(row_ptr<T>(a.q, b, ra), in, a.D, qf);
+  float delta = 0.f;
+  {
+    const T* gp = row_ptr<T>(a.dout, b, ra);
+    const T* op = row_ptr<T>(a.out, b, ra);
+#pragma unroll
+    for (int s = 0; s < NK; ++s) {
+      const int d = s * 16 + (lane >> 5) * 8;
+      const bool ok = in && d < a.D;
+      const Raw<T> g = ok ? raw_load(gp + d) : raw_zero<T>(), w = ok ? raw_load(op + d) : raw_zero<T>();
+      float gv[8], wv[8];
+      raw_floats<T>(g, gv);
+      raw_floats<T>(w, wv);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta = fmaf(gv[j], wv[j], delta);
+      gf[s] = raw_frag<T>(g);
+    }
+    delta = half_swap_sum(delta, delta);
+  }
+  float shift = minus_inf();                           // a row without keys: p = 2^-inf
+  if (in) {
+    const float lse = a.lse[rid];
+    shift = lse == minus_inf() ? minus_inf() : -lse * LOG2E;
+    if (split == 0 && lane < 32) a.delta[rid] = delta;
+  }
+  f32x16 acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
+  float factor = F16 ? F16_FACTOR0 : 1.f;
+
+  Stage<T, KT, DP, NW * 64> next;
+  if (k0 < k1) next.keys(a, kp, vp, mask, k0, k1);
+  for (int kb = k0; kb < k1; kb += KT) {
+    __syncthreads();
+    next.put(kt, vt);
+    const uint64_t bits = key_bits(mask, kb, k1, KT);
+    if (kb + KT < k1) next.keys(a, kp, vp, mask, kb + KT, k1);
+    __syncthreads();
+    if (!busy || bits == 0) continue;
+    const uint64_t mine = bits >> (4 * (lane >> 5));
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+      for (int c = 0; c < NK; ++c) {
+        s = mfma<T>(kt.rows(i * 32, c * 16), qf[c], s);
+        dp = mfma<T>(vt.rows(i * 32, c * 16), gf[c], dp);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, shift));
+        const bool on = (mine >> (i * 32 + acc_row(e))) & 1;
+        dp[e] = on ? p * (dp[e] - delta) : 0.f;
+      }
+      if constexpr (F16) factor = fit_f16<ND>(dp, factor, acc);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = F16 ? dp[c * 8 + j] * factor : dp[c * 8 + j];
+        const Frag<T> df = make_frag<T>(f);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[d] = mfma<T>(kt.cols(i * 32 + c * 16, d * 32), df, acc[d]);
+      }
+    }
+  }
+  if (!in) return;
+  const float by = a.scale / factor;
+  if (a.splits == 1) {
+    T* dst = const_cast<T*>(row_ptr<T>(a.dq, b, ra));
+#pragma unroll
+    for (int d = 0; d < ND; ++d) store_strip<T>(dst, d * 32, a.D, acc[d], by);
+  } else {
+    float* dst = a.part + ((int64_t)split * ((int64_t)a.B * a.Hkv * a.rows) + rid) * a.D;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) store_strip<float>(dst, d * 32, a.D, acc[d], by);
+  }
+}
+
+// dk and dv.  A wave owns 32 keys and walks the query rows in tiles of QB.
+template <class T, int DP, int NW, int QB>
+__global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(Attn a) {
+  constexpr int NS = QB / 32, NK = DP / 16, ND = DP / 32;
+  constexpr bool F16 = __is_same(T, f16_t);
+  __shared__ Tile<T, QB, DP> qt, gt;
+  __shared__ float4 shift_s[QB / 4], delta_s[QB / 4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int id = die_order(blockIdx.x, gridDim.x);
+  const int tile = id % a.key_tiles, bh = id / a.key_tiles, b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const int len = key_count(a, b);
+  const int key0 = tile * NW * 32, key = key0 + wave * 32 + (lane & 31);
+  const bool on = key < len && (!a.mask || a.mask[(int64_t)b * a.mask_ld + key]);
+  const bool busy = __any(on);
+  f32x16 dk[ND], dv[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{};
+  float factor = F16 ? F16_FACTOR0 : 1.f;
+  if (key0 < len) {
+    Frag<T> kf[NK], vf[NK];
+    load_row_frags<T, DP>((const T*)a.k.p + (int64_t)b * a.k.b + (int64_t)hk * a.k.h + (int64_t)(on ? key : 0) * a.k.t, on, a.D, kf);
+    load_row_frags<T, DP>((const T*)a.v.p + (int64_t)b * a.v.b + (int64_t)hk * a.v.h + (int64_t)(on ? key : 0) * a.v.t, on, a.D, vf);
+    Stage<T, QB, DP, NW * 64> next;
+    float lse_n = 0.f, delta_n = 0.f;
+    auto fetch = [&](int r0) {
+      next.list(a, b, hk, r0);
+      if (threadIdx.x < QB) {
+        const int r = r0 + threadIdx.x;
+        lse_n = minus_inf();
+        delta_n = 0.f;
+        if (r < a.rows) {
+          const int64_t rid = row_id(a, b, row_at(a, r, hk));
+          lse_n = a.lse[rid];
+          delta_n = a.delta[rid];
+        }
+      }
+    };
+    fetch(0);
+    for (int r0 = 0; r0 < a.rows; r0 += QB) {
+      __syncthreads();
+      next.put(qt, gt);
+      if (threadIdx.x < QB) {
+        reinterpret_cast<float*>(shift_s)[threadIdx.x] = lse_n == minus_inf() ? minus_inf() : Terms<T>::BIAS - lse_n * LOG2E;
+        reinterpret_cast<float*>(delta_s)[threadIdx.x] = delta_n;
+      }
+      if (r0 + QB < a.rows) fetch(r0 + QB);
+      __syncthreads();
+      if (!busy) continue;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+        for (int c = 0; c < NK; ++c) {
+          s = mfma<T>(qt.rows(i * 32, c * 16), kf[c], s);
+          dp = mfma<T>(gt.rows(i * 32, c * 16), vf[c], dp);
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int at = i * 8 + 2 * g + (lane >> 5);   // rows i * 32 + 8 g + 4 half .. + 3
+          const float4 sh = shift_s[at], de = delta_s[at];
+          const float shv[4] = {sh.x, sh.y, sh.z, sh.w}, dev[4] = {de.x, de.y, de.z, de.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float p = on ? __builtin_amdgcn_exp2f(fmaf(s[4 * g + j], a.scale2, shv[j])) : 0.f;
+            s[4 * g + j] = p;
+            dp[4 * g + j] = on ? p * (dp[4 * g + j] - dev[j]) : 0.f;
+          }
+        }
+        if constexpr (F16) factor = fit_f16<ND>(dp, factor, dk);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float f[8], e[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            f[j] = s[c * 8 + j];
+            e[j] = F16 ? dp[c * 8 + j] * factor : dp[c * 8 + j];
+          }
+          const Frag<T> pf = make_frag<T>(f), df = make_frag<T>(e);
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+            dv[d] = mfma<T>(gt.cols(i * 32 + c * 16, d * 32), pf, dv[d]);
+            dk[d] = mfma<T>(qt.cols(i * 32 + c * 16, d * 32), df, dk[d]);
+          }
+        }
+      }
+    }
+  }
+  if (key >= a.Tk) return;
+  const float one = 1.f / exp2f(Terms<T>::BIAS);        // ds carries p's factor too
+  T* kd = (T*)a.dk.p + (int64_t)b * a.dk.b + (int64_t)key * a.dk.t + (int64_t)hk * a.dk.h;
+  T* vd = (T*)a.dv.p + (int64_t)b * a.dv.b + (int64_t)key * a.dv.t + (int64_t)hk * a.dv.h;
+#pragma unroll
+  for (int d = 0; d < ND; ++d) {
+    store_strip<T>(kd, d * 32, a.D, dk[d], a.scale * one / factor);
+    store_strip<T>(vd, d * 32, a.D, dv[d], one);
+  }
+}
+
+// dq = the sum over the splits, in split order
+template <class T>
+__global__ __launch_bounds__(256) void attn_sum_kernel(Attn a, int64_t n_rows) {
+  const int quads = a.D / 4;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= n_rows * quads) return;
+  const int64_t rid = id / quads;
+  const int d = (int)(id - rid * quads) * 4;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < a.splits; ++i) {
+    const float4 v = *reinterpret_cast<const float4*>(a.part + (i * n_rows + rid) * a.D + d);
+    acc[0] += v.x;
+    acc[1] += v.y;
+    acc[2] += v.z;
+    acc[3] += v.w;
+  }
+  const int H = a.Hkv * a.G;
+  const int64_t bhead = rid / a.Tq;
+  const RowAt ra = {(int)(rid - bhead * a.Tq), (int)(bhead % H)};
+  T* dst = const_cast<T*>(row_ptr<T>(a.dq, (int)(bhead / H), ra)) + d;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) dst[j] = (T)acc[j];
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------
+static int padded_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
+static int pass_rows(int rows) { return rows <= 32 ? 32 : 128; }          // query rows of a block: one wave or four
+static int tile_keys(int dtype) { return dtype == CTR_F32 ? 32 : 64; }
+
+// Splits of the key axis: only where the row tiles alone leave most of the chip idle, and never below 256 keys each.
+static int key_splits(int64_t blocks, int Tk) {
+  const int64_t want = blocks < 1 ? 1 : 1024 / blocks, most = Tk / 256;
+  const int64_t n = want < most ? want : most;
+  return (int)(n < 1 ? 1 : n);
+}
+
+static void attn_plan(Attn* a, int dtype) {
+  a->rows = a->Tq * a->G;
+  a->row_tiles = (int)cdiv(a->rows, pass_rows(a->rows));
+  a->splits = key_splits((int64_t)a->row_tiles * a->B * a->Hkv, a->Tk);
+  a->per_split = (int)align_up(cdiv(a->Tk, a->splits), 64);
+  a->splits = a->Tk > 0 ? (int)cdiv(a->Tk, a->per_split) : 1;
+  a->key_tiles = (int)cdiv(a->Tk, 128);
+}
+static int64_t total_rows(const Attn& a) { return (int64_t)a.B * a.Hkv * a.rows; }
+static size_t fwd_ws(const Attn& a) { return a.splits > 1 ? (size_t)a.splits * total_rows(a) * (a.D + 1) * 4 + 256 : 0; }
+static size_t bwd_ws(const Attn& a) {
+  return align_up((size_t)total_rows(a) * 4, 256) + (a.splits > 1 ? (size_t)a.splits * total_rows(a) * a.D * 4 : 0) + 256;
+}
+
+static int attn_shape(const char* what, const ctr_attn_t* s, Attn* a) {
+  CTR_REQUIRE(s, "%s: no shape", what);
+  CTR_REQUIRE(type_bytes(s->dtype) != 0, "%s: unknown dtype %d", what, s->dtype);
+  CTR_REQUIRE(s->B >= 0 && s->Tq >= 0 && s->Tk >= 0 && s->H >= 1 && s->Hkv >= 1 && s->H % s->Hkv == 0,
+              "%s: B %d Tq %d Tk %d H %d Hkv %d (Hkv must divide H)", what, s->B, s->Tq, s->Tk, s->H, s->Hkv);
+  CTR_REQUIRE(s->D >= 8 && s->D <= 128 && s->D % 8 == 0, "%s: head size %d is not a multiple of 8 up to 128", what, s->D);
+  CTR_REQUIRE(s->scale > 0.f && s->scale <= 3.0e38f, "%s: scale must be positive and finite", what);
+  CTR_REQUIRE((int64_t)s->Tq * (s->H / s->Hkv) < (1 << 30) && s->Tk < (1 << 30) && (int64_t)s->B * s->H < (1 << 30),
+              "%s: more than 2^30 rows, keys or heads", what);
+  CTR_REQUIRE(!s->mask || s->mask_ld >= 0, "%s: the mask has a negative stride", what);
+  *a = Attn{};
+  a->B = s->B; a->Tq = s->Tq; a->Tk = s->Tk; a->Hkv = s->Hkv; a->G = s->H / s->Hkv; a->D = s->D;
+  a->scale = s->scale;
+  a->scale2 = s->scale * LOG2E;
+  a->sl = s->sl; a->mask = s->mask; a->mask_ld = s->mask_ld;
+  attn_plan(a, s->dtype);
+  CTR_REQUIRE((int64_t)a->row_tiles * a->B * a->Hkv * a->splits < (1ll << 31) &&
+              (int64_t)a->key_tiles * a->B * a->Hkv < (1ll << 31), "%s: too many tiles", what);
+  return CTR_OK;
+}
+
+// strides of a [B, T, heads, D] view: 16-byte rows; an output may not name an element twice
+static int attn_view(const char* what, const char* name, const ctr_heads_t* v, int B, int T, int heads, int D, int dtype,
+                     bool output, View4* w) {
+  CTR_REQUIRE(v, "%s: %s is missing", what, name);
+  *w = View4{v->p, v->stride_b, v->stride_t, v->stride_h};
+  if ((int64_t)B * T * heads == 0) return CTR_OK;
+  const int per = 16 / type_bytes(dtype);
+  CTR_REQUIRE(v->p, "%s: %s is NULL", what, name);
+  CTR_REQUIRE(((uintptr_t)v->p & 15) == 0 && v->stride_b % per == 0 && v->stride_t % per == 0 && v->stride_h % per == 0,
+              "%s: %s and its rows must lie on 16-byte boundaries", what, name);
+  CTR_REQUIRE(v->stride_b >= 0 && v->stride_t >= 0 && v->stride_h >= 0, "%s: %s has a negative stride", what, name);
+  if (output) {
+    int64_t st[3] = {v->stride_b, v->stride_t, v->stride_h}, n[3] = {B, T, heads}, span = D;
+    for (int i = 0; i < 3; ++i)
+      for (int j = i + 1; j < 3; ++j)
+        if (st[j] < st[i]) { const int64_t x = st[i], y = n[i]; st[i] = st[j]; n[i] = n[j]; st[j] = x; n[j] = y; }
+    for (int i = 0; i < 3; ++i) {
+      if (n[i] == 1) continue;
+      CTR_REQUIRE(st[i] >= span, "%s: %s holds an element twice", what, name);
+      span = st[i] * (n[i] - 1) + span;
+    }
+  }
+  return CTR_OK;
+}
+
+#define ATTN_DIM(T, D, CALL)                    \
+  do {                                          \
+    switch (padded_dim(D)) {                    \
+      case 32: { CALL(T, 32); } break;          \
+      case 64: { CALL(T, 64); } break;          \
+      case 96: { CALL(T, 96); } break;          \
+      default: { CALL(T, 128); } break;         \
+    }                                           \
+  } while (0)
+
+template <class T>
+static void attn_fwd_launch(const Attn& a, hipStream_t st) {
+  constexpr int KT = sizeof(T) == 4 ? 32 : 64;
+  const unsigned blocks = (unsigned)((int64_t)a.row_tiles * a.B * a.Hkv * a.splits);
+  const bool one = pass_rows(a.rows) == 32;
+#define ATTN_FWD(T_, DP_)                                                         \
+  if (one) attn_fwd_kernel<T_, DP_, 1, 1, 32><<<blocks, 64, 0, st>>>(a);          \
+  else attn_fwd_kernel<T_, DP_, 4, 1, KT><<<blocks, 256, 0, st>>>(a)
+  ATTN_DIM(T, a.D, ATTN_FWD);
+#undef ATTN_FWD
+  if (a.splits > 1) {
+    const int64_t n = total_rows(a);
+    attn_join_kernel<T><<<(unsigned)cdiv(n * (a.D / 4), 256), 256, 0, st>>>(a, n);
+  }
+}
+
+template <class T>
+static void attn_bwd_launch(const Attn& a, hipStream_t st) {
+  constexpr int KT = sizeof(T) == 4 ? 32 : 64;
+  const unsigned blocks = (unsigned)((int64_t)a.row_tiles * a.B * a.Hkv * a.splits);
+  const bool one = pass_rows(a.rows) == 32;
+  if (blocks) {
+#define ATTN_DQ(T_, DP_)                                                          \
+  if (one) attn_dq_kernel<T_, DP_, 1, 32><<<blocks, 64, 0, st>>>(a);              \
+  else attn_dq_kernel<T_, DP_, 4, KT><<<blocks, 256, 0, st>>>(a)
+    ATTN_DIM(T, a.D, ATTN_DQ);
+#undef ATTN_DQ
+    if (a.splits > 1) {
+      const int64_t n = total_rows(a);
+      attn_sum_kernel<T><<<(unsigned)cdiv(n * (a.D / 4), 256), 256, 0, st>>>(a, n);
+    }
+  }
+  const unsigned kblocks = (unsigned)((int64_t)a.key_tiles * a.B * a.Hkv);
+  if (kblocks) {
+#define ATTN_DKV(T_, DP_) attn_dkv_kernel<T_, DP_, 4, 32><<<kblocks, 256, 0, st>>>(a)
+    ATTN_DIM(T, a.D, ATTN_DKV);
+#undef ATTN_DKV
+  }
+}
+
+}  // namespace ctr
+
+using namespace ctr;
+
+extern "C" size_t ctr_cross_attn_fwd_workspace_bytes(const ctr_attn_t* shape) {
+  Attn a;
+  return attn_shape("cross_attn_fwd", shape, &a) ? 0 : fwd_ws(a);
+}
+extern "C" size_t ctr_cross_attn_bwd_workspace_bytes(const ctr_attn_t* shape) {
+  Attn a;
+  return attn_shape("cross_attn_bwd", shape, &a) ? 0 : bwd_ws(a);
+}
+
+extern "C" int ctr_cross_attn_fwd(const ctr_attn_t* s, const ctr_heads_t* q, const ctr_heads_t* k, const ctr_heads_t* v,
+                                  const ctr_heads_t* out, float* lse_out, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+  const char* what = "cross_attn_fwd";
+  Attn a;
+  int rc = attn_shape(what, s, &a);
+  if (rc) return rc;
+  if ((rc = attn_view(what, "q", q, s->B, s->Tq, s->H, s->D, s->dtype, false, &a.q))) return rc;
+  if ((rc = attn_view(what, "k", k, s->B, s->Tk, s->Hkv, s->D, s->dtype, false, &a.k))) return rc;
+  if ((rc = attn_view(what, "v", v, s->B, s->Tk, s->Hkv, s->D, s->dtype, false, &a.v))) return rc;
+  if ((rc = attn_view(what, "out", out, s->B, s->Tq, s->H, s->D, s->dtype, true, &a.out))) return rc;
+  a.lse = lse_out;
+  if (total_rows(a) == 0) return CTR_OK;
+  if (workspace_bytes < fwd_ws(a) || (!workspace && fwd_ws(a))) {
+    set_error("%s: workspace %zu < %zu", what, workspace_bytes, fwd_ws(a));
+    return CTR_EWORKSPACE;
+  }
+  if (a.splits > 1) {
+    a.part = (float*)align_up((size_t)workspace, 256);
+    a.part_lse = a.part + (size_t)a.splits * total_rows(a) * a.D;
+  }
+  hipStream_t st = (hipStream_t)stream;
+  if (s->dtype == CTR_F32) attn_fwd_launch<float>(a, st);
+  else if (s->dtype == CTR_BF16) attn_fwd_launch<bf16_t>(a, st);
+  else attn_fwd_launch<f16_t>(a, st);
+  CTR_LAUNCH_CHECK();
+  return CTR_OK;
+}
+
+extern "C" int ctr_cross_attn_bwd(const ctr_attn_t* s, const ctr_heads_t* dout, const ctr_heads_t* q,
+                                  const ctr_heads_t* k, const ctr_heads_t* v, const ctr_heads_t* out, const float* lse,
+                                  const ctr_heads_t* dq, const ctr_heads_t* dk, const ctr_heads_t* dv, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  const char* what = "cross_attn_bwd";
+  Attn a;
+  int rc = attn_shape(what, s, &a);
+  if (rc) return rc;
+  if ((rc = attn_view(what, "dout", dout, s->B, s->Tq, s->H, s->D, s->dtype, false, &a.dout))) return rc;
+  if ((rc = attn_view(what, "q", q, s->B, s->Tq, s->H, s->D, s->dtype, false, &a.q))) return rc;
+  if ((rc = attn_view(what, "k", k, s->B, s->Tk, s->Hkv, s->D, s->dtype, false, &a.k))) return rc;
+  if ((rc = attn_view(what, "v", v, s->B, s->Tk, s->Hkv, s->D, s->dtype, false, &a.v))) return rc;
+  if ((rc = attn_view(what, "out", out, s->B, s->Tq, s->H, s->D, s->dtype, false, &a.out))) return rc;
+  if ((rc = attn_view(what, "dq", dq, s->B, s->Tq, s->H, s->D, s->dtype, true, &a.dq))) return rc;
+  if ((rc = attn_view(what, "dk", dk, s->B, s->Tk, s->Hkv, s->D, s->dtype, true, &a.dk))) return rc;
+  if ((rc = attn_view(what, "dv", dv, s->B, s->Tk, s->Hkv, s->D, s->dtype, true, &a.dv))) return rc;
+  CTR_REQUIRE(lse || total_rows(a) == 0, "%s: lse is NULL", what);
+  if (s->B == 0) return CTR_OK;
+  if (!workspace || workspace_bytes < bwd_ws(a)) {
+    set_error("%s: workspace %zu < %zu", what, workspace_bytes, bwd_ws(a));
+    return CTR_EWORKSPACE;
+  }
+  a.lse = const_cast<float*>(lse);
+  a.delta = (float*)align_up((size_t)workspace, 256);
+  a.part = a.delta + align_up((size_t)total_rows(a) * 4, 256) / 4;
+  hipStream_t st = (hipStream_t)stream;
+  if (s->dtype == CTR_F32) attn_bwd_launch<float>(a, st);
+  else if (s->dtype == CTR_BF16) attn_bwd_launch<bf16_t>(a, st);
+  else attn_bwd_launch<f16_t>(a, st);
+  CTR_LAUNCH_CHECK();
+  return CTR_OK;
+}

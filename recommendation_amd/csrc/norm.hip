@@ -1,0 +1,492 @@
+// Layer norm over the last axis of a [rows, cols] view, forward and backward.
+//   mean = sum x / n,  var = sum (x - mean)^2 / n,  rstd = 1 / sqrt(var + eps),  xh = (x - mean) rstd
+//   y = xh gamma + beta
+//   g = dy gamma;  dx = rstd (g - sum g / n - xh sum(g xh) / n);  dgamma = sum_rows dy xh;  dbeta = sum_rows dy
+// Memory bound: the forward reads x and writes y once, the backward reads x and dy and writes dx once.  A row lives in
+// the registers of LPR lanes (16 elements per lane at most), so the two-pass variance costs no second read, and the
+// backward accumulates dgamma / dbeta of its lane's columns over all rows of its block before it writes one partial row
+// per block; a second launch adds those in block order.  Sums are fp32, in a fixed order: results are the same bits on
+// every run.  Rows above 16384 columns are walked in several passes instead.
+#include "types.h"
+
+namespace ctr {
+
+constexpr int LN_LANE_ELEMS = 16;
+constexpr int LN_MAX_COLS = 1024 * LN_LANE_ELEMS;     // a block of 1024 lanes holds the row
+constexpr int LN_STRIP = 64;                          // rows per block of the column sums of wider rows
+
+// sum of v over the LPR lanes of a row; LPR > 64: over the row's waves through LDS (red: one float per wave, reused
+// after the second barrier)
+template <int LPR>
+__device__ static inline float row_sum(float v, float* red) {
+  if constexpr (LPR <= 64) {
+    return group_sum<LPR>(v);
+  } else {
+    constexpr int W = LPR / 64;
+    v = wave_sum(v);
+    const int wave = threadIdx.x >> 6, first = wave / W * W;
+    if ((threadIdx.x & 63) == 0) red[wave] = v;
+    __syncthreads();
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) s += red[first + i];
+    __syncthreads();
+    return s;
+  }
+}
+
+// Row in registers: lane `l` of LPR holds the packets l, l + LPR, ... (NV of them).
+template <class T, int LPR, int NV, int THREADS>
+__global__ __launch_bounds__(THREADS) void ln_fwd_kernel(const T* x, int64_t x_ld, int64_t rows, int cols,
+                                                         const float* __restrict__ gamma,
+                                                         const float* __restrict__ beta, float eps, T* y, int64_t y_ld,
+                                                         float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+  constexpr int V = Packet<T>::V, GPB = THREADS / LPR;
+  __shared__ float red[THREADS / 64];
+  const int l = threadIdx.x % LPR, group = threadIdx.x / LPR;
+  const float inv_n = 1.f / (float)cols;
+  float ga[NV][V], be[NV][V];
+  int have[NV];                                        // elements of packet i inside the row
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (l + i * LPR) * V;
+    have[i] = min(max(cols - c, 0), V);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      ga[i][j] = gamma && j < have[i] ? gamma[c + j] : 1.f;
+      be[i][j] = beta && j < have[i] ? beta[c + j] : 0.f;
+    }
+  }
+  for (int64_t base = (int64_t)blockIdx.x * GPB; base < rows; base += (int64_t)gridDim.x * GPB) {
+    const int64_t row = base + group;
+    const bool active = row < rows;
+    const T* xr = x + (active ? row : 0) * x_ld;
+    float v[NV][V];
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (l + i * LPR) * V;
+      if (have[i] == V) Packet<T>::unpack(packet_load(xr + c), v[i]);
+      else load_part(xr + c, have[i], 0.f, v[i]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) s += v[i][j];
+    }
+    const float mean = row_sum<LPR>(s, red) * inv_n;
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (have[i] == V) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) { v[i][j] -= mean; q = fmaf(v[i][j], v[i][j], q); }
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (j < have[i]) { v[i][j] -= mean; q = fmaf(v[i][j], v[i][j], q); }
+      }
+    }
+    const float var = row_sum<LPR>(q, red) * inv_n;
+    const float rstd = 1.f / sqrtf(var + eps);
+    if (active) {
+      T* yr = y + row * y_ld;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (l + i * LPR) * V;
+        float o[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = fmaf(v[i][j] * rstd, ga[i][j], be[i][j]);
+        if (have[i] == V) packet_store(yr + c, Packet<T>::pack(o));
+        else store_part(yr + c, have[i], o);
+      }
+      if (l == 0) {
+        if (mean_out) mean_out[row] = mean;
+        if (rstd_out) rstd_out[row] = rstd;
+      }
+    }
+  }
+}
+
+// part: [gridDim.x][2][cols], dgamma and dbeta of the block's rows (NULL: not wanted)
+template <class T, int LPR, int NV, int THREADS>
+__global__ __launch_bounds__(THREADS) void ln_bwd_kernel(const T* dy, int64_t dy_ld, const T* x, int64_t x_ld,
+                                                         const float* __restrict__ mean_in,
+                                                         const float* __restrict__ rstd_in, int64_t rows, int cols,
+                                                         const float* __restrict__ gamma, T* dx, int64_t dx_ld, int acc,
+                                                         float* __restrict__ part) {
+  constexpr int V = Packet<T>::V, GPB = THREADS / LPR;
+  __shared__ float red[THREADS / 64];
+  __shared__ float fold[GPB > 1 ? THREADS * NV * V : 1];
+  const int l = threadIdx.x % LPR, group = threadIdx.x / LPR;
+  const float inv_n = 1.f / (float)cols;
+  float ga[NV][V], dg[NV][V], db[NV][V];
+  int have[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (l + i * LPR) * V;
+    have[i] = min(max(cols - c, 0), V);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      ga[i][j] = gamma && j < have[i] ? gamma[c + j] : 1.f;
+      dg[i][j] = db[i][j] = 0.f;
+    }
+  }
+  for (int64_t base = (int64_t)blockIdx.x * GPB; base < rows; base += (int64_t)gridDim.x * GPB) {
+    const int64_t row = base + group;
+    const bool active = row < rows;
+    const T* xr = x + (active ? row : 0) * x_ld;
+    const T* gr = dy + (active ? row : 0) * dy_ld;
+    const float mean = mean_in[active ? row : 0], rstd = rstd_in[active ? row : 0];
+    float xh[NV][V], g[NV][V];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (l + i * LPR) * V;
+      if (have[i] == V) {
+        Packet<T>::unpack(packet_load(xr + c), xh[i]);
+        Packet<T>::unpack(packet_load(gr + c), g[i]);
+      } else {
+        load_part(xr + c, have[i], 0.f, xh[i]);
+        load_part(gr + c, have[i], 0.f, g[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        xh[i][j] = (xh[i][j] - mean) * rstd;
+        if (active) {
+          dg[i][j] = fmaf(g[i][j], xh[i][j], dg[i][j]);
+          db[i][j] += g[i][j];
+        }
+        g[i][j] *= ga[i][j];
+        s1 += g[i][j];
+        s2 = fmaf(g[i][j], xh[i][j], s2);
+      }
+    s1 = row_sum<LPR>(s1, red) * inv_n;
+    s2 = row_sum<LPR>(s2, red) * inv_n;
+    if (active) {
+      T* dr = dx + row * dx_ld;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (l + i * LPR) * V;
+        float o[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = rstd * ((g[i][j] - s1) - xh[i][j] * s2);
+        if (acc) {
+          float old[V];
+          if (have[i] == V) Packet<T>::unpack(packet_load(dr + c), old);
+          else load_part(dr + c, have[i], 0.f, old);
+#pragma unroll
+          for (int j = 0; j < V; ++j) o[j] += old[j];
+        }
+        if (have[i] == V) packet_store(dr + c, Packet<T>::pack(o));
+        else store_part(dr + c, have[i], o);
+      }
+    }
+  }
+  if (!part) return;
+  float* out = part + (int64_t)blockIdx.x * 2 * cols;
+  if constexpr (GPB == 1) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j < have[i]) {
+          out[(l + i * LPR) * V + j] = dg[i][j];
+          out[cols + (l + i * LPR) * V + j] = db[i][j];
+        }
+  } else {
+    constexpr int W = LPR * NV * V;                    // padded row of one group
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) fold[group * W + (l + i * LPR) * V + j] = which ? db[i][j] : dg[i][j];
+      __syncthreads();
+      for (int c = threadIdx.x; c < cols; c += THREADS) {
+        float s = 0.f;
+        for (int k = 0; k < GPB; ++k) s += fold[k * W + c];
+        out[which * cols + c] = s;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// out[c] = sum_b part[b * stride + c]: 16 columns per block, 64 threads per column, folded through LDS in a fixed order
+__global__ __launch_bounds__(1024) void ln_fold_kernel(const float* __restrict__ part, int blocks, int cols,
+                                                       float* __restrict__ dgamma, float* __restrict__ dbeta) {
+  __shared__ float red[64][17];
+  const int c16 = threadIdx.x & 15, r = threadIdx.x >> 4;
+  const int c = blockIdx.x * 16 + c16;
+  float* out = blockIdx.y ? dbeta : dgamma;
+  const float* p = part + (blockIdx.y ? cols : 0) + c;
+  float s = 0.f;
+  if (c < cols)
+    for (int b = r; b < blocks; b += 64) s += p[(int64_t)b * 2 * cols];
+  red[r][c16] = s;
+  __syncthreads();
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    if (r < o) red[r][c16] += red[r + o][c16];
+    __syncthreads();
+  }
+  if (r == 0 && c < cols && out) out[c] = red[0][c16];
+}
+
+// ---- rows wider than LN_MAX_COLS: a block walks its row once per sum (the re-reads come from the caches) -----------
+template <class T>
+__device__ static inline void wide_load(const T* p, int c, int cols, float fill, float* f) {
+  if (c + Packet<T>::V <= cols) Packet<T>::unpack(packet_load(p + c), f);
+  else load_part(p + c, cols - c, fill, f);
+}
+
+template <class T>
+__global__ __launch_bounds__(1024) void ln_fwd_wide_kernel(const T* x, int64_t x_ld, int64_t rows, int cols,
+                                                           const float* __restrict__ gamma,
+                                                           const float* __restrict__ beta, float eps, T* y,
+                                                           int64_t y_ld, float* __restrict__ mean_out,
+                                                           float* __restrict__ rstd_out) {
+  constexpr int V = Packet<T>::V, STEP = 1024 * V;
+  __shared__ float red[16];
+  const float inv_n = 1.f / (float)cols;
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const T* xr = x + row * x_ld;
+    T* yr = y + row * y_ld;
+    float f[V], s = 0.f, q = 0.f;
+    for (int c = threadIdx.x * V; c < cols; c += STEP) {
+      wide_load(xr, c, cols, 0.f, f);
+#pragma unroll
+      for (int j = 0; j < V; ++j) s += f[j];
+    }
+    const float mean = row_sum<1024>(s, red) * inv_n;
+    for (int c = threadIdx.x * V; c < cols; c += STEP) {
+      wide_load(xr, c, cols, mean, f);
+#pragma unroll
+      for (int j = 0; j < V; ++j) q = fmaf(f[j] - mean, f[j] - mean, q);
+    }
+    const float rstd = 1.f / sqrtf(row_sum<1024>(q, red) * inv_n + eps);
+    for (int c = threadIdx.x * V; c < cols; c += STEP) {
+      wide_load(xr, c, cols, 0.f, f);
+      const int n = min(V, cols - c);
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j < n) f[j] = fmaf((f[j] - mean) * rstd, gamma ? gamma[c + j] : 1.f, beta ? beta[c + j] : 0.f);
+      if (n == V) packet_store(yr + c, Packet<T>::pack(f));
+      else store_part(yr + c, n, f);
+    }
+    if (threadIdx.x == 0) {
+      if (mean_out) mean_out[row] = mean;
+      if (rstd_out) rstd_out[row] = rstd;
+    }
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(1024) void ln_dx_wide_kernel(const T* dy, int64_t dy_ld, const T* x, int64_t x_ld,
+                                                          const float* __restrict__ mean_in,
+                                                          const float* __restrict__ rstd_in, int64_t rows, int cols,
+                                                          const float* __restrict__ gamma, T* dx, int64_t dx_ld,
+                                                          int acc) {
+  constexpr int V = Packet<T>::V, STEP = 1024 * V;
+  __shared__ float red[16];
+  const float inv_n = 1.f / (float)cols;
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const T* xr = x + row * x_ld;
+    const T* gr = dy + row * dy_ld;
+    T* dr = dx + row * dx_ld;
+    const float mean = mean_in[row], rstd = rstd_in[row];
+    float f[V], g[V], old[V], s1 = 0.f, s2 = 0.f;
+    for (int c = threadIdx.x * V; c < cols; c += STEP) {
+      wide_load(xr, c, cols, 0.f, f);
+      wide_load(gr, c, cols, 0.f, g);
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (c + j < cols) {
+          const float h = g[j] * (gamma ? gamma[c + j] : 1.f);
+          s1 += h;
+          s2 = fmaf(h, (f[j] - mean) * rstd, s2);
+        }
+    }
+    s1 = row_sum<1024>(s1, red) * inv_n;
+    s2 = row_sum<1024>(s2, red) * inv_n;
+    for (int c = threadIdx.x * V; c < cols; c += STEP) {
+      const int n = min(V, cols - c);
+      wide_load(xr, c, cols, 0.f, f);
+      wide_load(gr, c, cols, 0.f, g);
+      if (acc) wide_load(dr, c, cols, 0.f, old);
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j < n) {
+          const float h = g[j] * (gamma ? gamma[c + j] : 1.f);
+          f[j] = rstd * ((h - s1) - (f[j] - mean) * rstd * s2) + (acc ? old[j] : 0.f);
+        }
+      if (n == V) packet_store(dr + c, Packet<T>::pack(f));
+      else store_part(dr + c, n, f);
+    }
+  }
+}
+
+// dgamma / dbeta of LN_STRIP rows x 256 columns per block
+template <class T>
+__global__ __launch_bounds__(256) void ln_cols_wide_kernel(const T* dy, int64_t dy_ld, const T* x, int64_t x_ld,
+                                                           const float* __restrict__ mean_in,
+                                                           const float* __restrict__ rstd_in, int64_t rows, int cols,
+                                                           int strip, float* __restrict__ part) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= cols) return;
+  float dg = 0.f, db = 0.f;
+  const int64_t r0 = (int64_t)blockIdx.y * strip, r1 = min(rows, r0 + strip);
+  for (int64_t r = r0; r < r1; ++r) {
+    const float g = (float)dy[r * dy_ld + c];
+    dg = fmaf(g, ((float)x[r * x_ld + c] - mean_in[r]) * rstd_in[r], dg);
+    db += g;
+  }
+  float* out = part + (int64_t)blockIdx.y * 2 * cols;
+  out[c] = dg;
+  out[cols + c] = db;
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------
+// Blocks of the backward: every block ends with one partial row of 2 cols floats, so wide rows take fewer, larger blocks.
+static int ln_bwd_blocks(int64_t rows, int gpb, int threads) {
+  const int64_t need = cdiv(rows, gpb);
+  const int64_t cap = threads == 256 ? 1024 : 256;
+  return (int)(need < cap ? (need < 1 ? 1 : need) : cap);
+}
+// Column sums of wider rows: strips of LN_STRIP rows, longer ones when that would make more than 256 (rows >= 1).
+static int ln_wide_strip(int64_t rows) { return (int)(rows <= 256 * LN_STRIP ? LN_STRIP : cdiv(rows, 256)); }
+static int ln_wide_strips(int64_t rows) { return (int)cdiv(rows, ln_wide_strip(rows)); }
+
+struct LnShape { int lpr, nv, threads; };
+// The fewest lanes that hold the row at one packet per lane; from a whole wave on, up to 16 elements per lane, then
+// four rows to a block of 1024 lanes, then one.
+template <class T>
+static LnShape ln_shape(int cols) {
+  constexpr int V = Packet<T>::V, NVMAX = LN_LANE_ELEMS / V;
+  for (int lpr = 2; lpr <= 64; lpr *= 2)
+    if (cols <= lpr * V) return {lpr, 1, 256};
+  if (cols <= 64 * 2 * V) return {64, 2, 256};
+  if (cols <= 64 * NVMAX * V) return {64, NVMAX, 256};
+  if (cols <= 256 * NVMAX * V) return {256, NVMAX, 1024};
+  return {1024, NVMAX, 1024};
+}
+
+#define LN_DISPATCH(T, CALL)                                          \
+  do {                                                                \
+    constexpr int NVMAX = LN_LANE_ELEMS / Packet<T>::V;               \
+    const LnShape sh = ln_shape<T>(cols);                             \
+    if (sh.lpr == 2) { CALL(T, 2, 1, 256); }                          \
+    else if (sh.lpr == 4) { CALL(T, 4, 1, 256); }                     \
+    else if (sh.lpr == 8) { CALL(T, 8, 1, 256); }                     \
+    else if (sh.lpr == 16) { CALL(T, 16, 1, 256); }                   \
+    else if (sh.lpr == 32) { CALL(T, 32, 1, 256); }                   \
+    else if (sh.lpr == 64 && sh.nv == 1) { CALL(T, 64, 1, 256); }     \
+    else if (sh.lpr == 64 && sh.nv == 2) { CALL(T, 64, 2, 256); }     \
+    else if (sh.lpr == 64) { CALL(T, 64, NVMAX, 256); }               \
+    else if (sh.lpr == 256) { CALL(T, 256, NVMAX, 1024); }            \
+    else { CALL(T, 1024, NVMAX, 1024); }                              \
+  } while (0)
+
+template <class T>
+static void ln_fwd_launch(const T* x, int64_t x_ld, int64_t rows, int cols, const float* gamma, const float* beta,
+                          float eps, T* y, int64_t y_ld, float* mean, float* rstd, hipStream_t st) {
+  if (cols > LN_MAX_COLS) {
+    ln_fwd_wide_kernel<T><<<(int)(rows < 2048 ? rows : 2048), 1024, 0, st>>>(x, x_ld, rows, cols, gamma, beta, eps, y,
+                                                                            y_ld, mean, rstd);
+    return;
+  }
+#define LN_FWD(T_, LPR_, NV_, TH_)                                                                               \
+  do {                                                                                                           \
+    const int64_t need = cdiv(rows, TH_ / LPR_), cap = TH_ == 256 ? 2048 : 512;                                  \
+    ln_fwd_kernel<T_, LPR_, NV_, TH_><<<(int)(need < cap ? need : cap), TH_, 0, st>>>(x, x_ld, rows, cols, gamma, \
+                                                                                     beta, eps, y, y_ld, mean, rstd); \
+  } while (0)
+  LN_DISPATCH(T, LN_FWD);
+#undef LN_FWD
+}
+
+template <class T>
+static void ln_bwd_launch(const T* dy, int64_t dy_ld, const T* x, int64_t x_ld, const float* mean, const float* rstd,
+                          int64_t rows, int cols, const float* gamma, T* dx, int64_t dx_ld, int acc, float* dgamma,
+                          float* dbeta, float* ws, hipStream_t st) {
+  const bool sums = dgamma || dbeta;
+  float* part = sums ? ws : nullptr;
+  int blocks = 0;
+  if (rows > 0 && cols > LN_MAX_COLS) {
+    if (part) {
+      blocks = ln_wide_strips(rows);
+      ln_cols_wide_kernel<T><<<dim3((unsigned)cdiv(cols, 256), blocks), 256, 0, st>>>(dy, dy_ld, x, x_ld, mean, rstd,
+                                                                                     rows, cols, ln_wide_strip(rows), part);
+    }
+    ln_dx_wide_kernel<T><<<(int)(rows < 2048 ? rows : 2048), 1024, 0, st>>>(dy, dy_ld, x, x_ld, mean, rstd, rows, cols,
+                                                                           gamma, dx, dx_ld, acc);
+  } else if (rows > 0) {
+#define LN_BWD(T_, LPR_, NV_, TH_)                                                                                   \
+  do {                                                                                                               \
+    blocks = ln_bwd_blocks(rows, TH_ / LPR_, TH_);                                                             \
+    ln_bwd_kernel<T_, LPR_, NV_, TH_><<<blocks, TH_, 0, st>>>(dy, dy_ld, x, x_ld, mean, rstd, rows, cols, gamma, dx, \
+                                                             dx_ld, acc, part);                                      \
+  } while (0)
+    LN_DISPATCH(T, LN_BWD);
+#undef LN_BWD
+  }
+  if (sums)                                            // without rows: zeros
+    ln_fold_kernel<<<dim3((unsigned)cdiv(cols, 16), 2), 1024, 0, st>>>(part, blocks, cols, dgamma, dbeta);
+}
+
+static size_t ln_bwd_ws(int64_t rows, int cols) {
+  if (rows < 1 || cols < 1) return 0;
+  int64_t b = cols > LN_MAX_COLS ? ln_wide_strips(rows) : (rows < 1024 ? rows : 1024);
+  return (size_t)b * 2 * cols * sizeof(float);
+}
+
+}  // namespace ctr
+
+using namespace ctr;
+
+extern "C" int ctr_layer_norm_fwd(const void* x, int64_t x_ld, int64_t rows, int cols, int dtype, const float* gamma,
+                                  const float* beta, float eps, void* y, int64_t y_ld, float* mean_out, float* rstd_out,
+                                  void* stream) {
+  CTR_REQUIRE(rows >= 0 && cols >= 1, "layer_norm_fwd: rows %lld cols %d", (long long)rows, cols);
+  CTR_REQUIRE(type_bytes(dtype) != 0, "layer_norm_fwd: unknown dtype %d", dtype);
+  CTR_REQUIRE(eps >= 0.f, "layer_norm_fwd: eps must not be negative");
+  if (rows == 0) return CTR_OK;
+  CTR_REQUIRE(x && y && x_ld >= cols && y_ld >= cols, "layer_norm_fwd: missing x / y or a leading dimension below cols");
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == CTR_F32) ln_fwd_launch((const float*)x, x_ld, rows, cols, gamma, beta, eps, (float*)y, y_ld, mean_out, rstd_out, st);
+  else if (dtype == CTR_BF16) ln_fwd_launch((const bf16_t*)x, x_ld, rows, cols, gamma, beta, eps, (bf16_t*)y, y_ld, mean_out, rstd_out, st);
+  else ln_fwd_launch((const f16_t*)x, x_ld, rows, cols, gamma, beta, eps, (f16_t*)y, y_ld, mean_out, rstd_out, st);
+  CTR_LAUNCH_CHECK();
+  return CTR_OK;
+}
+
+extern "C" size_t ctr_layer_norm_bwd_workspace_bytes(int64_t rows, int cols) { return ln_bwd_ws(rows, cols); }
+
+extern "C" int ctr_layer_norm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, const float* mean,
+                                  const float* rstd, int64_t rows, int cols, int dtype, const float* gamma, void* dx,
+                                  int64_t dx_ld, int accumulate_dx, float* dgamma, float* dbeta, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  CTR_REQUIRE(rows >= 0 && cols >= 1, "layer_norm_bwd: rows %lld cols %d", (long long)rows, cols);
+  CTR_REQUIRE(type_bytes(dtype) != 0, "layer_norm_bwd: unknown dtype %d", dtype);
+  CTR_REQUIRE(rows == 0 || (dy && x && mean && rstd && dx && dy_ld >= cols && x_ld >= cols && dx_ld >= cols),
+              "layer_norm_bwd: missing tensor or a leading dimension below cols");
+  if ((dgamma || dbeta) && (workspace_bytes < ln_bwd_ws(rows, cols) || (!workspace && rows > 0))) {
+    set_error("layer_norm_bwd: workspace %zu < %zu", workspace_bytes, ln_bwd_ws(rows, cols));
+    return CTR_EWORKSPACE;
+  }
+  if (rows == 0 && !dgamma && !dbeta) return CTR_OK;
+  hipStream_t st = (hipStream_t)stream;
+  float* ws = (float*)workspace;
+  if (dtype == CTR_F32)
+    ln_bwd_launch((const float*)dy, dy_ld, (const float*)x, x_ld, mean, rstd, rows, cols, gamma, (float*)dx, dx_ld,
+                  accumulate_dx, dgamma, dbeta, ws, st);
+  else if (dtype == CTR_BF16)
+    ln_bwd_launch((const bf16_t*)dy, dy_ld, (const bf16_t*)x, x_ld, mean, rstd, rows, cols, gamma, (bf16_t*)dx, dx_ld,
+                  accumulate_dx, dgamma, dbeta, ws, st);
+  else
+    ln_bwd_launch((const f16_t*)dy, dy_ld, (const f16_t*)x, x_ld, mean, rstd, rows, cols, gamma, (f16_t*)dx, dx_ld,
+                  accumulate_dx, dgamma, dbeta, ws, st);
+  CTR_LAUNCH_CHECK();
+  return CTR_OK;
+}

@@ -12,7 +12,7 @@ import math
 import torch
 
 from . import _lib
-from ._lib import Dropout, Epilogue, FmBwd, Opt, check
+from ._lib import AttnShape, Dropout, Epilogue, FmBwd, Heads, Opt, check
 
 KEEP_ONE = 1 << 24
 
@@ -1199,3 +1199,270 @@ def mean_positive_diff(a, b, out):
         raise ValueError('mean_positive_diff size mismatch')
     check(lib().ctr_mean_positive_diff(_ptr(a, f32), _ptr(b, f32), n, _ptr(out, f32), _stream()),
           'ctr_mean_positive_diff')
+
+
+# ------------------------------------------------------------------ attention towers over behaviour sequences
+DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _dtype(t, name):
+    if t.dtype not in DTYPES:
+        raise TypeError('%s: expected float32, bfloat16 or float16, got %s' % (name, t.dtype))
+    return DTYPES[t.dtype]
+
+
+def _here(*named):
+    """Every tensor on the current device: the kernels run on its current stream."""
+    dev = None
+    for t, name in named:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError('%s must live on the GPU (libctrhip has no CPU path)' % name)
+        if dev is None:
+            dev = torch.cuda.current_device()
+        if t.device.index != dev:
+            raise ValueError('%s lives on %s, the current device is cuda:%d' % (name, t.device, dev))
+
+
+def _heads(t, shape, dtype, name):
+    if tuple(t.shape) != shape:
+        raise ValueError('%s must be %s, got %s' % (name, list(shape), list(t.shape)))
+    if t.dtype != dtype:
+        raise TypeError('%s: expected %s, got %s' % (name, dtype, t.dtype))
+    sb, st, sh, sd = t.stride()
+    if sd != 1:
+        raise ValueError('%s must have a contiguous last dimension' % name)
+    return Heads(t.data_ptr(), sb if shape[0] > 1 else 0, st if shape[1] > 1 else 0, sh if shape[2] > 1 else 0)
+
+
+def _attn_args(q, k, v, sl, mask, scale):
+    """(shape struct, q's shape, k's shape) of a cross-attention call, checked."""
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError('q must be [B, Tq, H, D] and k [B, Tk, Hkv, D]')
+    qs, ks = tuple(q.shape), tuple(k.shape)
+    if ks[0] != qs[0] or ks[3] != qs[3] or ks[2] < 1 or qs[2] < 1 or qs[2] % ks[2]:
+        raise ValueError('q %s and k %s do not belong together (one batch, one head size, H a multiple of Hkv)'
+                         % (list(qs), list(ks)))
+    B, Tk, D = qs[0], ks[1], qs[3]
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError('head size %d is not a multiple of 8 up to 128' % D)
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not 0.0 < scale <= 3e38:
+        raise ValueError('scale must be positive and finite')
+    mp, mld = None, 0
+    if mask is not None:
+        if mask.dtype not in (torch.bool, torch.uint8):
+            raise TypeError('mask: expected bool or uint8, got %s' % mask.dtype)
+        if tuple(mask.shape) != (B, Tk) or (Tk > 1 and mask.stride(1) != 1):
+            raise ValueError('mask must be [B, Tk] with a contiguous last dimension')
+        mp, mld = mask.data_ptr(), mask.stride(0) if B > 1 else 0
+    sp = None
+    if sl is not None:
+        if sl.dtype != torch.int32 or tuple(sl.shape) != (B,) or not sl.is_contiguous():
+            raise ValueError('sl must be a contiguous int32 [B] tensor')
+        sp = sl.data_ptr()
+    return AttnShape(B, qs[1], Tk, qs[2], ks[2], D, _dtype(q, 'q'), scale, sp, mp, mld), qs, ks
+
+
+def _lse(lse, qs):
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (qs[0], qs[2], qs[1]) or not lse.is_contiguous():
+        raise ValueError('lse must be contiguous float32 [B, H, Tq]')
+    return C.c_void_p(lse.data_ptr())
+
+
+def _apart(outs, ins):
+    """No output starts where another tensor of the call does (views that merely share a buffer are fine)."""
+    seen = {t.data_ptr(): name for t, name in ins if t.numel()}
+    for t, name in outs:
+        if t.numel():
+            if t.data_ptr() in seen:
+                raise ValueError('%s shares its memory with %s' % (name, seen[t.data_ptr()]))
+            seen[t.data_ptr()] = name
+
+
+@_timed
+def cross_attn_fwd(q, k, v, out, *, lse=None, sl=None, mask=None, scale=None, ws):
+    """out[b,i,h] = softmax(scale q[b,i,h] . k[b,:,h']) v[b,:,h'], h' = h // (H / Hkv): every query row attends to the
+    states of another sequence.  q, out [B,Tq,H,D], k, v [B,Tk,Hkv,D] in float32, bfloat16 or float16 (D a multiple of 8
+    up to 128, rows on 16-byte boundaries, other strides free).  sl (int32 [B]): only the first sl[b] keys; mask (bool or
+    uint8 [B,Tk]): only the keys that are set.  A row without keys gives zeros.  scale: 1 / sqrt(D) by default.
+    lse (float32 [B,H,Tq]): the logarithm of every softmax's sum, kept for cross_attn_bwd."""
+    sh, qs, ks = _attn_args(q, k, v, sl, mask, scale)
+    hq, hk, hv = _heads(q, qs, q.dtype, 'q'), _heads(k, ks, q.dtype, 'k'), _heads(v, ks, q.dtype, 'v')
+    ho = _heads(out, qs, q.dtype, 'out')
+    lp = None if lse is None else _lse(lse, qs)
+    _apart(((out, 'out'),), ((q, 'q'), (k, 'k'), (v, 'v')))
+    _here((q, 'q'), (k, 'k'), (v, 'v'), (out, 'out'), (lse, 'lse'), (sl, 'sl'), (mask, 'mask'))
+    L, r = lib(), C.byref
+    wp, wn = ws.get(L.ctr_cross_attn_fwd_workspace_bytes(r(sh)))
+    check(L.ctr_cross_attn_fwd(r(sh), r(hq), r(hk), r(hv), r(ho), lp, wp, wn, _stream()), 'ctr_cross_attn_fwd')
+
+
+@_timed
+def cross_attn_bwd(dout, q, k, v, out, lse, dq, dk, dv, *, sl=None, mask=None, scale=None, ws):
+    """Gradients of cross_attn_fwd from its own inputs, out and lse (the same sl, mask and scale).  dq, dk and dv are
+    overwritten; keys that no row attends to get zeros; heads that share keys add up in dk and dv."""
+    sh, qs, ks = _attn_args(q, k, v, sl, mask, scale)
+    t = q.dtype
+    hg, hq, hk, hv = _heads(dout, qs, t, 'dout'), _heads(q, qs, t, 'q'), _heads(k, ks, t, 'k'), _heads(v, ks, t, 'v')
+    ho, gq, gk, gv = _heads(out, qs, t, 'out'), _heads(dq, qs, t, 'dq'), _heads(dk, ks, t, 'dk'), _heads(dv, ks, t, 'dv')
+    lp = _lse(lse, qs)
+    _apart(((dq, 'dq'), (dk, 'dk'), (dv, 'dv')), ((dout, 'dout'), (q, 'q'), (k, 'k'), (v, 'v'), (out, 'out')))
+    _here((dout, 'dout'), (q, 'q'), (k, 'k'), (v, 'v'), (out, 'out'), (lse, 'lse'), (dq, 'dq'), (dk, 'dk'), (dv, 'dv'),
+          (sl, 'sl'), (mask, 'mask'))
+    L, r = lib(), C.byref
+    wp, wn = ws.get(L.ctr_cross_attn_bwd_workspace_bytes(r(sh)))
+    check(L.ctr_cross_attn_bwd(r(sh), r(hg), r(hq), r(hk), r(hv), r(ho), lp, r(gq), r(gk), r(gv), wp, wn, _stream()),
+          'ctr_cross_attn_bwd')
+
+
+def _ln_rows(t, shape, dtype, name):
+    if t.dim() != 2 or tuple(t.shape) != shape:
+        raise ValueError('%s must be %s, got %s' % (name, list(shape), list(t.shape)))
+    if t.dtype != dtype:
+        raise TypeError('%s: expected %s, got %s' % (name, dtype, t.dtype))
+    if t.stride(1) != 1 and shape[1] > 1 or (shape[0] > 1 and t.stride(0) < shape[1]):
+        raise ValueError('%s must have a contiguous last dimension and rows that do not overlap' % name)
+    return C.c_void_p(t.data_ptr()), int(t.stride(0)) if shape[0] > 1 else shape[1]
+
+
+def _ln_vec(t, n, name):
+    if t is None:
+        return None
+    if t.dtype != torch.float32:
+        raise TypeError('%s: expected torch.float32, got %s' % (name, t.dtype))
+    if t.numel() != n or not t.is_contiguous():
+        raise ValueError('%s must be contiguous with %d entries' % (name, n))
+    return C.c_void_p(t.data_ptr())
+
+
+def _ln_shape(x):
+    if x.dim() != 2 or x.shape[1] < 1 or x.shape[1] >= 1 << 30:
+        raise ValueError('layer norm wants a [rows, cols] view with at least one column')
+    return tuple(x.shape)
+
+
+@_timed
+def layer_norm_fwd(x, y, *, gamma=None, beta=None, eps=1e-5, mean=None, rstd=None):
+    """y = (x - mean) rstd gamma + beta over the columns of x [rows, cols] (float32, bfloat16 or float16; any row
+    stride).  gamma, beta: float32 [cols] or None; mean, rstd: float32 [rows], kept for layer_norm_bwd.  y may be x."""
+    rows, cols = shape = _ln_shape(x)
+    dt = _dtype(x, 'x')
+    if not 0.0 <= eps < float('inf'):
+        raise ValueError('eps must be finite and not negative')
+    (xp, xld), (yp, yld) = _ln_rows(x, shape, x.dtype, 'x'), _ln_rows(y, shape, x.dtype, 'y')
+    ga, be = _ln_vec(gamma, cols, 'gamma'), _ln_vec(beta, cols, 'beta')
+    mp, rp = _ln_vec(mean, rows, 'mean'), _ln_vec(rstd, rows, 'rstd')
+    _here((x, 'x'), (y, 'y'), (gamma, 'gamma'), (beta, 'beta'), (mean, 'mean'), (rstd, 'rstd'))
+    check(lib().ctr_layer_norm_fwd(xp, xld, rows, cols, dt, ga, be, float(eps), yp, yld, mp, rp, _stream()),
+          'ctr_layer_norm_fwd')
+
+
+@_timed
+def layer_norm_bwd(dy, x, mean, rstd, dx, *, gamma=None, dgamma=None, dbeta=None, accumulate=False, ws):
+    """dx, dgamma and dbeta of layer_norm_fwd from its x, mean and rstd.  accumulate: dx is added to what it holds (the
+    gradient that the residual branch left there).  dx may be dy or x."""
+    rows, cols = shape = _ln_shape(x)
+    dt = _dtype(x, 'x')
+    (gp, gld), (xp, xld) = _ln_rows(dy, shape, x.dtype, 'dy'), _ln_rows(x, shape, x.dtype, 'x')
+    dp, dld = _ln_rows(dx, shape, x.dtype, 'dx')
+    if mean is None or rstd is None:
+        raise ValueError('layer_norm_bwd needs the mean and rstd that layer_norm_fwd kept')
+    mp, rp, ga = _ln_vec(mean, rows, 'mean'), _ln_vec(rstd, rows, 'rstd'), _ln_vec(gamma, cols, 'gamma')
+    dg, db = _ln_vec(dgamma, cols, 'dgamma'), _ln_vec(dbeta, cols, 'dbeta')
+    _here((dy, 'dy'), (x, 'x'), (mean, 'mean'), (rstd, 'rstd'), (dx, 'dx'), (gamma, 'gamma'), (dgamma, 'dgamma'),
+          (dbeta, 'dbeta'))
+    wp, wn = None, 0
+    if dgamma is not None or dbeta is not None:
+        wp, wn = ws.get(lib().ctr_layer_norm_bwd_workspace_bytes(rows, cols))
+    check(lib().ctr_layer_norm_bwd(gp, gld, xp, xld, mp, rp, rows, cols, dt, ga, dp, dld, int(bool(accumulate)), dg, db,
+                                   wp, wn, _stream()), 'ctr_layer_norm_bwd')
+
+
+class GradList:
+    """The gradient tensors of a model (float32, bfloat16 and float16, contiguous, of any size), as grad_norm and
+    clip_grads take them.  Made once for buffers that stay; it holds the tensors' memory alive."""
+
+    def __init__(self, tensors):
+        self.tensors = list(tensors)
+        n = len(self.tensors)
+        for i, t in enumerate(self.tensors):
+            _dtype(t, 'tensor %d' % i)
+            if not t.is_contiguous():
+                raise ValueError('tensor %d must be contiguous' % i)
+        self.storages = [t.untyped_storage() for t in self.tensors]
+        self.ptrs = (C.c_void_p * n)(*[t.data_ptr() for t in self.tensors])
+        self.counts = (C.c_int64 * n)(*[t.numel() for t in self.tensors])
+        self.dtypes = (C.c_int * n)(*[DTYPES[t.dtype] for t in self.tensors])
+        self.kinds = [(t.numel(), t.dtype) for t in self.tensors]
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), i)
+                       for i, t in enumerate(self.tensors) if t.numel())
+        for (_, end, i), (start, _, j) in zip(spans, spans[1:]):
+            if start < end:
+                raise ValueError('tensors %d and %d share memory' % (i, j))
+        self.begins = torch.tensor([s[0] for s in spans], dtype=torch.int64).numpy()
+        self.ends = torch.tensor([s[1] for s in spans], dtype=torch.int64).numpy()
+        self.device = None
+        for i, t in enumerate(self.tensors):
+            if not t.is_cuda:
+                raise ValueError('tensor %d must live on the GPU (libctrhip has no CPU path)' % i)
+            if self.device is None:
+                self.device = t.device.index
+            elif t.device.index != self.device:
+                raise ValueError('tensor %d lives on %s, the others on cuda:%d' % (i, t.device, self.device))
+
+    def __len__(self):
+        return len(self.tensors)
+
+    def overlaps(self, other):
+        """Whether a tensor of this list shares memory with one of the other."""
+        at = other.begins.searchsorted(self.ends)      # spans of the other that begin before this one ends
+        return bool(((at > 0) & (other.ends.take(at - 1, mode='clip') > self.begins)).any()) if len(other.begins) else False
+
+
+def _grad_list(grads):
+    g = grads if isinstance(grads, GradList) else GradList(grads)
+    if g.device is not None and g.device != torch.cuda.current_device():
+        raise ValueError('the gradients live on cuda:%d, the current device is cuda:%d'
+                         % (g.device, torch.cuda.current_device()))
+    return g
+
+
+def _norm_ptr(norm):
+    if norm is None:
+        return None
+    if norm.dtype != torch.float32 or norm.numel() != 1:
+        raise ValueError('norm must be a float32 tensor of one element')
+    _here((norm, 'norm'))
+    return C.c_void_p(norm.data_ptr())
+
+
+@_timed
+def grad_norm(grads, norm, *, ws):
+    """norm[0] = the square root of the sum of all squares over a GradList (or a list of tensors), summed in fp64."""
+    g = _grad_list(grads)
+    if norm is None:
+        raise ValueError('grad_norm needs a norm tensor')
+    wp, wn = ws.get(lib().ctr_grad_norm_workspace_bytes(len(g)))
+    check(lib().ctr_grad_norm(g.ptrs, g.counts, g.dtypes, len(g), _norm_ptr(norm), wp, wn, _stream()), 'ctr_grad_norm')
+
+
+@_timed
+def clip_grads(grads, max_norm, norm=None, *, out=None, ws):
+    """tf.clip_by_global_norm: out = g * max_norm / max(norm, max_norm) over a GradList (or a list of tensors), in place
+    without `out`; norm (float32 [1], optional) receives the norm before clipping.  A norm that is not finite makes every
+    result NaN.  In place, nothing is written when the norm is within the bound."""
+    g = _grad_list(grads)
+    max_norm = float(max_norm)
+    if not 0.0 < max_norm <= 3e38:
+        raise ValueError('max_norm must be positive and finite')
+    o = g if out is None else _grad_list(out)
+    if o is not g:
+        if o.kinds != g.kinds:
+            raise ValueError('out must hold tensors of the same sizes and dtypes')
+        if list(o.ptrs) != list(g.ptrs) and o.overlaps(g):
+            raise ValueError('out shares memory with the gradients without being them')
+    wp, wn = ws.get(lib().ctr_grad_norm_workspace_bytes(len(g)))
+    check(lib().ctr_clip_grads(g.ptrs, o.ptrs, g.counts, g.dtypes, len(g), max_norm, _norm_ptr(norm), wp, wn, _stream()),
+          'ctr_clip_grads')
