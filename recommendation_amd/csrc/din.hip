@@ -239,6 +239,9 @@ __global__ __launch_bounds__(256) void din_attn_pool_bwd_kernel(const float* __r
     dot += att[b * T + t] * da;
   }
   dot = wave_sum(dot);
+  float rest = 0.f;                    // the weights add up to one: what is left of dot's own rounding (see the block kernel)
+  for (int t = lane; t < T; t += 64) rest += att[b * T + t] * (dscore[b * T + t] - dot);
+  dot += wave_sum(rest);
   for (int t = lane; t < T; t += 64) {
     const float a = att[b * T + t];
     const float da = dscore[b * T + t];
@@ -286,6 +289,12 @@ __global__ __launch_bounds__(256) void din_attn_pool_bwd_block_kernel(const floa
     dot += a * da;
   }
   dot = block_sum256(dot, red4);
+  // The gradients behind dscore (the scoring network's biases above all) are sums over all positions of terms that
+  // nearly cancel, since dscore adds up to zero: dot's rounding error is the same for every position and would be what
+  // is left.  The weights add up to one, so sum_t att (datt - dot) is that error, and it is put back.
+  float rest = 0.f;
+  for (int t = threadIdx.x; t < T; t += 256) rest += att_s[t] * (dscore[b * T + t] - dot);
+  dot += block_sum256(rest, red4);
   for (int t = threadIdx.x; t < T; t += 256) {
     const float da = dscore[b * T + t];
     dscore[b * T + t] = t < len ? att_s[t] * (da - dot) * inv : 0.f;
