@@ -178,6 +178,9 @@ struct Attn {
   float scale, scale2;                                 // scale2 = scale * log2(e)
   int rows, row_tiles, key_tiles, splits, per_split;
   float *part, *part_lse;                              // [splits][B H Tq][D], [splits][B H Tq]
+  float* kept;                                         // few rows: p, then dp, [B Hkv][Tk][R]
+  int few, waves, lanes;                               // rows padded to 1, 2 or 4 (0: the tiled kernels); waves per
+                                                       // block, lanes per key
 };
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -707,7 +710,404 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(Attn a, int64_t n_rows) {
   for (int j = 0; j < 4; ++j) dst[j] = (T)acc[j];
 }
 
+// ---- few query rows --------------------------------------------------------------------------------------------------
+// One to four rows per (sample, key head): a candidate per user, a decoded token.  Nothing to tile, the keys and values
+// are read once and that is the time: LPK lanes hold a key (16 bytes each), a wave 64 / LPK keys per step and ROW_STEP
+// steps in flight; products on the vector units, in fp32 throughout (p and ds are not rounded).  Every group of LPK lanes
+// keeps a running softmax of its own; they are joined at the end, over lanes, waves (LDS) and splits (a second launch).
+// The backward needs no `out`: pass one reads k and v, keeps p and dp = dout v^T per key and sums
+//   delta = sum p dp,  A = sum p dp k,  S = sum p k   (dq = scale (A - delta S)),
+// pass two writes dk = scale p (dp - delta) q and dv = p dout from the kept numbers: k and v are read once, delta is
+// the exact row sum.  While p and dp fit the LDS of one block the two passes are one launch.
+constexpr int ROW_STEP = 4;
+constexpr int ROWS_LDS = 4096;                         // (key, row) pairs whose p and dp a block keeps in LDS
+
+template <int LPK>
+__device__ static inline float slot_sum(float v) {
+#pragma unroll
+  for (int o = LPK; o < 64; o <<= 1) v += __shfl_xor(v, o);
+  return v;
+}
+template <int LPK>
+__device__ static inline float slot_max(float v) {
+#pragma unroll
+  for (int o = LPK; o < 64; o <<= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
+template <class T>
+__device__ static inline void packet_floats(const T* p, bool ok, float* f) {
+  Packet<T>::unpack(ok ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0), f);
+}
+
+struct PairAt { int split, b, hk, k0, k1; };
+__device__ static inline PairAt pair_at(const Attn& a) {
+  PairAt p;
+  const int id = die_order(blockIdx.x, gridDim.x);
+  p.split = id % a.splits;
+  const int pair = id / a.splits;
+  p.b = pair / a.Hkv;
+  p.hk = pair - p.b * a.Hkv;
+  p.k0 = p.split * a.per_split;
+  p.k1 = min(key_count(a, p.b), p.k0 + a.per_split);
+  return p;
+}
+
+template <class T, int R, int LPK, int NW>
+__global__ __launch_bounds__(NW * 64) void attn_rows_fwd_kernel(Attn a) {
+  constexpr int V = Packet<T>::V, KPW = 64 / LPK, U = ROW_STEP;
+  __shared__ float sm[NW > 1 ? NW * R * (LPK * V + 2) : 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LPK, slot = lane / LPK, d = sub * V;
+  const PairAt pa = pair_at(a);
+  const bool in_d = d < a.D;
+  const T* kp = (const T*)a.k.p + (int64_t)pa.b * a.k.b + (int64_t)pa.hk * a.k.h + d;
+  const T* vp = (const T*)a.v.p + (int64_t)pa.b * a.v.b + (int64_t)pa.hk * a.v.h + d;
+  const uint8_t* mask = a.mask ? a.mask + (int64_t)pa.b * a.mask_ld : nullptr;
+  float q[R][V], o[R][V], m[R], l[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    packet_floats(row_ptr<T>(a.q, pa.b, row_at(a, r < a.rows ? r : 0, pa.hk)) + d, in_d && r < a.rows, q[r]);
+    m[r] = minus_inf();
+    l[r] = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) { q[r][j] *= a.scale2; o[r][j] = 0.f; }
+  }
+  for (int base = pa.k0 + wave * KPW * U; base < pa.k1; base += NW * KPW * U) {
+    uint4 kr[U], vr[U];
+    bool ok[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int key = base + u * KPW + slot;
+      ok[u] = key < pa.k1;
+      const bool in = ok[u] && in_d;
+      kr[u] = in ? *reinterpret_cast<const uint4*>(kp + (int64_t)key * a.k.t) : make_uint4(0, 0, 0, 0);
+      vr[u] = in ? *reinterpret_cast<const uint4*>(vp + (int64_t)key * a.v.t) : make_uint4(0, 0, 0, 0);
+      if (mask && ok[u]) ok[u] = mask[key] != 0;
+    }
+    float s[U][R];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[V];
+      Packet<T>::unpack(kr[u], f);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float t = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) t = fmaf(q[r][j], f[j], t);
+        s[u][r] = t;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float t = group_sum<LPK>(s[u][r]);
+        s[u][r] = ok[u] ? t : minus_inf();
+      }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float top = m[r];
+#pragma unroll
+      for (int u = 0; u < U; ++u) top = fmaxf(top, s[u][r]);
+      const float at = top == minus_inf() ? 0.f : top;
+      const float fade = __builtin_amdgcn_exp2f(m[r] - at);
+      m[r] = top;
+      l[r] *= fade;
+#pragma unroll
+      for (int j = 0; j < V; ++j) o[r][j] *= fade;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        s[u][r] = __builtin_amdgcn_exp2f(s[u][r] - at);
+        l[r] += s[u][r];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[V];
+      Packet<T>::unpack(ok[u] ? vr[u] : make_uint4(0, 0, 0, 0), f);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[r][j] = fmaf(s[u][r], f[j], o[r][j]);
+    }
+  }
+  // join the lane groups, then the waves
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float top = slot_max<LPK>(m[r]);
+    const float fade = top == minus_inf() ? 0.f : __builtin_amdgcn_exp2f(m[r] - top);
+    m[r] = top;
+    l[r] = slot_sum<LPK>(l[r] * fade);
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[r][j] = slot_sum<LPK>(o[r][j] * fade);
+  }
+  if constexpr (NW > 1) {
+    constexpr int W = LPK * V + 2;
+    if (slot == 0)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float* w = sm + (wave * R + r) * W;
+#pragma unroll
+        for (int j = 0; j < V; ++j) w[d + j] = o[r][j];
+        if (sub == 0) { w[LPK * V] = m[r]; w[LPK * V + 1] = l[r]; }
+      }
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float top = minus_inf();
+      for (int w = 0; w < NW; ++w) top = fmaxf(top, sm[(w * R + r) * W + LPK * V]);
+      const float at = top == minus_inf() ? 0.f : top;
+      m[r] = top;
+      l[r] = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) o[r][j] = 0.f;
+      for (int w = 0; w < NW; ++w) {
+        const float* from = sm + (w * R + r) * W;
+        const float fade = __builtin_amdgcn_exp2f(from[LPK * V] - at);
+        l[r] = fmaf(from[LPK * V + 1], fade, l[r]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[r][j] = fmaf(from[d + j], fade, o[r][j]);
+      }
+    }
+  }
+  if (slot) return;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (r >= a.rows) break;
+    const RowAt ra = row_at(a, r, pa.hk);
+    const int64_t rid = row_id(a, pa.b, ra);
+    const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+    const float lse = l[r] == 0.f ? minus_inf() : m[r] * LN2 + logf(l[r]);
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[r][j] *= inv;
+    if (a.splits == 1) {
+      if (in_d) *reinterpret_cast<uint4*>(const_cast<T*>(row_ptr<T>(a.out, pa.b, ra)) + d) = Packet<T>::pack(o[r]);
+      if (a.lse && sub == 0) a.lse[rid] = lse;
+    } else {
+      const int64_t at = (int64_t)pa.split * ((int64_t)a.B * a.Hkv * a.rows) + rid;
+      if (in_d)
+#pragma unroll
+        for (int j = 0; j < V; j += 4)
+          *reinterpret_cast<float4*>(a.part + at * a.D + d + j) = make_float4(o[r][j], o[r][j + 1], o[r][j + 2], o[r][j + 3]);
+      if (sub == 0) a.part_lse[at] = lse;
+    }
+  }
+}
+
+// dk and dv of the keys [k0, k1) of a pair, KPW keys per wave and step; kept: p and dp of key k, row r at
+// kept[(k - from) * R + r] and `apart` floats behind
+template <class T, int R, int LPK>
+__device__ static inline void rows_write_kv(const Attn& a, int b, int hk, int k0, int k1, int live, int from,
+                                            const float* kept, int64_t apart, const float (&q)[R][Packet<T>::V],
+                                            const float (&g)[R][Packet<T>::V], const float (&delta)[R], int wave,
+                                            int waves) {
+  constexpr int V = Packet<T>::V, KPW = 64 / LPK;
+  const int lane = threadIdx.x & 63, sub = lane % LPK, slot = lane / LPK, d = sub * V;
+  T* kp = (T*)a.dk.p + (int64_t)b * a.dk.b + (int64_t)hk * a.dk.h + d;
+  T* vp = (T*)a.dv.p + (int64_t)b * a.dv.b + (int64_t)hk * a.dv.h + d;
+  for (int key = k0 + wave * KPW + slot; key < k1; key += waves * KPW) {
+    float dk[V], dv[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) dk[j] = dv[j] = 0.f;
+    if (key < live) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float p = kept[(int64_t)(key - from) * R + r], dp = kept[apart + (int64_t)(key - from) * R + r];
+        const float ds = p == 0.f ? 0.f : p * (dp - delta[r]) * a.scale;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          dk[j] = fmaf(ds, q[r][j], dk[j]);
+          dv[j] = fmaf(p, g[r][j], dv[j]);
+        }
+      }
+    }
+    if (d < a.D) {
+      *reinterpret_cast<uint4*>(kp + (int64_t)key * a.dk.t) = Packet<T>::pack(dk);
+      *reinterpret_cast<uint4*>(vp + (int64_t)key * a.dv.t) = Packet<T>::pack(dv);
+    }
+  }
+}
+
+// FUSED: one block holds all keys of its pair in LDS; else p and dp go to a.kept and the sums to a.part
+template <class T, int R, int LPK, int NW, bool FUSED>
+__global__ __launch_bounds__(NW * 64) void attn_rows_bwd_kernel(Attn a) {
+  constexpr int V = Packet<T>::V, KPW = 64 / LPK, U = ROW_STEP, W = 2 * LPK * V + 1;
+  extern __shared__ float dyn[];                       // joins [NW][R][W], then (FUSED) p, dp [per_split * R] each
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LPK, slot = lane / LPK, d = sub * V;
+  const PairAt pa = pair_at(a);
+  const bool in_d = d < a.D;
+  const T* kp = (const T*)a.k.p + (int64_t)pa.b * a.k.b + (int64_t)pa.hk * a.k.h + d;
+  const T* vp = (const T*)a.v.p + (int64_t)pa.b * a.v.b + (int64_t)pa.hk * a.v.h + d;
+  const uint8_t* mask = a.mask ? a.mask + (int64_t)pa.b * a.mask_ld : nullptr;
+  float* kept;
+  int64_t apart;
+  if constexpr (FUSED) {
+    kept = dyn + NW * R * W;
+    apart = (int64_t)a.per_split * R;
+  } else {
+    kept = a.kept + ((int64_t)(pa.b * a.Hkv + pa.hk) * a.Tk + pa.k0) * R;
+    apart = (int64_t)a.B * a.Hkv * a.Tk * R;
+  }
+  float q[R][V], g[R][V], A[R][V], S[R][V], delta[R], shift[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const bool in = r < a.rows;
+    const RowAt ra = row_at(a, in ? r : 0, pa.hk);
+    packet_floats(row_ptr<T>(a.q, pa.b, ra) + d, in_d && in, q[r]);
+    packet_floats(row_ptr<T>(a.dout, pa.b, ra) + d, in_d && in, g[r]);
+    const float lse = in ? a.lse[row_id(a, pa.b, ra)] : minus_inf();
+    shift[r] = lse == minus_inf() ? minus_inf() : -lse * LOG2E;
+    delta[r] = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) A[r][j] = S[r][j] = 0.f;
+  }
+  for (int base = pa.k0 + wave * KPW * U; base < pa.k1; base += NW * KPW * U) {
+    uint4 kr[U], vr[U];
+    bool ok[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int key = base + u * KPW + slot;
+      ok[u] = key < pa.k1;
+      const bool in = ok[u] && in_d;
+      kr[u] = in ? *reinterpret_cast<const uint4*>(kp + (int64_t)key * a.k.t) : make_uint4(0, 0, 0, 0);
+      vr[u] = in ? *reinterpret_cast<const uint4*>(vp + (int64_t)key * a.v.t) : make_uint4(0, 0, 0, 0);
+      if (mask && ok[u]) ok[u] = mask[key] != 0;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int key = base + u * KPW + slot;
+      float f[V], h[V];
+      Packet<T>::unpack(ok[u] ? kr[u] : make_uint4(0, 0, 0, 0), f);
+      Packet<T>::unpack(ok[u] ? vr[u] : make_uint4(0, 0, 0, 0), h);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float s = 0.f, dp = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          s = fmaf(q[r][j], f[j], s);
+          dp = fmaf(g[r][j], h[j], dp);
+        }
+        s = group_sum<LPK>(s);
+        dp = group_sum<LPK>(dp);
+        const float p = ok[u] ? __builtin_amdgcn_exp2f(fmaf(s, a.scale2, shift[r])) : 0.f;
+        const float pd = p == 0.f ? 0.f : p * dp;
+        delta[r] += pd;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          A[r][j] = fmaf(pd, f[j], A[r][j]);
+          S[r][j] = fmaf(p, f[j], S[r][j]);
+        }
+        if (sub == 0 && key < pa.k1) {
+          kept[(int64_t)(key - pa.k0) * R + r] = p;
+          kept[apart + (int64_t)(key - pa.k0) * R + r] = dp;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    delta[r] = slot_sum<LPK>(delta[r]);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      A[r][j] = slot_sum<LPK>(A[r][j]);
+      S[r][j] = slot_sum<LPK>(S[r][j]);
+    }
+  }
+  if constexpr (NW > 1) {
+    if (slot == 0)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float* w = dyn + (wave * R + r) * W;
+#pragma unroll
+        for (int j = 0; j < V; ++j) { w[d + j] = A[r][j]; w[LPK * V + d + j] = S[r][j]; }
+        if (sub == 0) w[2 * LPK * V] = delta[r];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      delta[r] = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) A[r][j] = S[r][j] = 0.f;
+      for (int w = 0; w < NW; ++w) {
+        const float* from = dyn + (w * R + r) * W;
+        delta[r] += from[2 * LPK * V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) { A[r][j] += from[d + j]; S[r][j] += from[LPK * V + d + j]; }
+      }
+    }
+  } else if constexpr (FUSED) {
+    __syncthreads();                                   // p and dp of this wave's other lanes
+  }
+  if (wave == 0 && slot == 0)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (r >= a.rows) break;
+      const RowAt ra = row_at(a, r, pa.hk);
+      const int64_t rid = row_id(a, pa.b, ra);
+      if constexpr (FUSED) {
+        float dq[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) dq[j] = a.scale * (A[r][j] - delta[r] * S[r][j]);
+        if (in_d) *reinterpret_cast<uint4*>((T*)a.dq.p + (int64_t)pa.b * a.dq.b + (int64_t)ra.t * a.dq.t + (int64_t)ra.h * a.dq.h + d) = Packet<T>::pack(dq);
+      } else {
+        float* part = a.part + ((int64_t)pa.split * ((int64_t)a.B * a.Hkv * a.rows) + rid) * (2 * a.D + 1);
+        if (in_d)
+#pragma unroll
+          for (int j = 0; j < V; ++j) { part[d + j] = A[r][j]; part[a.D + d + j] = S[r][j]; }
+        if (sub == 0) part[2 * a.D] = delta[r];
+      }
+    }
+  if constexpr (FUSED)
+    rows_write_kv<T, R, LPK>(a, pa.b, pa.hk, 0, a.Tk, pa.k1, 0, kept, apart, q, g, delta, wave, NW);
+}
+
+// Pass two over kept p and dp: block `chunk` of a pair writes its keys; chunk 0 also dq
+template <class T, int R, int LPK>
+__global__ __launch_bounds__(256) void attn_rows_kv_kernel(Attn a, int chunks, int per_chunk) {
+  constexpr int V = Packet<T>::V;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LPK, slot = lane / LPK, d = sub * V;
+  const int chunk = blockIdx.x % chunks, pair = blockIdx.x / chunks, b = pair / a.Hkv, hk = pair - b * a.Hkv;
+  const bool in_d = d < a.D;
+  float q[R][V], g[R][V], delta[R];
+  const int64_t n_rows = (int64_t)a.B * a.Hkv * a.rows;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const bool in = r < a.rows;
+    const RowAt ra = row_at(a, in ? r : 0, hk);
+    packet_floats(row_ptr<T>(a.q, b, ra) + d, in_d && in, q[r]);
+    packet_floats(row_ptr<T>(a.dout, b, ra) + d, in_d && in, g[r]);
+    delta[r] = 0.f;
+    if (in) {
+      const int64_t rid = row_id(a, b, ra);
+      for (int s = 0; s < a.splits; ++s) delta[r] += a.part[(s * n_rows + rid) * (2 * a.D + 1) + 2 * a.D];
+      if (chunk == 0 && wave == 0 && slot == 0 && in_d) {
+        float dq[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          float A = 0.f, S = 0.f;
+          for (int s = 0; s < a.splits; ++s) {
+            const float* part = a.part + (s * n_rows + rid) * (2 * a.D + 1);
+            A += part[d + j];
+            S += part[a.D + d + j];
+          }
+          dq[j] = a.scale * (A - delta[r] * S);
+        }
+        *reinterpret_cast<uint4*>((T*)a.dq.p + (int64_t)b * a.dq.b + (int64_t)ra.t * a.dq.t + (int64_t)ra.h * a.dq.h + d) = Packet<T>::pack(dq);
+      }
+    }
+  }
+  const int k0 = chunk * per_chunk, k1 = min(a.Tk, k0 + per_chunk);
+  rows_write_kv<T, R, LPK>(a, b, hk, k0, k1, key_count(a, b), 0, a.kept + (int64_t)pair * a.Tk * R,
+                           (int64_t)a.B * a.Hkv * a.Tk * R, q, g, delta, wave, 4);
+}
+
 // ---- host ----------------------------------------------------------------------------------------------------------
+// keys that a wave of the few-row kernels holds at once
+static int rows_lanes(int D, int dtype) {
+  const int packets = D / (16 / type_bytes(dtype));
+  return packets <= 2 ? 2 : packets <= 4 ? 4 : packets <= 8 ? 8 : packets <= 16 ? 16 : 32;
+}
+static int rows_step_keys(int D, int dtype) { return 64 / rows_lanes(D, dtype); }
 static int padded_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
 static int pass_rows(int rows) { return rows <= 32 ? 32 : 128; }          // query rows of a block: one wave or four
 static int tile_keys(int dtype) { return dtype == CTR_F32 ? 32 : 64; }
@@ -719,8 +1119,27 @@ static int key_splits(int64_t blocks, int Tk) {
   return (int)(n < 1 ? 1 : n);
 }
 
+// Few rows: waves for about eight per SIMD, each with at least ROW_STEP steps of keys; four to a block, more as splits.
+static void rows_plan(Attn* a, int dtype) {
+  a->lanes = rows_lanes(a->D, dtype);
+  a->few = a->rows <= 1 ? 1 : a->rows <= 2 ? 2 : 4;
+  const int64_t pairs = (int64_t)a->B * a->Hkv, step = rows_step_keys(a->D, dtype) * ROW_STEP;
+  const int64_t most = cdiv(a->Tk < 1 ? 1 : a->Tk, step), want = pairs < 1 ? 1 : 8192 / pairs;
+  const int64_t waves = want < 1 ? 1 : want < most ? want : most;
+  a->waves = waves >= 2 ? 4 : 1;
+  int64_t splits = waves / 8;                          // below eight waves one block holds the pair
+  a->splits = (int)(splits < 1 ? 1 : splits > 128 ? 128 : splits);
+  a->per_split = (int)align_up(cdiv(a->Tk, a->splits), step);
+  a->splits = a->Tk > 0 ? (int)cdiv(a->Tk, a->per_split) : 1;
+}
+
 static void attn_plan(Attn* a, int dtype) {
   a->rows = a->Tq * a->G;
+  if (a->rows >= 1 && a->rows <= 4) {
+    rows_plan(a, dtype);
+    return;
+  }
+  a->few = 0;
   a->row_tiles = (int)cdiv(a->rows, pass_rows(a->rows));
   a->splits = key_splits((int64_t)a->row_tiles * a->B * a->Hkv, a->Tk);
   a->per_split = (int)align_up(cdiv(a->Tk, a->splits), 64);
@@ -728,9 +1147,16 @@ static void attn_plan(Attn* a, int dtype) {
   a->key_tiles = (int)cdiv(a->Tk, 128);
 }
 static int64_t total_rows(const Attn& a) { return (int64_t)a.B * a.Hkv * a.rows; }
+static bool rows_fused(const Attn& a) { return a.splits == 1 && (int64_t)a.per_split * a.few <= ROWS_LDS; }
 static size_t fwd_ws(const Attn& a) { return a.splits > 1 ? (size_t)a.splits * total_rows(a) * (a.D + 1) * 4 + 256 : 0; }
+// tiled: delta, then the splits' dq; few rows: the splits' sums, then p and dp of every key
+static size_t bwd_ws_first(const Attn& a) {
+  if (a.few) return rows_fused(a) ? 0 : align_up((size_t)a.splits * total_rows(a) * (2 * a.D + 1) * 4, 256);
+  return align_up((size_t)total_rows(a) * 4, 256);
+}
 static size_t bwd_ws(const Attn& a) {
-  return align_up((size_t)total_rows(a) * 4, 256) + (a.splits > 1 ? (size_t)a.splits * total_rows(a) * a.D * 4 : 0) + 256;
+  if (a.few) return rows_fused(a) ? 256 : bwd_ws_first(a) + (size_t)a.B * a.Hkv * a.Tk * a.few * 8 + 256;
+  return bwd_ws_first(a) + (a.splits > 1 ? (size_t)a.splits * total_rows(a) * a.D * 4 : 0) + 256;
 }
 
 static int attn_shape(const char* what, const ctr_attn_t* s, Attn* a) {
@@ -749,8 +1175,8 @@ static int attn_shape(const char* what, const ctr_attn_t* s, Attn* a) {
   a->scale2 = s->scale * LOG2E;
   a->sl = s->sl; a->mask = s->mask; a->mask_ld = s->mask_ld;
   attn_plan(a, s->dtype);
-  CTR_REQUIRE((int64_t)a->row_tiles * a->B * a->Hkv * a->splits < (1ll << 31) &&
-              (int64_t)a->key_tiles * a->B * a->Hkv < (1ll << 31), "%s: too many tiles", what);
+  CTR_REQUIRE((a->few ? 1 : (int64_t)a->row_tiles) * a->B * a->Hkv * a->splits < (1ll << 31) &&
+              cdiv(a->Tk, 128) * a->B * a->Hkv < (1ll << 31), "%s: too many tiles", what);
   return CTR_OK;
 }
 
@@ -789,8 +1215,63 @@ static int attn_view(const char* what, const char* name, const ctr_heads_t* v, i
     }                                           \
   } while (0)
 
+// LPK is at most 16 for 16-bit types
+#define ROWS_LANES(T, LPK, CALL)                                                     \
+  do {                                                                               \
+    switch (LPK) {                                                                   \
+      case 2: { CALL(T, 2); } break;                                                 \
+      case 4: { CALL(T, 4); } break;                                                 \
+      case 8: { CALL(T, 8); } break;                                                 \
+      case 16: { CALL(T, 16); } break;                                               \
+      default: if constexpr (sizeof(T) == 4) { CALL(T, 32); } break;                 \
+    }                                                                                \
+  } while (0)
+
+template <class T, int R>
+static void rows_fwd_launch(const Attn& a, hipStream_t st) {
+  const unsigned blocks = (unsigned)((int64_t)a.B * a.Hkv * a.splits);
+#define ROWS_FWD(T_, LPK_)                                                           \
+  if (a.waves == 1) attn_rows_fwd_kernel<T_, R, LPK_, 1><<<blocks, 64, 0, st>>>(a);  \
+  else attn_rows_fwd_kernel<T_, R, LPK_, 4><<<blocks, 256, 0, st>>>(a)
+  ROWS_LANES(T, a.lanes, ROWS_FWD);
+#undef ROWS_FWD
+}
+
+template <class T, int R>
+static void rows_bwd_launch(const Attn& a, hipStream_t st) {
+  const unsigned blocks = (unsigned)((int64_t)a.B * a.Hkv * a.splits);
+  const size_t joins = (size_t)a.waves * R * (2 * a.lanes * Packet<T>::V + 1) * 4;
+  if (rows_fused(a)) {
+    const size_t lds = joins + (size_t)a.per_split * R * 8;
+#define ROWS_BWD(T_, LPK_)                                                                        \
+  if (a.waves == 1) attn_rows_bwd_kernel<T_, R, LPK_, 1, true><<<blocks, 64, lds, st>>>(a);       \
+  else attn_rows_bwd_kernel<T_, R, LPK_, 4, true><<<blocks, 256, lds, st>>>(a)
+    ROWS_LANES(T, a.lanes, ROWS_BWD);
+#undef ROWS_BWD
+    return;
+  }
+  const int64_t pairs = (int64_t)a.B * a.Hkv;
+  const int64_t want = cdiv(2048, pairs), most = cdiv(a.Tk, 64);
+  const int per = (int)cdiv(a.Tk, want < most ? want : most), chunks = (int)cdiv(a.Tk, per);
+#define ROWS_BWD(T_, LPK_)                                                                        \
+  attn_rows_bwd_kernel<T_, R, LPK_, 4, false><<<blocks, 256, joins, st>>>(a);                     \
+  attn_rows_kv_kernel<T_, R, LPK_><<<(unsigned)(pairs * chunks), 256, 0, st>>>(a, chunks, per)
+  ROWS_LANES(T, a.lanes, ROWS_BWD);
+#undef ROWS_BWD
+}
+
 template <class T>
 static void attn_fwd_launch(const Attn& a, hipStream_t st) {
+  if (a.few) {
+    if (a.few == 1) rows_fwd_launch<T, 1>(a, st);
+    else if (a.few == 2) rows_fwd_launch<T, 2>(a, st);
+    else rows_fwd_launch<T, 4>(a, st);
+    if (a.splits > 1) {
+      const int64_t n = total_rows(a);
+      attn_join_kernel<T><<<(unsigned)cdiv(n * (a.D / 4), 256), 256, 0, st>>>(a, n);
+    }
+    return;
+  }
   constexpr int KT = sizeof(T) == 4 ? 32 : 64;
   const unsigned blocks = (unsigned)((int64_t)a.row_tiles * a.B * a.Hkv * a.splits);
   const bool one = pass_rows(a.rows) == 32;
@@ -807,6 +1288,12 @@ static void attn_fwd_launch(const Attn& a, hipStream_t st) {
 
 template <class T>
 static void attn_bwd_launch(const Attn& a, hipStream_t st) {
+  if (a.few) {
+    if (a.few == 1) rows_bwd_launch<T, 1>(a, st);
+    else if (a.few == 2) rows_bwd_launch<T, 2>(a, st);
+    else rows_bwd_launch<T, 4>(a, st);
+    return;
+  }
   constexpr int KT = sizeof(T) == 4 ? 32 : 64;
   const unsigned blocks = (unsigned)((int64_t)a.row_tiles * a.B * a.Hkv * a.splits);
   const bool one = pass_rows(a.rows) == 32;
@@ -894,8 +1381,14 @@ extern "C" int ctr_cross_attn_bwd(const ctr_attn_t* s, const ctr_heads_t* dout, 
     return CTR_EWORKSPACE;
   }
   a.lse = const_cast<float*>(lse);
-  a.delta = (float*)align_up((size_t)workspace, 256);
-  a.part = a.delta + align_up((size_t)total_rows(a) * 4, 256) / 4;
+  float* ws = (float*)align_up((size_t)workspace, 256);
+  if (a.few) {
+    a.part = ws;
+    a.kept = ws + bwd_ws_first(a) / 4;
+  } else {
+    a.delta = ws;
+    a.part = ws + bwd_ws_first(a) / 4;
+  }
   hipStream_t st = (hipStream_t)stream;
   if (s->dtype == CTR_F32) attn_bwd_launch<float>(a, st);
   else if (s->dtype == CTR_BF16) attn_bwd_launch<bf16_t>(a, st);

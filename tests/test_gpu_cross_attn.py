@@ -104,6 +104,16 @@ def test_long_cache_in_splits(Tq, G, dtype):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('B,Tq,Tk,H,Hkv,D', [(103, 1, 4200, 10, 10, 8), (300, 1, 33, 4, 4, 16), (40, 4, 260, 3, 3, 128),
+                                             (9, 1, 1500, 4, 1, 56)])
+def test_few_rows_of_many_pairs(B, Tq, Tk, H, Hkv, D, dtype):
+    """One to four rows per key head: whole histories in one block's LDS, too long for it, and split."""
+    q, k, v, dout = _make(B, Tq, Tk, H, Hkv, D, dtype, seed=6)
+    sl = _lengths(B, Tk)
+    _check(_run(q, k, v, dout, sl), attention(q, k, v, sl, dout=dout))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('Tq', [1, 70])
 def test_strided_views(dtype, Tq):
     """Keys and values as halves of one projection, heads before time, a query that every sample shares."""
