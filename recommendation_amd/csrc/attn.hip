@@ -124,10 +124,11 @@ __device__ static inline Frag<T> raw_frag(const Raw<T>& r) {
   return o;
 }
 
-// A tile of ROWS x DP values in LDS, one plane per term.  16 bytes of padding per row spread the rows over the banks.
-template <class T, int ROWS, int DP>
+// A tile of ROWS x DP values in LDS, one plane per term.  PAD (16-bit values) spreads the rows over the 32 banks: 8 for
+// rows() - eight lanes read 16 bytes of eight rows per cycle -, 16 where only cols() reads - four rows of 32 bytes.
+template <class T, int ROWS, int DP, int PAD = 8>
 struct Tile {
-  static constexpr int LD = DP + 8, NP = Terms<T>::NP, PLANE = ROWS * LD;
+  static constexpr int LD = DP + PAD, NP = Terms<T>::NP, PLANE = ROWS * LD;
   short v[NP * PLANE];
   __device__ inline void put(int row, int col, const Frag<T>& f) {
 #pragma unroll
@@ -179,6 +180,7 @@ struct Attn {
   int rows, row_tiles, key_tiles, splits, per_split;
   float *part, *part_lse;                              // [splits][B H Tq][D], [splits][B H Tq]
   float* kept;                                         // few rows: p, then dp, [B Hkv][Tk][R]
+  bool near;                                           // a tile's rows lie within 2^31 bytes of its first
   int few, waves, lanes;                               // rows padded to 1, 2 or 4 (0: the tiled kernels); waves per
                                                        // block, lanes per key
 };
@@ -197,6 +199,17 @@ __device__ static inline int die_order(int id, int n) {
 __device__ static inline int key_count(const Attn& a, int b) {
   if (!a.sl) return a.Tk;
   return min(max(a.sl[b], 0), a.Tk);
+}
+
+// Fewer than two keys left: p is 1 whatever the score, so dq and dk are zero - exactly, not up to the rounding of p.
+__device__ static inline bool lone_key(const Attn& a, int b) {
+  const int len = key_count(a, b), lane = threadIdx.x & 63;
+  if (len < 2) return true;
+  if (!a.mask) return false;
+  const uint8_t* mask = a.mask + (int64_t)b * a.mask_ld;
+  int n = 0;
+  for (int base = 0; base < len && n < 2; base += 64) n += __popcll(__ballot(base + lane < len && mask[min(base + lane, len - 1)]));
+  return n < 2;
 }
 
 struct RowAt { int t, h; };
@@ -251,214 +264,301 @@ __device__ static inline void store_strip(T* row, int col0, int D, const f32x16&
   }
 }
 
-// Registers of a thread on the way from memory to a pair of tiles: ROWS rows of DP values of two views, dealt to THREADS
+// Registers of a thread on the way from memory to a tile: ROWS rows of DP values, dealt to THREADS.  Loads are
+// unconditional: a row behind the end reads the last one, a column behind D the first, both stay in bounds and are
+// zeroed (rows) or never stored (columns) by put().  As long as whole tiles lie inside, a thread's offsets from the
+// tile's first row are the same for every tile, so the loop adds nothing per lane.
 template <class T, int ROWS, int DP, int THREADS>
 struct Stage {
   static constexpr int PER = DP / 8, N = (ROWS * PER + THREADS - 1) / THREADS;
-  Raw<T> a[N], b[N];
+  Raw<T> a[N];
+  unsigned off[N];                                     // byte offsets inside a whole tile
   bool on[N];
-  // keys k0 + row < k1 of one (sample, head); a masked key is read and dropped
-  __device__ inline void keys(const Attn& p, const T* ka, const T* kb, const uint8_t* mask, int k0, int k1) {
+  __device__ static inline int row(int i) { return (int)(threadIdx.x + i * THREADS) / PER; }
+  __device__ static inline int col(int i) { return (int)(threadIdx.x + i * THREADS) % PER * 8; }
+  __device__ inline void load(const T* first) {
+    const char* p = reinterpret_cast<const char*>(first);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = threadIdx.x + i * THREADS, row = c / PER, d = (c - row * PER) * 8, key = k0 + row;
-      const bool in = row < ROWS && key < k1 && d < p.D;
-      a[i] = in ? raw_load(ka + (int64_t)key * p.k.t + d) : raw_zero<T>();
-      b[i] = in ? raw_load(kb + (int64_t)key * p.v.t + d) : raw_zero<T>();
-      on[i] = in && (!mask || mask[key]);
-    }
-  }
-  // rows r0 + row of the row list
-  __device__ inline void list(const Attn& p, int b_, int hk, int r0) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = threadIdx.x + i * THREADS, row = c / PER, d = (c - row * PER) * 8, r = r0 + row;
-      const bool in = row < ROWS && r < p.rows && d < p.D;
-      const RowAt ra = row_at(p, in ? r : 0, hk);
-      a[i] = in ? raw_load(row_ptr<T>(p.q, b_, ra) + d) : raw_zero<T>();
-      b[i] = in ? raw_load(row_ptr<T>(p.dout, b_, ra) + d) : raw_zero<T>();
+      a[i] = raw_load(reinterpret_cast<const T*>(p + off[i]));
       on[i] = true;
     }
   }
-  __device__ inline void put(Tile<T, ROWS, DP>& ta, Tile<T, ROWS, DP>& tb) const {
+  __device__ inline void keys_init(const Attn& p, const View4& w) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      off[i] = (unsigned)((min(row(i), ROWS - 1) * w.t + (col(i) < p.D ? col(i) : 0)) * sizeof(T));
+  }
+  // keys k0 .. of one (sample, head), k0 < k1
+  __device__ inline void keys(const Attn& p, const View4& w, const T* base, const uint8_t* mask, int k0, int k1) {
+    if (k0 + ROWS <= k1 && !mask && p.near) return load(base + (int64_t)k0 * w.t);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = threadIdx.x + i * THREADS, row = c / PER, d = (c - row * PER) * 8;
-      if (row < ROWS) {
-        ta.put(row, d, raw_frag<T>(on[i] ? a[i] : raw_zero<T>()));
-        tb.put(row, d, raw_frag<T>(on[i] ? b[i] : raw_zero<T>()));
-      }
+      const int d = col(i) < p.D ? col(i) : 0, key = min(k0 + row(i), k1 - 1);
+      a[i] = raw_load(base + (int64_t)key * w.t + d);
+      on[i] = k0 + row(i) < k1 && (!mask || mask[key]);
+    }
+  }
+  __device__ inline void list_init(const Attn& p, const View4& w) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = min(row(i), ROWS - 1), t = r / p.G, h = r - t * p.G;
+      off[i] = (unsigned)((t * w.t + h * w.h + (col(i) < p.D ? col(i) : 0)) * sizeof(T));
+    }
+  }
+  // rows r0 .. of the row list, r0 < rows
+  __device__ inline void list(const Attn& p, const View4& w, int b, int hk, int r0) {
+    if (r0 + ROWS <= p.rows && ROWS % p.G == 0 && p.near) return load(row_ptr<T>(w, b, {r0 / p.G, hk * p.G}));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      a[i] = raw_load(row_ptr<T>(w, b, row_at(p, min(r0 + row(i), p.rows - 1), hk)) + (col(i) < p.D ? col(i) : 0));
+      on[i] = r0 + row(i) < p.rows;
+    }
+  }
+  template <class TILE>
+  __device__ inline void put(TILE& t, int D, bool whole) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (row(i) >= ROWS || col(i) >= D) continue;
+      t.put(row(i), col(i), raw_frag<T>(whole || on[i] ? a[i] : raw_zero<T>()));
     }
   }
 };
 
-// Bit i: key k0 + i may be attended to (the same in every lane)
+// LDS starts as zeros where the head size leaves columns of a tile unwritten (0 * NaN in the products over d otherwise)
+template <class TILE>
+__device__ static inline void clear_tile(TILE& t) {
+  constexpr int N = sizeof(t.v) / 16;
+  static_assert(sizeof(t.v) % 16 == 0, "16-byte rows");
+  for (int i = threadIdx.x; i < N; i += blockDim.x) reinterpret_cast<uint4*>(t.v)[i] = make_uint4(0, 0, 0, 0);
+}
+
+// The keys that a tile leaves out: adds -infinity to their scores.  Bit i of `bits`: key k0 + i may be attended to.
 __device__ static inline uint64_t key_bits(const uint8_t* mask, int k0, int k1, int n) {
   const int lane = threadIdx.x & 63, key = k0 + lane;
   return __ballot(lane < n && key < k1 && (!mask || mask[key]));
 }
+__device__ static inline void leave_out(f32x16& s, uint64_t bits, int i) {
+  const uint64_t mine = bits >> (4 * ((threadIdx.x & 63) >> 5));
+#pragma unroll
+  for (int e = 0; e < 16; ++e) s[e] = (mine >> (i * 32 + acc_row(e))) & 1 ? s[e] : minus_inf();
+}
+
+// Waves per SIMD the tiled kernels are built for.  Two keep a wave within 256 registers, and only then does the compiler
+// leave the accumulators where the vector units reach them: at one (512 registers) it keeps them in the other half of
+// the register file and moves every value over and back (a third of the instructions of the forward's loop).
+template <class T, int DP>
+constexpr int WAVES = Terms<T>::NP == 3 && DP > 64 ? 1 : 2;
+// The forward needs fewer registers: four waves at head sizes up to 64 (tiles of 64 keys), three above (32 keys).
+template <class T, int DP>
+constexpr int FWD_WAVES = Terms<T>::NP == 3 ? (DP > 64 ? 1 : DP > 32 ? 2 : 3) : DP > 64 ? 3 : 4;
 
 // ---- forward -------------------------------------------------------------------------------------------------------
-// A wave owns QT x 32 query rows; the NW waves of a block share each tile of KT keys.
-template <class T, int DP, int NW, int QT, int KT>
-__global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(Attn a) {
-  constexpr int NS = KT / 32, NK = DP / 16, ND = DP / 32;
-  __shared__ Tile<T, KT, DP> kt, vt;
+// A wave owns 32 query rows; the NW waves of a block share each tile of KT keys.  Two tiles of LDS and one barrier per
+// tile: behind it tile i + 1 goes from registers to the buffer that tile i - 1 has left, tile i + 2 is requested, and
+// tile i is computed.  One wave alone needs neither.
+// The running maximum is a reference, not the maximum itself: accumulators and sum are rescaled only when a score passes
+// it by more than LIMIT (a power of two), so p stays below 2^(BIAS + LIMIT) and after the first tiles that is rare.
+template <class T, int DP, int NW, int KT>
+__global__ __launch_bounds__(NW * 64, (NW == 1 ? WAVES<T, DP> : FWD_WAVES<T, DP>)) void attn_fwd_kernel(Attn a) {
+  constexpr int NS = KT / 32, NK = DP / 16, ND = DP / 32, NBUF = NW > 1 ? 2 : 1;
+  constexpr float BIAS = __is_same(T, f16_t) ? 8.f : 0.f, LIMIT = 7.f;
+  __shared__ Tile<T, KT, DP> kt[NBUF];
+  __shared__ Tile<T, KT, DP, 16> vt[NBUF];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int id = die_order(blockIdx.x, gridDim.x);
   const int split = id % a.splits;
   id /= a.splits;
   const int tile = id % a.row_tiles, bh = id / a.row_tiles, b = bh / a.Hkv, hk = bh - b * a.Hkv;
   const int k0 = split * a.per_split, k1 = min(key_count(a, b), k0 + a.per_split);
-  const int r0 = (tile * NW + wave) * QT * 32;
+  const int r0 = (tile * NW + wave) * 32;
   const bool busy = r0 < a.rows;
   const T* kp = (const T*)a.k.p + (int64_t)b * a.k.b + (int64_t)hk * a.k.h;
   const T* vp = (const T*)a.v.p + (int64_t)b * a.v.b + (int64_t)hk * a.v.h;
   const uint8_t* mask = a.mask ? a.mask + (int64_t)b * a.mask_ld : nullptr;
 
-  Frag<T> qf[QT][NK];
-  f32x16 o[QT][ND];
-  float m[QT], l[QT];
+  Stage<T, KT, DP, NW * 64> nk, nv;
+  nk.keys_init(a, a.k);
+  nv.keys_init(a, a.v);
+  auto load = [&](int kb) {
+    if (kb >= k1) return;
+    nk.keys(a, a.k, kp, mask, kb, k1);
+    nv.keys(a, a.v, vp, mask, kb, k1);
+  };
+  auto put = [&](int buf, int kb) {
+    if (kb >= k1) return;
+    const bool whole = !mask && kb + KT <= k1;
+    nk.put(kt[buf], a.D, whole);
+    nv.put(vt[buf], a.D, whole);
+  };
+  load(k0);
+  const int r = r0 + (lane & 31);
+  const RowAt ra = row_at(a, r < a.rows ? r : 0, hk);
+  Frag<T> qf[NK];
+  load_row_frags<T, DP>(row_ptr<T>(a.q, b, ra), r < a.rows, a.D, qf);
+  f32x16 o[ND];
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int r = r0 + t * 32 + (lane & 31);
-    load_row_frags<T, DP>(row_ptr<T>(a.q, b, row_at(a, r < a.rows ? r : 0, hk)), r < a.rows, a.D, qf[t]);
-    m[t] = minus_inf();
-    l[t] = 0.f;
+  for (int d = 0; d < ND; ++d) o[d] = f32x16{};
+  float m = minus_inf(), l = 0.f;
+  if (a.D < DP) {
 #pragma unroll
-    for (int d = 0; d < ND; ++d) o[t][d] = f32x16{};
-  }
-
-  Stage<T, KT, DP, NW * 64> next;
-  if (k0 < k1) next.keys(a, kp, vp, mask, k0, k1);
-  for (int kb = k0; kb < k1; kb += KT) {
-    __syncthreads();                                   // every wave is done with the tile before this one
-    next.put(kt, vt);
-    const uint64_t bits = key_bits(mask, kb, k1, KT);
-    if (kb + KT < k1) next.keys(a, kp, vp, mask, kb + KT, k1);
+    for (int i = 0; i < NBUF; ++i) clear_tile(kt[i]);
     __syncthreads();
-    if (!busy || bits == 0) continue;
-    f32x16 s[QT][NS];
+  }
+  if constexpr (NBUF == 2) {
+    put(0, k0);
+    load(k0 + KT);
+  }
+  int at = 0;
+  for (int kb = k0; kb < k1; kb += KT) {
+    __syncthreads();
+    if constexpr (NBUF == 2) {
+      put(at ^ 1, kb + KT);
+      load(kb + 2 * KT);
+    } else {
+      put(0, kb);
+      load(kb + KT);
+      __syncthreads();
+    }
+    const auto& ks = kt[at];
+    const auto& vs = vt[at];
+    if constexpr (NBUF == 2) at ^= 1;
+    if (!busy) continue;
+    f32x16 s[NS];
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
+      s[i] = f32x16{};
 #pragma unroll
-      for (int t = 0; t < QT; ++t) s[t][i] = f32x16{};
-#pragma unroll
-      for (int c = 0; c < NK; ++c) {
-        const Frag<T> kf = kt.rows(i * 32, c * 16);
-#pragma unroll
-        for (int t = 0; t < QT; ++t) s[t][i] = mfma<T>(kf, qf[t][c], s[t][i]);
-      }
+      for (int c = 0; c < NK; ++c) s[i] = mfma<T>(ks.rows(i * 32, c * 16), qf[c], s[i]);
     }
-    const bool all = bits == (KT == 64 ? ~0ull : ((1ull << (KT & 63)) - 1));
-    if (!all) {
-      const uint64_t mine = bits >> (4 * (lane >> 5));
+    if (mask || kb + KT > k1) {
+      const uint64_t bits = key_bits(mask, kb, k1, KT);
 #pragma unroll
-      for (int i = 0; i < NS; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const bool on = (mine >> (i * 32 + acc_row(r))) & 1;
-#pragma unroll
-          for (int t = 0; t < QT; ++t) s[t][i][r] = on ? s[t][i][r] : minus_inf();
-        }
+      for (int i = 0; i < NS; ++i) leave_out(s[i], bits, i);
     }
+    float top = s[0][0];
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      float top = m[t];
+    for (int i = 0; i < NS; ++i)
 #pragma unroll
-      for (int i = 0; i < NS; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][i][r]);
-      top = half_max(top);
-      const float base = top == minus_inf() ? 0.f : top;          // nothing seen yet: every p below is 2^-inf = 0
-      const float shift = Terms<T>::BIAS - base * a.scale2;
-      const float fade = __builtin_amdgcn_exp2f((m[t] - base) * a.scale2);
-      m[t] = top;
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < NS; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[t][i][r] = __builtin_amdgcn_exp2f(fmaf(s[t][i][r], a.scale2, shift));
-          sum += s[t][i][r];
-        }
-      l[t] = fmaf(l[t], fade, sum);
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[i][e]);
+    top = half_max(top);
+    if (__any((top - m) * a.scale2 > LIMIT)) {         // a row's first score is infinitely far from m
+      const float to = fmaxf(m, top);
+      const float fade = to == minus_inf() ? 1.f : __builtin_amdgcn_exp2f((m - to) * a.scale2);
+      m = to;
+      l *= fade;
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[t][d][r] *= fade;
+        for (int e = 0; e < 16; ++e) o[d][e] *= fade;
     }
+    const float shift = BIAS - (m == minus_inf() ? 0.f : m) * a.scale2;      // nothing seen yet: p = 2^-inf
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[i][e] = __builtin_amdgcn_exp2f(fmaf(s[i][e], a.scale2, shift));
+        sum += s[i][e];
+      }
+    l += sum;
 #pragma unroll
     for (int i = 0; i < NS; ++i)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        Frag<T> pf[QT];
+        float f[8];
 #pragma unroll
-        for (int t = 0; t < QT; ++t) {
-          float f[8];
+        for (int j = 0; j < 8; ++j) f[j] = s[i][c * 8 + j];
+        const Frag<T> pf = make_frag<T>(f);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] = s[t][i][c * 8 + j];
-          pf[t] = make_frag<T>(f);
-        }
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          const Frag<T> vf = vt.cols(i * 32 + c * 16, d * 32);
-#pragma unroll
-          for (int t = 0; t < QT; ++t) o[t][d] = mfma<T>(vf, pf[t], o[t][d]);
-        }
+        for (int d = 0; d < ND; ++d) o[d] = mfma<T>(vs.cols(i * 32 + c * 16, d * 32), pf, o[d]);
       }
   }
-  if (!busy) return;
+  const float sum = half_swap_sum(l, l);
+  if (r >= a.rows) return;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int64_t rid = row_id(a, b, ra);
+  const float lse = sum == 0.f ? minus_inf() : m * a.scale + (logf(sum) - BIAS * LN2);
+  if (a.splits == 1) {
+    T* dst = const_cast<T*>(row_ptr<T>(a.out, b, ra));
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int r = r0 + t * 32 + (lane & 31);
-    const float sum = half_swap_sum(l[t], l[t]);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    if (r >= a.rows) continue;
-    const RowAt ra = row_at(a, r, hk);
-    const int64_t rid = row_id(a, b, ra);
-    const float lse = sum == 0.f ? minus_inf() : m[t] * a.scale + (logf(sum) - Terms<T>::BIAS * LN2);
-    if (a.splits == 1) {
-      T* dst = const_cast<T*>(row_ptr<T>(a.out, b, ra));
+    for (int d = 0; d < ND; ++d) store_strip<T>(dst, d * 32, a.D, o[d], inv);
+    if (a.lse && lane < 32) a.lse[rid] = lse;
+  } else {
+    const int64_t to = (int64_t)split * ((int64_t)a.B * a.Hkv * a.rows) + rid;
+    float* dst = a.part + to * a.D;
 #pragma unroll
-      for (int d = 0; d < ND; ++d) store_strip<T>(dst, d * 32, a.D, o[t][d], inv);
-      if (a.lse && lane < 32) a.lse[rid] = lse;
-    } else {
-      const int64_t at = (int64_t)split * ((int64_t)a.B * a.Hkv * a.rows) + rid;
-      float* dst = a.part + at * a.D;
-#pragma unroll
-      for (int d = 0; d < ND; ++d) store_strip<float>(dst, d * 32, a.D, o[t][d], inv);
-      if (lane < 32) a.part_lse[at] = lse;
-    }
+    for (int d = 0; d < ND; ++d) store_strip<float>(dst, d * 32, a.D, o[d], inv);
+    if (lane < 32) a.part_lse[to] = lse;
   }
 }
 
-// Joins the splits: out = sum_i w_i out_i, w_i = exp(lse_i - max) / sum; a thread per four columns of a row
+// A row's place in a [B, T, heads, D] view from its number
 template <class T>
-__global__ __launch_bounds__(256) void attn_join_kernel(Attn a, int64_t n_rows) {
-  const int quads = a.D / 4;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (id >= n_rows * quads) return;
-  const int64_t rid = id / quads;
-  const int d = (int)(id - rid * quads) * 4;
-  float top = minus_inf();
-  for (int i = 0; i < a.splits; ++i) top = fmaxf(top, a.part_lse[i * n_rows + rid]);
-  const float base = top == minus_inf() ? 0.f : top;
-  float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < a.splits; ++i) {
-    const float w = expf(a.part_lse[i * n_rows + rid] - base);
-    const float4 v = *reinterpret_cast<const float4*>(a.part + (i * n_rows + rid) * a.D + d);
-    sum += w;
-    acc[0] = fmaf(w, v.x, acc[0]);
-    acc[1] = fmaf(w, v.y, acc[1]);
-    acc[2] = fmaf(w, v.z, acc[2]);
-    acc[3] = fmaf(w, v.w, acc[3]);
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+__device__ static inline T* row_of(const Attn& a, const View4& w, int64_t rid) {
   const int H = a.Hkv * a.G;
   const int64_t bhead = rid / a.Tq;
   const RowAt ra = {(int)(rid - bhead * a.Tq), (int)(bhead % H)};
-  T* dst = const_cast<T*>(row_ptr<T>(a.out, (int)(bhead / H), ra)) + d;
+  return const_cast<T*>(row_ptr<T>(w, (int)(bhead / H), ra));
+}
+
+// Joins the splits of a row: sum over i of weight(i) * part[i], in split order.  Few splits: a thread per four columns of
+// a row walks them all; from JOIN_WIDE on, a block per row, eight groups of 32 threads take every eighth split and are
+// added in group order (one thread over 128 splits took 33 us where the forward before it took 48).
+constexpr int JOIN_WIDE = 8;
+template <class T, bool WIDE>
+__global__ __launch_bounds__(256) void attn_join_kernel(Attn a, int64_t n_rows) {
+  const int quads = a.D / 4;
+  int64_t rid;
+  int quad, first = 0, every = 1;
+  if constexpr (WIDE) {
+    rid = blockIdx.x;
+    quad = threadIdx.x & 31;
+    first = threadIdx.x >> 5;
+    every = 8;
+  } else {
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= n_rows * quads) return;
+    rid = id / quads;
+    quad = (int)(id - rid * quads);
+  }
+  const int d = quad * 4;
+  float top = minus_inf();
+  if constexpr (WIDE) {
+    for (int i = threadIdx.x & 63; i < a.splits; i += 64) top = fmaxf(top, a.part_lse[i * n_rows + rid]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  } else {
+    for (int i = 0; i < a.splits; ++i) top = fmaxf(top, a.part_lse[i * n_rows + rid]);
+  }
+  const float base = top == minus_inf() ? 0.f : top;
+  float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i = first; i < a.splits; i += every) {
+    const float w = expf(a.part_lse[i * n_rows + rid] - base);
+    sum += w;
+    if (quad < quads) {
+      const float4 v = *reinterpret_cast<const float4*>(a.part + (i * n_rows + rid) * a.D + d);
+      acc[0] = fmaf(w, v.x, acc[0]);
+      acc[1] = fmaf(w, v.y, acc[1]);
+      acc[2] = fmaf(w, v.z, acc[2]);
+      acc[3] = fmaf(w, v.w, acc[3]);
+    }
+  }
+  if constexpr (WIDE) {
+    __shared__ float red[8][32][5];
+    float* mine = red[first][quad];
+    mine[0] = acc[0]; mine[1] = acc[1]; mine[2] = acc[2]; mine[3] = acc[3]; mine[4] = sum;
+    __syncthreads();
+    if (first) return;
+    for (int g = 1; g < 8; ++g) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] += red[g][quad][j];
+      sum += red[g][quad][4];
+    }
+    if (quad >= quads) return;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T* dst = row_of<T>(a, a.out, rid) + d;
 #pragma unroll
   for (int j = 0; j < 4; ++j) dst[j] = (T)(acc[j] * inv);
   if (a.lse && d == 0) a.lse[rid] = sum == 0.f ? minus_inf() : base + logf(sum);
@@ -486,12 +586,17 @@ __device__ static inline float fit_f16(const f32x16& ds, float factor, f32x16* a
 }
 constexpr float F16_FACTOR0 = 1.2676506e30f;           // 2^100: the first strip with a gradient sets the factor
 
-// dq, and delta for the dk / dv pass.  A wave owns 32 query rows.
+// dq, and delta for the dk / dv pass.  A wave owns 32 query rows; buffers and barrier as in the forward, both tiles at
+// the same distance.
+// For 16-bit tensors delta = sum_d dout out carries the rounding of out, the same error e for every key of a row: dq
+// would be off by e times the row's mean key, dk alike.  The sum of ds over all keys is exactly that error (it is zero
+// otherwise), so it is summed in fp32, put into delta for the dk / dv pass, and taken out of dq with the row's mean key
+// (KEYS: sum p k, a second product per strip over operands that are there already).
 template <class T, int DP, int NW, int KT>
-__global__ __launch_bounds__(NW * 64) void attn_dq_kernel(Attn a) {
-  constexpr int NS = KT / 32, NK = DP / 16, ND = DP / 32;
-  constexpr bool F16 = __is_same(T, f16_t);
-  __shared__ Tile<T, KT, DP> kt, vt;
+__global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dq_kernel(Attn a) {
+  constexpr int NS = KT / 32, NK = DP / 16, ND = DP / 32, NBUF = NW > 1 ? 2 : 1;
+  constexpr bool F16 = __is_same(T, f16_t), KEYS = Terms<T>::NP == 1;
+  __shared__ Tile<T, KT, DP> kt[NBUF], vt[NBUF];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int id = die_order(blockIdx.x, gridDim.x);
   const int split = id % a.splits;
@@ -504,6 +609,22 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(Attn a) {
   const T* vp = (const T*)a.v.p + (int64_t)b * a.v.b + (int64_t)hk * a.v.h;
   const uint8_t* mask = a.mask ? a.mask + (int64_t)b * a.mask_ld : nullptr;
 
+  Stage<T, KT, DP, NW * 64> nk, nv;
+  nk.keys_init(a, a.k);
+  nv.keys_init(a, a.v);
+  auto is_whole = [&](int kb) { return !mask && kb + KT <= k1; };
+  auto load = [&](int kb) {
+    if (kb >= k1) return;
+    nk.keys(a, a.k, kp, mask, kb, k1);
+    nv.keys(a, a.v, vp, mask, kb, k1);
+  };
+  auto put = [&](int buf, int kb) {
+    if (kb >= k1) return;
+    const bool whole = is_whole(kb);
+    nk.put(kt[buf], a.D, whole);
+    nv.put(vt[buf], a.D, whole);
+  };
+  load(k0);
   const int r = r0 + (lane & 31);
   const bool in = r < a.rows;
   const RowAt ra = row_at(a, in ? r : 0, hk);
@@ -531,70 +652,119 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(Attn a) {
   float shift = minus_inf();                           // a row without keys: p = 2^-inf
   if (in) {
     const float lse = a.lse[rid];
-    shift = lse == minus_inf() ? minus_inf() : -lse * LOG2E;
-    if (split == 0 && lane < 32) a.delta[rid] = delta;
+    shift = lse == minus_inf() ? minus_inf() : Terms<T>::BIAS - lse * LOG2E;
   }
-  f32x16 acc[ND];
+  f32x16 acc[ND], keys[KEYS ? ND : 1];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
-  float factor = F16 ? F16_FACTOR0 : 1.f;
+#pragma unroll
+  for (int d = 0; d < (KEYS ? ND : 1); ++d) keys[d] = f32x16{};
+  float factor = F16 ? F16_FACTOR0 : 1.f, rest = 0.f;
 
-  Stage<T, KT, DP, NW * 64> next;
-  if (k0 < k1) next.keys(a, kp, vp, mask, k0, k1);
-  for (int kb = k0; kb < k1; kb += KT) {
-    __syncthreads();
-    next.put(kt, vt);
-    const uint64_t bits = key_bits(mask, kb, k1, KT);
-    if (kb + KT < k1) next.keys(a, kp, vp, mask, kb + KT, k1);
-    __syncthreads();
-    if (!busy || bits == 0) continue;
-    const uint64_t mine = bits >> (4 * (lane >> 5));
+  auto tile_work = [&](int buf, bool whole, int kb) {
+    const uint64_t bits = whole ? 0 : key_bits(mask, kb, k1, KT);
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
       for (int c = 0; c < NK; ++c) {
-        s = mfma<T>(kt.rows(i * 32, c * 16), qf[c], s);
-        dp = mfma<T>(vt.rows(i * 32, c * 16), gf[c], dp);
+        s = mfma<T>(kt[buf].rows(i * 32, c * 16), qf[c], s);
+        dp = mfma<T>(vt[buf].rows(i * 32, c * 16), gf[c], dp);
       }
+      if (!whole) leave_out(s, bits, i);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, shift));
-        const bool on = (mine >> (i * 32 + acc_row(e))) & 1;
-        dp[e] = on ? p * (dp[e] - delta) : 0.f;
+        s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, shift));
+        dp[e] = s[e] * (dp[e] - delta);
+        if (KEYS) rest += dp[e];
       }
       if constexpr (F16) factor = fit_f16<ND>(dp, factor, acc);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float f[8];
+        float f[8], e[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = F16 ? dp[c * 8 + j] * factor : dp[c * 8 + j];
+        for (int j = 0; j < 8; ++j) {
+          f[j] = F16 ? dp[c * 8 + j] * factor : dp[c * 8 + j];
+          e[j] = s[c * 8 + j];
+        }
         const Frag<T> df = make_frag<T>(f);
+        Frag<T> pf;
+        if constexpr (KEYS) pf = make_frag<T>(e);
 #pragma unroll
-        for (int d = 0; d < ND; ++d) acc[d] = mfma<T>(kt.cols(i * 32 + c * 16, d * 32), df, acc[d]);
+        for (int d = 0; d < ND; ++d) {
+          const Frag<T> kf = kt[buf].cols(i * 32 + c * 16, d * 32);
+          acc[d] = mfma<T>(kf, df, acc[d]);
+          if constexpr (KEYS) keys[d] = mfma<T>(kf, pf, keys[d]);
+        }
       }
     }
+  };
+  if (a.D < DP) {
+#pragma unroll
+    for (int i = 0; i < NBUF; ++i) {
+      clear_tile(kt[i]);
+      clear_tile(vt[i]);
+    }
+    __syncthreads();
+  }
+  if constexpr (NBUF == 2) {
+    put(0, k0);
+    load(k0 + KT);
+  }
+  int at = 0;
+  for (int kb = k0; kb < k1; kb += KT) {
+    __syncthreads();
+    if constexpr (NBUF == 2) {
+      put(at ^ 1, kb + KT);
+      load(kb + 2 * KT);
+    } else {
+      put(0, kb);
+      load(kb + KT);
+      __syncthreads();
+    }
+    if (busy) tile_work(at, is_whole(kb), kb);
+    if constexpr (NBUF == 2) at ^= 1;
+  }
+  constexpr float unbias = 1.f / (1 << (int)Terms<T>::BIAS);
+  rest = half_swap_sum(rest, rest) * unbias;
+  if (lone_key(a, b)) {
+    rest = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
   }
   if (!in) return;
-  const float by = a.scale / factor;
   if (a.splits == 1) {
+    if (lane < 32) a.delta[rid] = delta + rest;
     T* dst = const_cast<T*>(row_ptr<T>(a.dq, b, ra));
 #pragma unroll
-    for (int d = 0; d < ND; ++d) store_strip<T>(dst, d * 32, a.D, acc[d], by);
-  } else {
-    float* dst = a.part + ((int64_t)split * ((int64_t)a.B * a.Hkv * a.rows) + rid) * a.D;
+    for (int d = 0; d < ND; ++d) {
+      if constexpr (KEYS)
 #pragma unroll
-    for (int d = 0; d < ND; ++d) store_strip<float>(dst, d * 32, a.D, acc[d], by);
+        for (int e = 0; e < 16; ++e) acc[d][e] = acc[d][e] * (unbias / factor) - rest * (keys[d][e] * unbias);
+      store_strip<T>(dst, d * 32, a.D, acc[d], a.scale);
+    }
+  } else {                                             // sum ds k, then sum p k, then sum ds; the join follows
+    const int64_t n_rows = (int64_t)a.B * a.Hkv * a.rows;
+    float* dst = a.part + ((int64_t)split * n_rows + rid) * (KEYS ? 2 * a.D : a.D);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      store_strip<float>(dst, d * 32, a.D, acc[d], unbias / factor);
+      if constexpr (KEYS) store_strip<float>(dst + a.D, d * 32, a.D, keys[d], unbias);
+    }
+    if (lane < 32) {
+      if constexpr (KEYS) a.part_lse[(int64_t)split * n_rows + rid] = rest;
+      if (split == 0) a.delta[rid] = delta;
+    }
   }
 }
 
 // dk and dv.  A wave owns 32 keys and walks the query rows in tiles of QB.
 template <class T, int DP, int NW, int QB>
-__global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(Attn a) {
+__global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dkv_kernel(Attn a) {
   constexpr int NS = QB / 32, NK = DP / 16, ND = DP / 32;
   constexpr bool F16 = __is_same(T, f16_t);
-  __shared__ Tile<T, QB, DP> qt, gt;
-  __shared__ float4 shift_s[QB / 4], delta_s[QB / 4];
+  __shared__ Tile<T, QB, DP> qt[2], gt[2];
+  __shared__ float4 shift_s[2][QB / 4], delta_s[2][QB / 4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int id = die_order(blockIdx.x, gridDim.x);
   const int tile = id % a.key_tiles, bh = id / a.key_tiles, b = bh / a.Hkv, hk = bh - b * a.Hkv;
@@ -606,14 +776,15 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(Attn a) {
 #pragma unroll
   for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{};
   float factor = F16 ? F16_FACTOR0 : 1.f;
-  if (key0 < len) {
-    Frag<T> kf[NK], vf[NK];
-    load_row_frags<T, DP>((const T*)a.k.p + (int64_t)b * a.k.b + (int64_t)hk * a.k.h + (int64_t)(on ? key : 0) * a.k.t, on, a.D, kf);
-    load_row_frags<T, DP>((const T*)a.v.p + (int64_t)b * a.v.b + (int64_t)hk * a.v.h + (int64_t)(on ? key : 0) * a.v.t, on, a.D, vf);
-    Stage<T, QB, DP, NW * 64> next;
+  if (key0 < len && a.rows > 0) {
+    Stage<T, QB, DP, NW * 64> nq, ng;
+    nq.list_init(a, a.q);
+    ng.list_init(a, a.dout);
     float lse_n = 0.f, delta_n = 0.f;
-    auto fetch = [&](int r0) {
-      next.list(a, b, hk, r0);
+    auto load = [&](int r0) {
+      if (r0 >= a.rows) return;
+      nq.list(a, a.q, b, hk, r0);
+      ng.list(a, a.dout, b, hk, r0);
       if (threadIdx.x < QB) {
         const int r = r0 + threadIdx.x;
         lse_n = minus_inf();
@@ -625,35 +796,47 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(Attn a) {
         }
       }
     };
-    fetch(0);
-    for (int r0 = 0; r0 < a.rows; r0 += QB) {
-      __syncthreads();
-      next.put(qt, gt);
+    auto put = [&](int buf, int r0) {
+      if (r0 >= a.rows) return;
+      nq.put(qt[buf], a.D, r0 + QB <= a.rows);
+      ng.put(gt[buf], a.D, r0 + QB <= a.rows);
       if (threadIdx.x < QB) {
-        reinterpret_cast<float*>(shift_s)[threadIdx.x] = lse_n == minus_inf() ? minus_inf() : Terms<T>::BIAS - lse_n * LOG2E;
-        reinterpret_cast<float*>(delta_s)[threadIdx.x] = delta_n;
+        reinterpret_cast<float*>(shift_s[buf])[threadIdx.x] = lse_n == minus_inf() ? minus_inf() : Terms<T>::BIAS - lse_n * LOG2E;
+        reinterpret_cast<float*>(delta_s[buf])[threadIdx.x] = delta_n;
       }
-      if (r0 + QB < a.rows) fetch(r0 + QB);
+    };
+    load(0);
+    Frag<T> kf[NK], vf[NK];
+    load_row_frags<T, DP>((const T*)a.k.p + (int64_t)b * a.k.b + (int64_t)hk * a.k.h + (int64_t)(on ? key : 0) * a.k.t, on, a.D, kf);
+    load_row_frags<T, DP>((const T*)a.v.p + (int64_t)b * a.v.b + (int64_t)hk * a.v.h + (int64_t)(on ? key : 0) * a.v.t, on, a.D, vf);
+    if (a.D < DP) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        clear_tile(qt[i]);
+        clear_tile(gt[i]);
+      }
       __syncthreads();
-      if (!busy) continue;
+    }
+    auto tile_work = [&](int buf) {
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
         for (int c = 0; c < NK; ++c) {
-          s = mfma<T>(qt.rows(i * 32, c * 16), kf[c], s);
-          dp = mfma<T>(gt.rows(i * 32, c * 16), vf[c], dp);
+          s = mfma<T>(qt[buf].rows(i * 32, c * 16), kf[c], s);
+          dp = mfma<T>(gt[buf].rows(i * 32, c * 16), vf[c], dp);
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const int at = i * 8 + 2 * g + (lane >> 5);   // rows i * 32 + 8 g + 4 half .. + 3
-          const float4 sh = shift_s[at], de = delta_s[at];
+          const int g4 = i * 8 + 2 * g + (lane >> 5);   // rows i * 32 + 8 g + 4 half .. + 3
+          const float4 sh = shift_s[buf][g4], de = delta_s[buf][g4];
           const float shv[4] = {sh.x, sh.y, sh.z, sh.w}, dev[4] = {de.x, de.y, de.z, de.w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float p = on ? __builtin_amdgcn_exp2f(fmaf(s[4 * g + j], a.scale2, shv[j])) : 0.f;
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * g + j], a.scale2, shv[j]));
+            const float ds = p * (dp[4 * g + j] - dev[j]);
             s[4 * g + j] = p;
-            dp[4 * g + j] = on ? p * (dp[4 * g + j] - dev[j]) : 0.f;
+            dp[4 * g + j] = ds;
           }
         }
         if constexpr (F16) factor = fit_f16<ND>(dp, factor, dk);
@@ -668,46 +851,91 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(Attn a) {
           const Frag<T> pf = make_frag<T>(f), df = make_frag<T>(e);
 #pragma unroll
           for (int d = 0; d < ND; ++d) {
-            dv[d] = mfma<T>(gt.cols(i * 32 + c * 16, d * 32), pf, dv[d]);
-            dk[d] = mfma<T>(qt.cols(i * 32 + c * 16, d * 32), df, dk[d]);
+            dv[d] = mfma<T>(gt[buf].cols(i * 32 + c * 16, d * 32), pf, dv[d]);
+            dk[d] = mfma<T>(qt[buf].cols(i * 32 + c * 16, d * 32), df, dk[d]);
           }
         }
       }
+    };
+    put(0, 0);
+    load(QB);
+    int at = 0;
+    for (int r0 = 0; r0 < a.rows; r0 += QB, at ^= 1) {
+      __syncthreads();
+      put(at ^ 1, r0 + QB);
+      load(r0 + 2 * QB);
+      if (busy) tile_work(at);
     }
   }
+  const bool lone = lone_key(a, b);
   if (key >= a.Tk) return;
-  const float one = 1.f / exp2f(Terms<T>::BIAS);        // ds carries p's factor too
+  if (!on) factor = 1.f;
+  constexpr float one = 1.f / (1 << (int)Terms<T>::BIAS);   // ds carries p's factor too
   T* kd = (T*)a.dk.p + (int64_t)b * a.dk.b + (int64_t)key * a.dk.t + (int64_t)hk * a.dk.h;
   T* vd = (T*)a.dv.p + (int64_t)b * a.dv.b + (int64_t)key * a.dv.t + (int64_t)hk * a.dv.h;
 #pragma unroll
   for (int d = 0; d < ND; ++d) {
+    if (lone) dk[d] = f32x16{};
+    if (!on) dk[d] = dv[d] = f32x16{};                  // a key that is left out: its lane computed with zeros for k, v
     store_strip<T>(kd, d * 32, a.D, dk[d], a.scale * one / factor);
     store_strip<T>(vd, d * 32, a.D, dv[d], one);
   }
 }
 
-// dq = the sum over the splits, in split order
-template <class T>
+// Joins the splits of dq as attn_join_kernel does the forward's; KEYS: also what delta was off by (attn_dq_kernel)
+template <class T, bool WIDE>
 __global__ __launch_bounds__(256) void attn_sum_kernel(Attn a, int64_t n_rows) {
-  const int quads = a.D / 4;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (id >= n_rows * quads) return;
-  const int64_t rid = id / quads;
-  const int d = (int)(id - rid * quads) * 4;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < a.splits; ++i) {
-    const float4 v = *reinterpret_cast<const float4*>(a.part + (i * n_rows + rid) * a.D + d);
-    acc[0] += v.x;
-    acc[1] += v.y;
-    acc[2] += v.z;
-    acc[3] += v.w;
+  constexpr bool KEYS = Terms<T>::NP == 1;
+  constexpr int N = KEYS ? 9 : 4;                      // four columns of sum ds k, of sum p k, and sum ds
+  const int quads = a.D / 4, width = KEYS ? 2 * a.D : a.D;
+  int64_t rid;
+  int quad, first = 0, every = 1;
+  if constexpr (WIDE) {
+    rid = blockIdx.x;
+    quad = threadIdx.x & 31;
+    first = threadIdx.x >> 5;
+    every = 8;
+  } else {
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= n_rows * quads) return;
+    rid = id / quads;
+    quad = (int)(id - rid * quads);
   }
-  const int H = a.Hkv * a.G;
-  const int64_t bhead = rid / a.Tq;
-  const RowAt ra = {(int)(rid - bhead * a.Tq), (int)(bhead % H)};
-  T* dst = const_cast<T*>(row_ptr<T>(a.dq, (int)(bhead / H), ra)) + d;
+  const int d = quad * 4;
+  float acc[N];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) dst[j] = (T)acc[j];
+  for (int j = 0; j < N; ++j) acc[j] = 0.f;
+  if (quad < quads)
+    for (int i = first; i < a.splits; i += every) {
+      const float* from = a.part + (i * n_rows + rid) * width + d;
+      const float4 v = *reinterpret_cast<const float4*>(from);
+      acc[0] += v.x;
+      acc[1] += v.y;
+      acc[2] += v.z;
+      acc[3] += v.w;
+      if constexpr (KEYS) {
+        const float4 k = *reinterpret_cast<const float4*>(from + a.D);
+        acc[4] += k.x;
+        acc[5] += k.y;
+        acc[6] += k.z;
+        acc[7] += k.w;
+        acc[8] += a.part_lse[i * n_rows + rid];
+      }
+    }
+  if constexpr (WIDE) {
+    __shared__ float red[8][32][N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) red[first][quad][j] = acc[j];
+    __syncthreads();
+    if (first || quad >= quads) return;
+    for (int g = 1; g < 8; ++g)
+#pragma unroll
+      for (int j = 0; j < N; ++j) acc[j] += red[g][quad][j];
+  }
+  if (KEYS && d == 0) a.delta[rid] += acc[N - 1];
+  T* dst = row_of<T>(a, a.dq, rid) + d;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) dst[j] = (T)(a.scale * (KEYS ? acc[j] - acc[N - 1] * acc[KEYS ? 4 + j : 0] : acc[j]));
 }
 
 // ---- few query rows --------------------------------------------------------------------------------------------------
@@ -899,8 +1127,8 @@ __global__ __launch_bounds__(NW * 64) void attn_rows_fwd_kernel(Attn a) {
 template <class T, int R, int LPK>
 __device__ static inline void rows_write_kv(const Attn& a, int b, int hk, int k0, int k1, int live, int from,
                                             const float* kept, int64_t apart, const float (&q)[R][Packet<T>::V],
-                                            const float (&g)[R][Packet<T>::V], const float (&delta)[R], int wave,
-                                            int waves) {
+                                            const float (&g)[R][Packet<T>::V], const float (&delta)[R], bool lone,
+                                            int wave, int waves) {
   constexpr int V = Packet<T>::V, KPW = 64 / LPK;
   const int lane = threadIdx.x & 63, sub = lane % LPK, slot = lane / LPK, d = sub * V;
   T* kp = (T*)a.dk.p + (int64_t)b * a.dk.b + (int64_t)hk * a.dk.h + d;
@@ -913,7 +1141,7 @@ __device__ static inline void rows_write_kv(const Attn& a, int b, int hk, int k0
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const float p = kept[(int64_t)(key - from) * R + r], dp = kept[apart + (int64_t)(key - from) * R + r];
-        const float ds = p == 0.f ? 0.f : p * (dp - delta[r]) * a.scale;
+        const float ds = p == 0.f || lone ? 0.f : p * (dp - delta[r]) * a.scale;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           dk[j] = fmaf(ds, q[r][j], dk[j]);
@@ -1038,6 +1266,7 @@ __global__ __launch_bounds__(NW * 64) void attn_rows_bwd_kernel(Attn a) {
   } else if constexpr (FUSED) {
     __syncthreads();                                   // p and dp of this wave's other lanes
   }
+  const bool lone = FUSED && lone_key(a, pa.b);
   if (wave == 0 && slot == 0)
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -1047,7 +1276,7 @@ __global__ __launch_bounds__(NW * 64) void attn_rows_bwd_kernel(Attn a) {
       if constexpr (FUSED) {
         float dq[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) dq[j] = a.scale * (A[r][j] - delta[r] * S[r][j]);
+        for (int j = 0; j < V; ++j) dq[j] = lone ? 0.f : a.scale * (A[r][j] - delta[r] * S[r][j]);
         if (in_d) *reinterpret_cast<uint4*>((T*)a.dq.p + (int64_t)pa.b * a.dq.b + (int64_t)ra.t * a.dq.t + (int64_t)ra.h * a.dq.h + d) = Packet<T>::pack(dq);
       } else {
         float* part = a.part + ((int64_t)pa.split * ((int64_t)a.B * a.Hkv * a.rows) + rid) * (2 * a.D + 1);
@@ -1058,7 +1287,7 @@ __global__ __launch_bounds__(NW * 64) void attn_rows_bwd_kernel(Attn a) {
       }
     }
   if constexpr (FUSED)
-    rows_write_kv<T, R, LPK>(a, pa.b, pa.hk, 0, a.Tk, pa.k1, 0, kept, apart, q, g, delta, wave, NW);
+    rows_write_kv<T, R, LPK>(a, pa.b, pa.hk, 0, a.Tk, pa.k1, 0, kept, apart, q, g, delta, lone, wave, NW);
 }
 
 // Pass two over kept p and dp: block `chunk` of a pair writes its keys; chunk 0 also dq
@@ -1068,6 +1297,7 @@ __global__ __launch_bounds__(256) void attn_rows_kv_kernel(Attn a, int chunks, i
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LPK, slot = lane / LPK, d = sub * V;
   const int chunk = blockIdx.x % chunks, pair = blockIdx.x / chunks, b = pair / a.Hkv, hk = pair - b * a.Hkv;
   const bool in_d = d < a.D;
+  const bool lone = lone_key(a, b);
   float q[R][V], g[R][V], delta[R];
   const int64_t n_rows = (int64_t)a.B * a.Hkv * a.rows;
 #pragma unroll
@@ -1090,7 +1320,7 @@ __global__ __launch_bounds__(256) void attn_rows_kv_kernel(Attn a, int chunks, i
             A += part[d + j];
             S += part[a.D + d + j];
           }
-          dq[j] = a.scale * (A - delta[r] * S);
+          dq[j] = lone ? 0.f : a.scale * (A - delta[r] * S);
         }
         *reinterpret_cast<uint4*>((T*)a.dq.p + (int64_t)b * a.dq.b + (int64_t)ra.t * a.dq.t + (int64_t)ra.h * a.dq.h + d) = Packet<T>::pack(dq);
       }
@@ -1098,7 +1328,7 @@ __global__ __launch_bounds__(256) void attn_rows_kv_kernel(Attn a, int chunks, i
   }
   const int k0 = chunk * per_chunk, k1 = min(a.Tk, k0 + per_chunk);
   rows_write_kv<T, R, LPK>(a, b, hk, k0, k1, key_count(a, b), 0, a.kept + (int64_t)pair * a.Tk * R,
-                           (int64_t)a.B * a.Hkv * a.Tk * R, q, g, delta, wave, 4);
+                           (int64_t)a.B * a.Hkv * a.Tk * R, q, g, delta, lone, wave, 4);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
@@ -1110,11 +1340,11 @@ static int rows_lanes(int D, int dtype) {
 static int rows_step_keys(int D, int dtype) { return 64 / rows_lanes(D, dtype); }
 static int padded_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
 static int pass_rows(int rows) { return rows <= 32 ? 32 : 128; }          // query rows of a block: one wave or four
-static int tile_keys(int dtype) { return dtype == CTR_F32 ? 32 : 64; }
 
-// Splits of the key axis: only where the row tiles alone leave most of the chip idle, and never below 256 keys each.
+// Splits of the key axis: only where the row tiles alone leave part of the chip without a block (every split writes its
+// share of the result as fp32, which is read again), and never below 256 keys each.
 static int key_splits(int64_t blocks, int Tk) {
-  const int64_t want = blocks < 1 ? 1 : 1024 / blocks, most = Tk / 256;
+  const int64_t want = blocks < 1 ? 1 : 512 / blocks, most = Tk / 256;
   const int64_t n = want < most ? want : most;
   return (int)(n < 1 ? 1 : n);
 }
@@ -1156,7 +1386,7 @@ static size_t bwd_ws_first(const Attn& a) {
 }
 static size_t bwd_ws(const Attn& a) {
   if (a.few) return rows_fused(a) ? 256 : bwd_ws_first(a) + (size_t)a.B * a.Hkv * a.Tk * a.few * 8 + 256;
-  return bwd_ws_first(a) + (a.splits > 1 ? (size_t)a.splits * total_rows(a) * a.D * 4 : 0) + 256;
+  return bwd_ws_first(a) + (a.splits > 1 ? (size_t)a.splits * total_rows(a) * (2 * a.D + 1) * 4 : 0) + 256;
 }
 
 static int attn_shape(const char* what, const ctr_attn_t* s, Attn* a) {
@@ -1260,30 +1490,36 @@ static void rows_bwd_launch(const Attn& a, hipStream_t st) {
 #undef ROWS_BWD
 }
 
+static bool tile_is_near(const View4& w, int64_t rows, int bytes) {
+  return rows * (w.t + w.h) * bytes < ((int64_t)1 << 31);
+}
+
+template <class T>
+static void join_launch(const Attn& a, hipStream_t st) {
+  if (a.splits == 1) return;
+  const int64_t n = total_rows(a);
+  if (a.splits >= JOIN_WIDE) attn_join_kernel<T, true><<<(unsigned)n, 256, 0, st>>>(a, n);
+  else attn_join_kernel<T, false><<<(unsigned)cdiv(n * (a.D / 4), 256), 256, 0, st>>>(a, n);
+}
+
 template <class T>
 static void attn_fwd_launch(const Attn& a, hipStream_t st) {
   if (a.few) {
     if (a.few == 1) rows_fwd_launch<T, 1>(a, st);
     else if (a.few == 2) rows_fwd_launch<T, 2>(a, st);
     else rows_fwd_launch<T, 4>(a, st);
-    if (a.splits > 1) {
-      const int64_t n = total_rows(a);
-      attn_join_kernel<T><<<(unsigned)cdiv(n * (a.D / 4), 256), 256, 0, st>>>(a, n);
-    }
+    join_launch<T>(a, st);
     return;
   }
   constexpr int KT = sizeof(T) == 4 ? 32 : 64;
   const unsigned blocks = (unsigned)((int64_t)a.row_tiles * a.B * a.Hkv * a.splits);
   const bool one = pass_rows(a.rows) == 32;
 #define ATTN_FWD(T_, DP_)                                                         \
-  if (one) attn_fwd_kernel<T_, DP_, 1, 1, 32><<<blocks, 64, 0, st>>>(a);          \
-  else attn_fwd_kernel<T_, DP_, 4, 1, KT><<<blocks, 256, 0, st>>>(a)
+  if (one) attn_fwd_kernel<T_, DP_, 1, 32><<<blocks, 64, 0, st>>>(a);          \
+  else attn_fwd_kernel<T_, DP_, 4, (DP_ > 64 ? 32 : KT)><<<blocks, 256, 0, st>>>(a)
   ATTN_DIM(T, a.D, ATTN_FWD);
 #undef ATTN_FWD
-  if (a.splits > 1) {
-    const int64_t n = total_rows(a);
-    attn_join_kernel<T><<<(unsigned)cdiv(n * (a.D / 4), 256), 256, 0, st>>>(a, n);
-  }
+  join_launch<T>(a, st);
 }
 
 template <class T>
@@ -1300,17 +1536,18 @@ static void attn_bwd_launch(const Attn& a, hipStream_t st) {
   if (blocks) {
 #define ATTN_DQ(T_, DP_)                                                          \
   if (one) attn_dq_kernel<T_, DP_, 1, 32><<<blocks, 64, 0, st>>>(a);              \
-  else attn_dq_kernel<T_, DP_, 4, KT><<<blocks, 256, 0, st>>>(a)
+  else attn_dq_kernel<T_, DP_, 4, (DP_ > 64 ? 32 : KT)><<<blocks, 256, 0, st>>>(a)
     ATTN_DIM(T, a.D, ATTN_DQ);
 #undef ATTN_DQ
     if (a.splits > 1) {
       const int64_t n = total_rows(a);
-      attn_sum_kernel<T><<<(unsigned)cdiv(n * (a.D / 4), 256), 256, 0, st>>>(a, n);
+      if (a.splits >= JOIN_WIDE) attn_sum_kernel<T, true><<<(unsigned)n, 256, 0, st>>>(a, n);
+      else attn_sum_kernel<T, false><<<(unsigned)cdiv(n * (a.D / 4), 256), 256, 0, st>>>(a, n);
     }
   }
   const unsigned kblocks = (unsigned)((int64_t)a.key_tiles * a.B * a.Hkv);
   if (kblocks) {
-#define ATTN_DKV(T_, DP_) attn_dkv_kernel<T_, DP_, 4, 32><<<kblocks, 256, 0, st>>>(a)
+#define ATTN_DKV(T_, DP_) attn_dkv_kernel<T_, DP_, 4, (sizeof(T_) == 2 && DP_ <= 64 ? 64 : 32)><<<kblocks, 256, 0, st>>>(a)
     ATTN_DIM(T, a.D, ATTN_DKV);
 #undef ATTN_DKV
   }
@@ -1346,6 +1583,7 @@ extern "C" int ctr_cross_attn_fwd(const ctr_attn_t* s, const ctr_heads_t* q, con
     set_error("%s: workspace %zu < %zu", what, workspace_bytes, fwd_ws(a));
     return CTR_EWORKSPACE;
   }
+  a.near = tile_is_near(a.k, 128, type_bytes(s->dtype)) && tile_is_near(a.v, 128, type_bytes(s->dtype));
   if (a.splits > 1) {
     a.part = (float*)align_up((size_t)workspace, 256);
     a.part_lse = a.part + (size_t)a.splits * total_rows(a) * a.D;
@@ -1381,6 +1619,8 @@ extern "C" int ctr_cross_attn_bwd(const ctr_attn_t* s, const ctr_heads_t* dout, 
     return CTR_EWORKSPACE;
   }
   a.lse = const_cast<float*>(lse);
+  a.near = true;
+  for (const View4* w : {&a.k, &a.v, &a.q, &a.dout}) a.near = a.near && tile_is_near(*w, 128, type_bytes(s->dtype));
   float* ws = (float*)align_up((size_t)workspace, 256);
   if (a.few) {
     a.part = ws;
@@ -1388,6 +1628,7 @@ extern "C" int ctr_cross_attn_bwd(const ctr_attn_t* s, const ctr_heads_t* dout, 
   } else {
     a.delta = ws;
     a.part = ws + bwd_ws_first(a) / 4;
+    a.part_lse = a.part + (size_t)a.splits * total_rows(a) * 2 * a.D;
   }
   hipStream_t st = (hipStream_t)stream;
   if (s->dtype == CTR_F32) attn_bwd_launch<float>(a, st);

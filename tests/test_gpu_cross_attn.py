@@ -190,6 +190,23 @@ def test_gradients_against_differences(Tq):
         assert abs((ends[0] - ends[1]) / (2 * h) - slope) <= allowed, name
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('Tq', [1, 40])
+@pytest.mark.parametrize('left', ['one key', 'lengths', 'mask'])
+def test_a_single_key_has_no_gradient_of_its_score(dtype, Tq, left):
+    """softmax over one key is 1 whatever the score: dq and dk are zeros exactly."""
+    Tk = 1 if left == 'one key' else 2600
+    q, k, v, dout = _make(2, Tq, Tk, 4, 2, 64, dtype, seed=21)
+    sl = torch.tensor([1, 1], dtype=torch.int32, device=DEV) if left == 'lengths' else None
+    mask = None
+    if left == 'mask':
+        mask = torch.zeros(2, Tk, dtype=torch.bool, device=DEV)
+        mask[0, 2000] = mask[1, 7] = True
+    got = _run(q, k, v, dout, sl, mask)
+    _check(got, attention(q, k, v, sl, mask, dout=dout))
+    assert (got['dq'] == 0).all() and (got['dk'] == 0).all()
+
+
 def test_no_queries_no_keys_no_samples():
     from recommendation_amd import ops
     for dtype in TYPES:
