@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # CTRHIP_LIB: another build of the same library (A/B timing of a kernel change); default: the in-tree build
@@ -44,16 +45,9 @@ class Epilogue(C.Structure):
                 ('b_amax_floor', C.c_float), ('c_amax_out', C.c_void_p)]
 
 
-class AttnShape(C.Structure):
-    _fields_ = [('B', C.c_int), ('Tq', C.c_int), ('Tk', C.c_int), ('H', C.c_int), ('Hkv', C.c_int), ('D', C.c_int),
-                ('dtype', C.c_int), ('scale', C.c_float), ('sl', C.c_void_p), ('mask', C.c_void_p),
-                ('mask_ld', C.c_int64)]
-
-
-class Heads(C.Structure):
-    _fields_ = [('p', C.c_void_p), ('stride_b', C.c_int64), ('stride_t', C.c_int64), ('stride_h', C.c_int64)]
-
-
+# ctr_attn_t (B, Tq, Tk, H, Hkv, D, dtype, scale, sl, mask, mask_ld) and ctr_heads_t (p, stride_b, stride_t, stride_h)
+ATTN = struct.Struct('@7if2Pq')
+HEADS = struct.Struct('@P3q')
 F32, BF16, F16 = 0, 1, 2     # CTR_F32 / CTR_BF16 / CTR_F16
 OPT_GRAD_ONLY, OPT_ADAM, OPT_ADAGRAD, OPT_SGD, OPT_FTRL = 0, 1, 2, 3, 4
 COMM_ID_BYTES = 128          # CTR_COMM_ID_BYTES

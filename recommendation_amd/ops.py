@@ -12,7 +12,7 @@ import math
 import torch
 
 from . import _lib
-from ._lib import AttnShape, Dropout, Epilogue, FmBwd, Heads, Opt, check
+from ._lib import Dropout, Epilogue, FmBwd, Opt, check
 
 KEEP_ONE = 1 << 24
 
@@ -1202,83 +1202,91 @@ def mean_positive_diff(a, b, out):
 
 
 # ------------------------------------------------------------------ attention towers over behaviour sequences
+# These calls run on small tensors too (a candidate, a serving batch), where the host's share of a call is most of its
+# time: their checks read each property once, and the structs of the C ABI are packed, not built field by field.
 DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
 def _dtype(t, name):
-    if t.dtype not in DTYPES:
+    dt = DTYPES.get(t.dtype)
+    if dt is None:
         raise TypeError('%s: expected float32, bfloat16 or float16, got %s' % (name, t.dtype))
-    return DTYPES[t.dtype]
+    return dt
 
 
-def _here(*named):
-    """Every tensor on the current device: the kernels run on its current stream."""
-    dev = None
-    for t, name in named:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError('%s must live on the GPU (libctrhip has no CPU path)' % name)
-        if dev is None:
-            dev = torch.cuda.current_device()
-        if t.device.index != dev:
-            raise ValueError('%s lives on %s, the current device is cuda:%d' % (name, t.device, dev))
+def _here(names, *tensors):
+    """The current stream of the device that every tensor (None: not given) lies on; it must be the current one."""
+    dev = tensors[0].get_device()
+    for i, t in enumerate(tensors):
+        if t is not None and (dev < 0 or t.get_device() != dev):
+            name, at = names.split()[i], t.device
+            if t.get_device() < 0:
+                raise ValueError('%s must live on the GPU (libctrhip has no CPU path)' % name)
+            raise ValueError('%s lives on %s, %s on cuda:%d' % (name, at, names.split()[0], dev))
+    if torch._C._cuda_getDevice() != dev:
+        raise ValueError('%s lives on cuda:%d, the current device is cuda:%d'
+                         % (names.split()[0], dev, torch._C._cuda_getDevice()))
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _heads(t, shape, dtype, name):
-    if tuple(t.shape) != shape:
+    """ctr_heads_t of a [B, T, heads, D] view (the stride of an axis of one plays no part)."""
+    if t.shape != shape:
         raise ValueError('%s must be %s, got %s' % (name, list(shape), list(t.shape)))
     if t.dtype != dtype:
         raise TypeError('%s: expected %s, got %s' % (name, dtype, t.dtype))
     sb, st, sh, sd = t.stride()
     if sd != 1:
         raise ValueError('%s must have a contiguous last dimension' % name)
-    return Heads(t.data_ptr(), sb if shape[0] > 1 else 0, st if shape[1] > 1 else 0, sh if shape[2] > 1 else 0)
+    return _lib.HEADS.pack(t.data_ptr(), sb if shape[0] > 1 else 0, st if shape[1] > 1 else 0, sh if shape[2] > 1 else 0)
 
 
-def _attn_args(q, k, v, sl, mask, scale):
-    """(shape struct, q's shape, k's shape) of a cross-attention call, checked."""
+def _attn_args(q, k, sl, mask, scale):
+    """(ctr_attn_t, q's shape, k's shape) of a cross-attention call, checked."""
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError('q must be [B, Tq, H, D] and k [B, Tk, Hkv, D]')
-    qs, ks = tuple(q.shape), tuple(k.shape)
-    if ks[0] != qs[0] or ks[3] != qs[3] or ks[2] < 1 or qs[2] < 1 or qs[2] % ks[2]:
+    qs, ks = q.shape, k.shape
+    (B, Tq, H, D), (Bk, Tk, Hkv, Dk) = qs, ks
+    if Bk != B or Dk != D or Hkv < 1 or H < 1 or H % Hkv:
         raise ValueError('q %s and k %s do not belong together (one batch, one head size, H a multiple of Hkv)'
                          % (list(qs), list(ks)))
-    B, Tk, D = qs[0], ks[1], qs[3]
     if D % 8 or not 8 <= D <= 128:
         raise ValueError('head size %d is not a multiple of 8 up to 128' % D)
+    if Tq * (H // Hkv) >= 1 << 30 or Tk >= 1 << 30 or B * H >= 1 << 30:
+        raise ValueError('more than 2^30 query rows, keys or heads')
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not 0.0 < scale <= 3e38:
         raise ValueError('scale must be positive and finite')
-    mp, mld = None, 0
+    mp = mld = sp = 0
     if mask is not None:
         if mask.dtype not in (torch.bool, torch.uint8):
             raise TypeError('mask: expected bool or uint8, got %s' % mask.dtype)
-        if tuple(mask.shape) != (B, Tk) or (Tk > 1 and mask.stride(1) != 1):
+        if mask.shape != (B, Tk) or (Tk > 1 and mask.stride(1) != 1):
             raise ValueError('mask must be [B, Tk] with a contiguous last dimension')
         mp, mld = mask.data_ptr(), mask.stride(0) if B > 1 else 0
-    sp = None
     if sl is not None:
-        if sl.dtype != torch.int32 or tuple(sl.shape) != (B,) or not sl.is_contiguous():
+        if sl.dtype != torch.int32 or sl.shape != (B,) or not sl.is_contiguous():
             raise ValueError('sl must be a contiguous int32 [B] tensor')
         sp = sl.data_ptr()
-    return AttnShape(B, qs[1], Tk, qs[2], ks[2], D, _dtype(q, 'q'), scale, sp, mp, mld), qs, ks
+    return _lib.ATTN.pack(B, Tq, Tk, H, Hkv, D, _dtype(q, 'q'), scale, sp, mp, mld), qs, ks
 
 
 def _lse(lse, qs):
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (qs[0], qs[2], qs[1]) or not lse.is_contiguous():
+    if lse.dtype != torch.float32 or lse.shape != (qs[0], qs[2], qs[1]) or not lse.is_contiguous():
         raise ValueError('lse must be contiguous float32 [B, H, Tq]')
-    return C.c_void_p(lse.data_ptr())
+    return lse.data_ptr()
 
 
-def _apart(outs, ins):
+def _apart(names, outs, ins):
     """No output starts where another tensor of the call does (views that merely share a buffer are fine)."""
-    seen = {t.data_ptr(): name for t, name in ins if t.numel()}
-    for t, name in outs:
-        if t.numel():
-            if t.data_ptr() in seen:
-                raise ValueError('%s shares its memory with %s' % (name, seen[t.data_ptr()]))
-            seen[t.data_ptr()] = name
+    seen = [t.data_ptr() for t in outs + ins if t.numel()]
+    if len(set(seen[:len(outs)])) == len(outs) and not set(seen[:len(outs)]) & set(seen[len(outs):]):
+        return
+    ptrs = [(t.data_ptr() if t.numel() else None) for t in outs + ins]
+    for i in range(len(outs)):
+        for j in range(len(ptrs)):
+            if j != i and ptrs[i] is not None and ptrs[i] == ptrs[j]:
+                raise ValueError('%s shares its memory with %s' % (names.split()[i], names.split()[j]))
 
 
 @_timed
@@ -1288,43 +1296,44 @@ def cross_attn_fwd(q, k, v, out, *, lse=None, sl=None, mask=None, scale=None, ws
     up to 128, rows on 16-byte boundaries, other strides free).  sl (int32 [B]): only the first sl[b] keys; mask (bool or
     uint8 [B,Tk]): only the keys that are set.  A row without keys gives zeros.  scale: 1 / sqrt(D) by default.
     lse (float32 [B,H,Tq]): the logarithm of every softmax's sum, kept for cross_attn_bwd."""
-    sh, qs, ks = _attn_args(q, k, v, sl, mask, scale)
-    hq, hk, hv = _heads(q, qs, q.dtype, 'q'), _heads(k, ks, q.dtype, 'k'), _heads(v, ks, q.dtype, 'v')
-    ho = _heads(out, qs, q.dtype, 'out')
+    sh, qs, ks = _attn_args(q, k, sl, mask, scale)
+    t = q.dtype
+    hq, hk, hv, ho = _heads(q, qs, t, 'q'), _heads(k, ks, t, 'k'), _heads(v, ks, t, 'v'), _heads(out, qs, t, 'out')
     lp = None if lse is None else _lse(lse, qs)
-    _apart(((out, 'out'),), ((q, 'q'), (k, 'k'), (v, 'v')))
-    _here((q, 'q'), (k, 'k'), (v, 'v'), (out, 'out'), (lse, 'lse'), (sl, 'sl'), (mask, 'mask'))
-    L, r = lib(), C.byref
-    wp, wn = ws.get(L.ctr_cross_attn_fwd_workspace_bytes(r(sh)))
-    check(L.ctr_cross_attn_fwd(r(sh), r(hq), r(hk), r(hv), r(ho), lp, wp, wn, _stream()), 'ctr_cross_attn_fwd')
+    _apart('out q k v', (out,), (q, k, v))
+    stream = _here('q k v out lse sl mask', q, k, v, out, lse, sl, mask)
+    L = lib()
+    wp, wn = ws.get(L.ctr_cross_attn_fwd_workspace_bytes(sh))
+    check(L.ctr_cross_attn_fwd(sh, hq, hk, hv, ho, lp, wp, wn, stream), 'ctr_cross_attn_fwd')
 
 
 @_timed
 def cross_attn_bwd(dout, q, k, v, out, lse, dq, dk, dv, *, sl=None, mask=None, scale=None, ws):
     """Gradients of cross_attn_fwd from its own inputs, out and lse (the same sl, mask and scale).  dq, dk and dv are
     overwritten; keys that no row attends to get zeros; heads that share keys add up in dk and dv."""
-    sh, qs, ks = _attn_args(q, k, v, sl, mask, scale)
+    sh, qs, ks = _attn_args(q, k, sl, mask, scale)
     t = q.dtype
     hg, hq, hk, hv = _heads(dout, qs, t, 'dout'), _heads(q, qs, t, 'q'), _heads(k, ks, t, 'k'), _heads(v, ks, t, 'v')
     ho, gq, gk, gv = _heads(out, qs, t, 'out'), _heads(dq, qs, t, 'dq'), _heads(dk, ks, t, 'dk'), _heads(dv, ks, t, 'dv')
     lp = _lse(lse, qs)
-    _apart(((dq, 'dq'), (dk, 'dk'), (dv, 'dv')), ((dout, 'dout'), (q, 'q'), (k, 'k'), (v, 'v'), (out, 'out')))
-    _here((dout, 'dout'), (q, 'q'), (k, 'k'), (v, 'v'), (out, 'out'), (lse, 'lse'), (dq, 'dq'), (dk, 'dk'), (dv, 'dv'),
-          (sl, 'sl'), (mask, 'mask'))
-    L, r = lib(), C.byref
-    wp, wn = ws.get(L.ctr_cross_attn_bwd_workspace_bytes(r(sh)))
-    check(L.ctr_cross_attn_bwd(r(sh), r(hg), r(hq), r(hk), r(hv), r(ho), lp, r(gq), r(gk), r(gv), wp, wn, _stream()),
-          'ctr_cross_attn_bwd')
+    _apart('dq dk dv dout q k v out', (dq, dk, dv), (dout, q, k, v, out))
+    stream = _here('dout q k v out lse dq dk dv sl mask', dout, q, k, v, out, lse, dq, dk, dv, sl, mask)
+    L = lib()
+    wp, wn = ws.get(L.ctr_cross_attn_bwd_workspace_bytes(sh))
+    check(L.ctr_cross_attn_bwd(sh, hg, hq, hk, hv, ho, lp, gq, gk, gv, wp, wn, stream), 'ctr_cross_attn_bwd')
 
 
 def _ln_rows(t, shape, dtype, name):
-    if t.dim() != 2 or tuple(t.shape) != shape:
+    """(address, leading dimension)"""
+    if t.shape != shape:
         raise ValueError('%s must be %s, got %s' % (name, list(shape), list(t.shape)))
     if t.dtype != dtype:
         raise TypeError('%s: expected %s, got %s' % (name, dtype, t.dtype))
-    if t.stride(1) != 1 and shape[1] > 1 or (shape[0] > 1 and t.stride(0) < shape[1]):
+    ld, one = t.stride()
+    rows, cols = shape
+    if (one != 1 and cols > 1) or (rows > 1 and ld < cols):
         raise ValueError('%s must have a contiguous last dimension and rows that do not overlap' % name)
-    return C.c_void_p(t.data_ptr()), int(t.stride(0)) if shape[0] > 1 else shape[1]
+    return t.data_ptr(), ld if rows > 1 else cols
 
 
 def _ln_vec(t, n, name):
@@ -1334,13 +1343,13 @@ def _ln_vec(t, n, name):
         raise TypeError('%s: expected torch.float32, got %s' % (name, t.dtype))
     if t.numel() != n or not t.is_contiguous():
         raise ValueError('%s must be contiguous with %d entries' % (name, n))
-    return C.c_void_p(t.data_ptr())
+    return t.data_ptr()
 
 
 def _ln_shape(x):
-    if x.dim() != 2 or x.shape[1] < 1 or x.shape[1] >= 1 << 30:
+    if x.dim() != 2 or not 1 <= x.shape[1] < 1 << 30:
         raise ValueError('layer norm wants a [rows, cols] view with at least one column')
-    return tuple(x.shape)
+    return x.shape
 
 
 @_timed
@@ -1349,14 +1358,13 @@ def layer_norm_fwd(x, y, *, gamma=None, beta=None, eps=1e-5, mean=None, rstd=Non
     stride).  gamma, beta: float32 [cols] or None; mean, rstd: float32 [rows], kept for layer_norm_bwd.  y may be x."""
     rows, cols = shape = _ln_shape(x)
     dt = _dtype(x, 'x')
-    if not 0.0 <= eps < float('inf'):
+    if not 0.0 <= eps < math.inf:
         raise ValueError('eps must be finite and not negative')
     (xp, xld), (yp, yld) = _ln_rows(x, shape, x.dtype, 'x'), _ln_rows(y, shape, x.dtype, 'y')
     ga, be = _ln_vec(gamma, cols, 'gamma'), _ln_vec(beta, cols, 'beta')
     mp, rp = _ln_vec(mean, rows, 'mean'), _ln_vec(rstd, rows, 'rstd')
-    _here((x, 'x'), (y, 'y'), (gamma, 'gamma'), (beta, 'beta'), (mean, 'mean'), (rstd, 'rstd'))
-    check(lib().ctr_layer_norm_fwd(xp, xld, rows, cols, dt, ga, be, float(eps), yp, yld, mp, rp, _stream()),
-          'ctr_layer_norm_fwd')
+    stream = _here('x y gamma beta mean rstd', x, y, gamma, beta, mean, rstd)
+    check(lib().ctr_layer_norm_fwd(xp, xld, rows, cols, dt, ga, be, eps, yp, yld, mp, rp, stream), 'ctr_layer_norm_fwd')
 
 
 @_timed
@@ -1371,13 +1379,11 @@ def layer_norm_bwd(dy, x, mean, rstd, dx, *, gamma=None, dgamma=None, dbeta=None
         raise ValueError('layer_norm_bwd needs the mean and rstd that layer_norm_fwd kept')
     mp, rp, ga = _ln_vec(mean, rows, 'mean'), _ln_vec(rstd, rows, 'rstd'), _ln_vec(gamma, cols, 'gamma')
     dg, db = _ln_vec(dgamma, cols, 'dgamma'), _ln_vec(dbeta, cols, 'dbeta')
-    _here((dy, 'dy'), (x, 'x'), (mean, 'mean'), (rstd, 'rstd'), (dx, 'dx'), (gamma, 'gamma'), (dgamma, 'dgamma'),
-          (dbeta, 'dbeta'))
-    wp, wn = None, 0
-    if dgamma is not None or dbeta is not None:
-        wp, wn = ws.get(lib().ctr_layer_norm_bwd_workspace_bytes(rows, cols))
-    check(lib().ctr_layer_norm_bwd(gp, gld, xp, xld, mp, rp, rows, cols, dt, ga, dp, dld, int(bool(accumulate)), dg, db,
-                                   wp, wn, _stream()), 'ctr_layer_norm_bwd')
+    stream = _here('dy x mean rstd dx gamma dgamma dbeta', dy, x, mean, rstd, dx, gamma, dgamma, dbeta)
+    L = lib()
+    wp, wn = (None, 0) if dg is None and db is None else ws.get(L.ctr_layer_norm_bwd_workspace_bytes(rows, cols))
+    check(L.ctr_layer_norm_bwd(gp, gld, xp, xld, mp, rp, rows, cols, dt, ga, dp, dld, 1 if accumulate else 0, dg, db, wp,
+                               wn, stream), 'ctr_layer_norm_bwd')
 
 
 class GradList:
@@ -1396,6 +1402,7 @@ class GradList:
         self.counts = (C.c_int64 * n)(*[t.numel() for t in self.tensors])
         self.dtypes = (C.c_int * n)(*[DTYPES[t.dtype] for t in self.tensors])
         self.kinds = [(t.numel(), t.dtype) for t in self.tensors]
+        self.places = [t.data_ptr() for t in self.tensors]
         spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), i)
                        for i, t in enumerate(self.tensors) if t.numel())
         for (_, end, i), (start, _, j) in zip(spans, spans[1:]):
@@ -1422,20 +1429,23 @@ class GradList:
 
 
 def _grad_list(grads):
-    g = grads if isinstance(grads, GradList) else GradList(grads)
-    if g.device is not None and g.device != torch.cuda.current_device():
-        raise ValueError('the gradients live on cuda:%d, the current device is cuda:%d'
-                         % (g.device, torch.cuda.current_device()))
-    return g
+    return grads if isinstance(grads, GradList) else GradList(grads)
 
 
-def _norm_ptr(norm):
-    if norm is None:
-        return None
-    if norm.dtype != torch.float32 or norm.numel() != 1:
-        raise ValueError('norm must be a float32 tensor of one element')
-    _here((norm, 'norm'))
-    return C.c_void_p(norm.data_ptr())
+def _grad_call(g, norm):
+    """(address of norm, the current stream) of a call on the list g."""
+    np_ = None
+    if norm is not None:
+        if norm.dtype != torch.float32 or norm.numel() != 1:
+            raise ValueError('norm must be a float32 tensor of one element')
+        if norm.get_device() < 0:
+            raise ValueError('norm must live on the GPU (libctrhip has no CPU path)')
+        np_ = norm.data_ptr()
+    dev = torch.cuda.current_device()
+    for d in (g.device, None if norm is None else norm.get_device()):
+        if d is not None and d != dev:
+            raise ValueError('the gradients or norm live on cuda:%d, the current device is cuda:%d' % (d, dev))
+    return np_, torch._C._cuda_getCurrentRawStream(dev)
 
 
 @_timed
@@ -1444,8 +1454,9 @@ def grad_norm(grads, norm, *, ws):
     g = _grad_list(grads)
     if norm is None:
         raise ValueError('grad_norm needs a norm tensor')
+    np_, stream = _grad_call(g, norm)
     wp, wn = ws.get(lib().ctr_grad_norm_workspace_bytes(len(g)))
-    check(lib().ctr_grad_norm(g.ptrs, g.counts, g.dtypes, len(g), _norm_ptr(norm), wp, wn, _stream()), 'ctr_grad_norm')
+    check(lib().ctr_grad_norm(g.ptrs, g.counts, g.dtypes, len(g), np_, wp, wn, stream), 'ctr_grad_norm')
 
 
 @_timed
@@ -1461,8 +1472,9 @@ def clip_grads(grads, max_norm, norm=None, *, out=None, ws):
     if o is not g:
         if o.kinds != g.kinds:
             raise ValueError('out must hold tensors of the same sizes and dtypes')
-        if list(o.ptrs) != list(g.ptrs) and o.overlaps(g):
+        if o.places != g.places and o.overlaps(g):
             raise ValueError('out shares memory with the gradients without being them')
+    np_, stream = _grad_call(g, norm)
     wp, wn = ws.get(lib().ctr_grad_norm_workspace_bytes(len(g)))
-    check(lib().ctr_clip_grads(g.ptrs, o.ptrs, g.counts, g.dtypes, len(g), max_norm, _norm_ptr(norm), wp, wn, _stream()),
+    check(lib().ctr_clip_grads(g.ptrs, o.ptrs, g.counts, g.dtypes, len(g), max_norm, np_, wp, wn, stream),
           'ctr_clip_grads')
