@@ -15,8 +15,8 @@ constexpr int LN_LANE_ELEMS = 16;
 constexpr int LN_MAX_COLS = 1024 * LN_LANE_ELEMS;     // a block of 1024 lanes holds the row
 constexpr int LN_STRIP = 64;                          // rows per block of the column sums of wider rows
 
-// sum of v over the LPR lanes of a row; LPR > 64: over the row's waves through LDS (red: one float per wave, reused
-// after the second barrier)
+// Sum of v over the LPR lanes of a row; LPR > 64: over the row's waves through LDS, one barrier.  red holds one float per
+// wave; the next sum of the block must use another array (it may come back to this one after that).
 template <int LPR>
 __device__ static inline float row_sum(float v, float* red) {
   if constexpr (LPR <= 64) {
@@ -30,8 +30,31 @@ __device__ static inline float row_sum(float v, float* red) {
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < W; ++i) s += red[first + i];
-    __syncthreads();
     return s;
+  }
+}
+// a packet on its way: whole ones as they lie, the one at the end of a row element by element
+template <class T>
+__device__ static inline uint4 fetch_packet(const T* p, int have) {
+  if (have == Packet<T>::V) return packet_load(p);
+  float f[Packet<T>::V];
+  load_part(p, have, 0.f, f);
+  return Packet<T>::pack(f);
+}
+
+// V entries of a parameter vector from column c on, n of them inside the row (16 bytes at a time where all are)
+template <int V>
+__device__ static inline void load_param(const float* __restrict__ w, int c, int n, float fill, float* f) {
+  if (w && n == V) {
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+      float4 v;
+      __builtin_memcpy(&v, w + c + j, 16);
+      f[j] = v.x; f[j + 1] = v.y; f[j + 2] = v.z; f[j + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = w && j < n ? w[c + j] : fill;
   }
 }
 
@@ -42,7 +65,7 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_kernel(const T* x, int64_t x_l
                                                          const float* __restrict__ beta, float eps, T* y, int64_t y_ld,
                                                          float* __restrict__ mean_out, float* __restrict__ rstd_out) {
   constexpr int V = Packet<T>::V, GPB = THREADS / LPR;
-  __shared__ float red[THREADS / 64];
+  __shared__ float red[2][THREADS / 64];
   const int l = threadIdx.x % LPR, group = threadIdx.x / LPR;
   const float inv_n = 1.f / (float)cols;
   float ga[NV][V], be[NV][V];
@@ -51,27 +74,30 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_kernel(const T* x, int64_t x_l
   for (int i = 0; i < NV; ++i) {
     const int c = (l + i * LPR) * V;
     have[i] = min(max(cols - c, 0), V);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      ga[i][j] = gamma && j < have[i] ? gamma[c + j] : 1.f;
-      be[i][j] = beta && j < have[i] ? beta[c + j] : 0.f;
-    }
+    load_param<V>(gamma, c, have[i], 1.f, ga[i]);
+    load_param<V>(beta, c, have[i], 0.f, be[i]);
   }
-  for (int64_t base = (int64_t)blockIdx.x * GPB; base < rows; base += (int64_t)gridDim.x * GPB) {
+  const int64_t step = (int64_t)gridDim.x * GPB;
+  uint4 next[NV];                                      // the next row travels while this one is reduced
+  auto fetch = [&](int64_t row) {
+    const T* xr = x + min(row, rows - 1) * x_ld;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) next[i] = fetch_packet(xr + (l + i * LPR) * V, have[i]);
+  };
+  fetch((int64_t)blockIdx.x * GPB + group);
+  for (int64_t base = (int64_t)blockIdx.x * GPB; base < rows; base += step) {
     const int64_t row = base + group;
     const bool active = row < rows;
-    const T* xr = x + (active ? row : 0) * x_ld;
     float v[NV][V];
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (l + i * LPR) * V;
-      if (have[i] == V) Packet<T>::unpack(packet_load(xr + c), v[i]);
-      else load_part(xr + c, have[i], 0.f, v[i]);
+      Packet<T>::unpack(next[i], v[i]);
 #pragma unroll
       for (int j = 0; j < V; ++j) s += v[i][j];
     }
-    const float mean = row_sum<LPR>(s, red) * inv_n;
+    if (base + step < rows) fetch(row + step);
+    const float mean = row_sum<LPR>(s, red[0]) * inv_n;
     float q = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -84,7 +110,7 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_kernel(const T* x, int64_t x_l
           if (j < have[i]) { v[i][j] -= mean; q = fmaf(v[i][j], v[i][j], q); }
       }
     }
-    const float var = row_sum<LPR>(q, red) * inv_n;
+    const float var = row_sum<LPR>(q, red[1]) * inv_n;
     const float rstd = 1.f / sqrtf(var + eps);
     if (active) {
       T* yr = y + row * y_ld;
@@ -113,7 +139,7 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_kernel(const T* dy, int64_t dy
                                                          const float* __restrict__ gamma, T* dx, int64_t dx_ld, int acc,
                                                          float* __restrict__ part) {
   constexpr int V = Packet<T>::V, GPB = THREADS / LPR;
-  __shared__ float red[THREADS / 64];
+  __shared__ float red[2][2][THREADS / 64];
   __shared__ float fold[GPB > 1 ? THREADS * NV * V : 1];
   const int l = threadIdx.x % LPR, group = threadIdx.x / LPR;
   const float inv_n = 1.f / (float)cols;
@@ -123,31 +149,39 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_kernel(const T* dy, int64_t dy
   for (int i = 0; i < NV; ++i) {
     const int c = (l + i * LPR) * V;
     have[i] = min(max(cols - c, 0), V);
+    load_param<V>(gamma, c, have[i], 1.f, ga[i]);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      ga[i][j] = gamma && j < have[i] ? gamma[c + j] : 1.f;
-      dg[i][j] = db[i][j] = 0.f;
-    }
+    for (int j = 0; j < V; ++j) dg[i][j] = db[i][j] = 0.f;
   }
-  for (int64_t base = (int64_t)blockIdx.x * GPB; base < rows; base += (int64_t)gridDim.x * GPB) {
+  const int64_t step = (int64_t)gridDim.x * GPB;
+  uint4 next_x[NV], next_g[NV];
+  float next_mean, next_rstd;
+  auto fetch = [&](int64_t row) {
+    row = min(row, rows - 1);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      next_x[i] = fetch_packet(x + row * x_ld + (l + i * LPR) * V, have[i]);
+      next_g[i] = fetch_packet(dy + row * dy_ld + (l + i * LPR) * V, have[i]);
+    }
+    next_mean = mean_in[row];
+    next_rstd = rstd_in[row];
+  };
+  constexpr bool AHEAD = THREADS == 256;               // 1024 threads have 128 registers each, and the row needs them
+  if (AHEAD) fetch((int64_t)blockIdx.x * GPB + group);
+  int turn = 0;
+  for (int64_t base = (int64_t)blockIdx.x * GPB; base < rows; base += step, turn ^= 1) {
     const int64_t row = base + group;
     const bool active = row < rows;
-    const T* xr = x + (active ? row : 0) * x_ld;
-    const T* gr = dy + (active ? row : 0) * dy_ld;
-    const float mean = mean_in[active ? row : 0], rstd = rstd_in[active ? row : 0];
+    if (!AHEAD) fetch(row);
+    const float mean = next_mean, rstd = next_rstd;
     float xh[NV][V], g[NV][V];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (l + i * LPR) * V;
-      if (have[i] == V) {
-        Packet<T>::unpack(packet_load(xr + c), xh[i]);
-        Packet<T>::unpack(packet_load(gr + c), g[i]);
-      } else {
-        load_part(xr + c, have[i], 0.f, xh[i]);
-        load_part(gr + c, have[i], 0.f, g[i]);
-      }
+      Packet<T>::unpack(next_x[i], xh[i]);
+      Packet<T>::unpack(next_g[i], g[i]);
     }
+    if (AHEAD && base + step < rows) fetch(row + step);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -161,8 +195,8 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_kernel(const T* dy, int64_t dy
         s1 += g[i][j];
         s2 = fmaf(g[i][j], xh[i][j], s2);
       }
-    s1 = row_sum<LPR>(s1, red) * inv_n;
-    s2 = row_sum<LPR>(s2, red) * inv_n;
+    s1 = row_sum<LPR>(s1, red[turn][0]) * inv_n;
+    s2 = row_sum<LPR>(s2, red[turn][1]) * inv_n;
     if (active) {
       T* dr = dx + row * dx_ld;
 #pragma unroll
@@ -248,7 +282,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_wide_kernel(const T* x, int64_t x
                                                            int64_t y_ld, float* __restrict__ mean_out,
                                                            float* __restrict__ rstd_out) {
   constexpr int V = Packet<T>::V, STEP = 1024 * V;
-  __shared__ float red[16];
+  __shared__ float red[2][16];
   const float inv_n = 1.f / (float)cols;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* xr = x + row * x_ld;
@@ -259,13 +293,13 @@ __global__ __launch_bounds__(1024) void ln_fwd_wide_kernel(const T* x, int64_t x
 #pragma unroll
       for (int j = 0; j < V; ++j) s += f[j];
     }
-    const float mean = row_sum<1024>(s, red) * inv_n;
+    const float mean = row_sum<1024>(s, red[0]) * inv_n;
     for (int c = threadIdx.x * V; c < cols; c += STEP) {
       wide_load(xr, c, cols, mean, f);
 #pragma unroll
       for (int j = 0; j < V; ++j) q = fmaf(f[j] - mean, f[j] - mean, q);
     }
-    const float rstd = 1.f / sqrtf(row_sum<1024>(q, red) * inv_n + eps);
+    const float rstd = 1.f / sqrtf(row_sum<1024>(q, red[1]) * inv_n + eps);
     for (int c = threadIdx.x * V; c < cols; c += STEP) {
       wide_load(xr, c, cols, 0.f, f);
       const int n = min(V, cols - c);
@@ -289,7 +323,7 @@ __global__ __launch_bounds__(1024) void ln_dx_wide_kernel(const T* dy, int64_t d
                                                           const float* __restrict__ gamma, T* dx, int64_t dx_ld,
                                                           int acc) {
   constexpr int V = Packet<T>::V, STEP = 1024 * V;
-  __shared__ float red[16];
+  __shared__ float red[2][16];
   const float inv_n = 1.f / (float)cols;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* xr = x + row * x_ld;
@@ -308,8 +342,8 @@ __global__ __launch_bounds__(1024) void ln_dx_wide_kernel(const T* dy, int64_t d
           s2 = fmaf(h, (f[j] - mean) * rstd, s2);
         }
     }
-    s1 = row_sum<1024>(s1, red) * inv_n;
-    s2 = row_sum<1024>(s2, red) * inv_n;
+    s1 = row_sum<1024>(s1, red[0]) * inv_n;
+    s2 = row_sum<1024>(s2, red[1]) * inv_n;
     for (int c = threadIdx.x * V; c < cols; c += STEP) {
       const int n = min(V, cols - c);
       wide_load(xr, c, cols, 0.f, f);
@@ -398,8 +432,9 @@ static void ln_fwd_launch(const T* x, int64_t x_ld, int64_t rows, int cols, cons
   }
 #define LN_FWD(T_, LPR_, NV_, TH_)                                                                               \
   do {                                                                                                           \
-    const int64_t need = cdiv(rows, TH_ / LPR_), cap = TH_ == 256 ? 2048 : 512;                                  \
-    ln_fwd_kernel<T_, LPR_, NV_, TH_><<<(int)(need < cap ? need : cap), TH_, 0, st>>>(x, x_ld, rows, cols, gamma, \
+    constexpr int TH2 = LPR_ == 256 ? 256 : TH_;                                                                 \
+    const int64_t need = cdiv(rows, TH2 / LPR_), cap = TH2 == 256 ? 2048 : 512;                                  \
+    ln_fwd_kernel<T_, LPR_, NV_, TH2><<<(int)(need < cap ? need : cap), TH2, 0, st>>>(x, x_ld, rows, cols, gamma, \
                                                                                      beta, eps, y, y_ld, mean, rstd); \
   } while (0)
   LN_DISPATCH(T, LN_FWD);
