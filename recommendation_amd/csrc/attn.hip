@@ -178,6 +178,7 @@ struct Attn {
   int B, Tq, Tk, Hkv, G, D;
   float scale, scale2;                                 // scale2 = scale * log2(e)
   int rows, row_tiles, key_tiles, splits, per_split;
+  int row_waves, key_waves, row_splits, rows_per;      // waves per block; splits of the row list in the dk / dv pass
   float *part, *part_lse;                              // [splits][B H Tq][D], [splits][B H Tq]
   float* kept;                                         // few rows: p, then dp, [B Hkv][Tk][R]
   bool near;                                           // a tile's rows lie within 2^31 bytes of its first
@@ -189,11 +190,23 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 __device__ static inline float minus_inf() { return -__builtin_inff(); }
 
-// Blocks that share a key head are neighbours in the logical order; the hardware deals consecutive blocks to the eight
-// dies in turn, so die d takes the d-th eighth of the logical order and its L2 holds only that eighth's keys.
-__device__ static inline int die_order(int id, int n) {
-  const int per = n >> 3, rem = n & 7, die = id & 7;
-  return die * per + min(die, rem) + (id >> 3);
+// Where block `id` of a launch with `per` blocks per pair (sample, key head) works.  The hardware deals consecutive blocks
+// to the eight dies in turn; a pair's blocks read the same keys (or rows), so they are kept on one die, whose L2 then
+// holds them once.  Die x takes the pairs x, x + 8, ...: the samples of a ragged batch, neighbours in this order, go to
+// different dies (500 candidates against up to 1000 events: 42.5 us; 46.5 with blocks of a pair dealt to all dies, 49.6
+// with four neighbouring pairs to a die).  Where the pairs would leave some dies a turn short, every die takes blocks of
+// all pairs.
+struct BlockAt { int pair, part; };
+__host__ __device__ static inline bool by_dies(int64_t pairs) { return pairs >= 64 || (pairs & 7) == 0; }
+__device__ static inline BlockAt block_at(const Attn& a, int per) {
+  const int id = blockIdx.x;
+  if (!by_dies((int64_t)a.B * a.Hkv)) return {id / per, id % per};
+  const int turn = id >> 3;
+  return {turn / per * 8 + (id & 7), turn % per};
+}
+static unsigned pair_blocks(const Attn& a, int64_t per) {              // blocks of pairs beyond the last one leave at once
+  const int64_t pairs = (int64_t)a.B * a.Hkv;
+  return (unsigned)((by_dies(pairs) ? (pairs + 7) / 8 * 8 : pairs) * per);
 }
 
 __device__ static inline int key_count(const Attn& a, int b) {
@@ -213,6 +226,12 @@ __device__ static inline bool lone_key(const Attn& a, int b) {
 }
 
 struct RowAt { int t, h; };
+// A lane's row again after a loop: without this the compiler keeps the row's addresses in registers all along.
+__device__ static inline int row_again(int r0) {
+  int lane = threadIdx.x & 31;
+  asm volatile("" : "+v"(lane));
+  return r0 + lane;
+}
 __device__ static inline RowAt row_at(const Attn& a, int r, int hk) {
   if (a.G == 1) return {r, hk};
   const int t = r / a.G;
@@ -271,57 +290,69 @@ __device__ static inline void store_strip(T* row, int col0, int D, const f32x16&
 template <class T, int ROWS, int DP, int THREADS>
 struct Stage {
   static constexpr int PER = DP / 8, N = (ROWS * PER + THREADS - 1) / THREADS;
+  static constexpr bool EVEN = THREADS % PER == 0;     // a thread's packets lie in one column, THREADS / PER rows apart
   Raw<T> a[N];
-  unsigned off[N];                                     // byte offsets inside a whole tile
-  bool on[N];
+  unsigned off[EVEN ? 1 : N];                          // byte offsets of its packets (EVEN: of the first) in a whole tile
   __device__ static inline int row(int i) { return (int)(threadIdx.x + i * THREADS) / PER; }
   __device__ static inline int col(int i) { return (int)(threadIdx.x + i * THREADS) % PER * 8; }
-  __device__ inline void load(const T* first) {
-    const char* p = reinterpret_cast<const char*>(first);
+  __device__ inline void load(const T* first, int64_t step) {           // step: elements between a thread's packets (EVEN)
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      a[i] = raw_load(reinterpret_cast<const T*>(p + off[i]));
-      on[i] = true;
+      const char* p = reinterpret_cast<const char*>(EVEN ? first + i * step : first);
+      a[i] = raw_load(reinterpret_cast<const T*>(p + off[EVEN ? 0 : i]));
     }
   }
   __device__ inline void keys_init(const Attn& p, const View4& w) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+    for (int i = 0; i < (EVEN ? 1 : N); ++i)
       off[i] = (unsigned)((min(row(i), ROWS - 1) * w.t + (col(i) < p.D ? col(i) : 0)) * sizeof(T));
   }
   // keys k0 .. of one (sample, head), k0 < k1
-  __device__ inline void keys(const Attn& p, const View4& w, const T* base, const uint8_t* mask, int k0, int k1) {
-    if (k0 + ROWS <= k1 && !mask && p.near) return load(base + (int64_t)k0 * w.t);
+  __device__ inline void keys(const Attn& p, const View4& w, const T* base, int k0, int k1) {
+    if (k0 + ROWS <= k1 && p.near) return load(base + (int64_t)k0 * w.t, THREADS / PER * w.t);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int d = col(i) < p.D ? col(i) : 0, key = min(k0 + row(i), k1 - 1);
-      a[i] = raw_load(base + (int64_t)key * w.t + d);
-      on[i] = k0 + row(i) < k1 && (!mask || mask[key]);
-    }
+    for (int i = 0; i < N; ++i)
+      a[i] = raw_load(base + (int64_t)min(k0 + row(i), k1 - 1) * w.t + (col(i) < p.D ? col(i) : 0));
+  }
+  // bit i: the mask leaves the key of packet i
+  __device__ static inline unsigned mask_bits(const uint8_t* mask, int k0, int k1) {
+    unsigned on = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) on |= (mask[min(k0 + row(i), k1 - 1)] != 0 ? 1u : 0u) << i;
+    return on;
   }
   __device__ inline void list_init(const Attn& p, const View4& w) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
+    for (int i = 0; i < (EVEN ? 1 : N); ++i) {
       const int r = min(row(i), ROWS - 1), t = r / p.G, h = r - t * p.G;
       off[i] = (unsigned)((t * w.t + h * w.h + (col(i) < p.D ? col(i) : 0)) * sizeof(T));
     }
   }
   // rows r0 .. of the row list, r0 < rows
   __device__ inline void list(const Attn& p, const View4& w, int b, int hk, int r0) {
-    if (r0 + ROWS <= p.rows && ROWS % p.G == 0 && p.near) return load(row_ptr<T>(w, b, {r0 / p.G, hk * p.G}));
+    // whole groups between a thread's packets: G divides ROWS and their distance
+    constexpr int APART = EVEN && N > 1 ? THREADS / PER : ROWS;
+    if (r0 + ROWS <= p.rows && APART % p.G == 0 && p.near)
+      return load(row_ptr<T>(w, b, {r0 / p.G, hk * p.G}), APART / p.G * w.t);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
+    for (int i = 0; i < N; ++i)
       a[i] = raw_load(row_ptr<T>(w, b, row_at(p, min(r0 + row(i), p.rows - 1), hk)) + (col(i) < p.D ? col(i) : 0));
-      on[i] = r0 + row(i) < p.rows;
-    }
   }
+  // the tile holds rows first .. of `end`; rows behind the end and masked ones (bit i of on: kept) become zeros
   template <class TILE>
-  __device__ inline void put(TILE& t, int D, bool whole) const {
+  __device__ inline void put(TILE& t, int D, int first, int end, bool masked = false, unsigned on = 0) const {
+    if (first + ROWS <= end && !masked) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (row(i) >= ROWS || col(i) >= D) continue;
-      t.put(row(i), col(i), raw_frag<T>(whole || on[i] ? a[i] : raw_zero<T>()));
+      for (int i = 0; i < N; ++i)
+        if (row(i) < ROWS && col(i) < D) t.put(row(i), col(i), raw_frag<T>(a[i]));
+      return;
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (row(i) < ROWS && col(i) < D) {
+        const bool in = first + row(i) < end && (!masked || (on >> i & 1));
+        t.put(row(i), col(i), raw_frag<T>(in ? a[i] : raw_zero<T>()));
+      }
   }
 };
 
@@ -333,15 +364,20 @@ __device__ static inline void clear_tile(TILE& t) {
   for (int i = threadIdx.x; i < N; i += blockDim.x) reinterpret_cast<uint4*>(t.v)[i] = make_uint4(0, 0, 0, 0);
 }
 
-// The keys that a tile leaves out: adds -infinity to their scores.  Bit i of `bits`: key k0 + i may be attended to.
+// Bit i: key k0 + i may be attended to
 __device__ static inline uint64_t key_bits(const uint8_t* mask, int k0, int k1, int n) {
   const int lane = threadIdx.x & 63, key = k0 + lane;
   return __ballot(lane < n && key < k1 && (!mask || mask[key]));
 }
+// -infinity to the scores of the keys that strip i of a tile leaves out.  They were staged as zeros, so their scores are
+// zeros, and the bits of -infinity are simply or-ed in: two instructions per score.
 __device__ static inline void leave_out(f32x16& s, uint64_t bits, int i) {
-  const uint64_t mine = bits >> (4 * ((threadIdx.x & 63) >> 5));
+  const unsigned off = ~(unsigned)(bits >> (32 * i)) >> (4 * ((threadIdx.x & 63) >> 5));
 #pragma unroll
-  for (int e = 0; e < 16; ++e) s[e] = (mine >> (i * 32 + acc_row(e))) & 1 ? s[e] : minus_inf();
+  for (int e = 0; e < 16; ++e) {
+    const unsigned all = (unsigned)__builtin_amdgcn_sbfe((int)off, acc_row(e), 1);
+    s[e] = __uint_as_float(__float_as_uint(s[e]) | (all & 0xff800000u));
+  }
 }
 
 // Waves per SIMD the tiled kernels are built for.  Two keep a wave within 256 registers, and only then does the compiler
@@ -366,10 +402,9 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? WAVES<T, DP> : FWD_WAVES<T, DP>
   __shared__ Tile<T, KT, DP> kt[NBUF];
   __shared__ Tile<T, KT, DP, 16> vt[NBUF];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int id = die_order(blockIdx.x, gridDim.x);
-  const int split = id % a.splits;
-  id /= a.splits;
-  const int tile = id % a.row_tiles, bh = id / a.row_tiles, b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const BlockAt ba = block_at(a, a.row_tiles * a.splits);
+  if (ba.pair >= a.B * a.Hkv) return;
+  const int split = ba.part % a.splits, tile = ba.part / a.splits, b = ba.pair / a.Hkv, hk = ba.pair - b * a.Hkv;
   const int k0 = split * a.per_split, k1 = min(key_count(a, b), k0 + a.per_split);
   const int r0 = (tile * NW + wave) * 32;
   const bool busy = r0 < a.rows;
@@ -380,22 +415,24 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? WAVES<T, DP> : FWD_WAVES<T, DP>
   Stage<T, KT, DP, NW * 64> nk, nv;
   nk.keys_init(a, a.k);
   nv.keys_init(a, a.v);
+  unsigned left = 0;
   auto load = [&](int kb) {
     if (kb >= k1) return;
-    nk.keys(a, a.k, kp, mask, kb, k1);
-    nv.keys(a, a.v, vp, mask, kb, k1);
+    nk.keys(a, a.k, kp, kb, k1);
+    nv.keys(a, a.v, vp, kb, k1);
+    if (mask) left = nk.mask_bits(mask, kb, k1);
   };
   auto put = [&](int buf, int kb) {
     if (kb >= k1) return;
-    const bool whole = !mask && kb + KT <= k1;
-    nk.put(kt[buf], a.D, whole);
-    nv.put(vt[buf], a.D, whole);
+    nk.put(kt[buf], a.D, kb, k1, mask, left);
+    nv.put(vt[buf], a.D, kb, k1, mask, left);
   };
   load(k0);
-  const int r = r0 + (lane & 31);
-  const RowAt ra = row_at(a, r < a.rows ? r : 0, hk);
   Frag<T> qf[NK];
-  load_row_frags<T, DP>(row_ptr<T>(a.q, b, ra), r < a.rows, a.D, qf);
+  {
+    const int r = r0 + (lane & 31);
+    load_row_frags<T, DP>(row_ptr<T>(a.q, b, row_at(a, r < a.rows ? r : 0, hk)), r < a.rows, a.D, qf);
+  }
   f32x16 o[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = f32x16{};
@@ -475,7 +512,9 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? WAVES<T, DP> : FWD_WAVES<T, DP>
       }
   }
   const float sum = half_swap_sum(l, l);
+  const int r = row_again(r0);
   if (r >= a.rows) return;
+  const RowAt ra = row_at(a, r, hk);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int64_t rid = row_id(a, b, ra);
   const float lse = sum == 0.f ? minus_inf() : m * a.scale + (logf(sum) - BIAS * LN2);
@@ -598,10 +637,9 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dq_kernel(Attn a
   constexpr bool F16 = __is_same(T, f16_t), KEYS = Terms<T>::NP == 1;
   __shared__ Tile<T, KT, DP> kt[NBUF], vt[NBUF];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int id = die_order(blockIdx.x, gridDim.x);
-  const int split = id % a.splits;
-  id /= a.splits;
-  const int tile = id % a.row_tiles, bh = id / a.row_tiles, b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const BlockAt ba = block_at(a, a.row_tiles * a.splits);
+  if (ba.pair >= a.B * a.Hkv) return;
+  const int split = ba.part % a.splits, tile = ba.part / a.splits, b = ba.pair / a.Hkv, hk = ba.pair - b * a.Hkv;
   const int k0 = split * a.per_split, k1 = min(key_count(a, b), k0 + a.per_split);
   const int r0 = (tile * NW + wave) * 32;
   const bool busy = r0 < a.rows;
@@ -612,27 +650,27 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dq_kernel(Attn a
   Stage<T, KT, DP, NW * 64> nk, nv;
   nk.keys_init(a, a.k);
   nv.keys_init(a, a.v);
+  unsigned left = 0;
   auto is_whole = [&](int kb) { return !mask && kb + KT <= k1; };
   auto load = [&](int kb) {
     if (kb >= k1) return;
-    nk.keys(a, a.k, kp, mask, kb, k1);
-    nv.keys(a, a.v, vp, mask, kb, k1);
+    nk.keys(a, a.k, kp, kb, k1);
+    nv.keys(a, a.v, vp, kb, k1);
+    if (mask) left = nk.mask_bits(mask, kb, k1);
   };
   auto put = [&](int buf, int kb) {
     if (kb >= k1) return;
-    const bool whole = is_whole(kb);
-    nk.put(kt[buf], a.D, whole);
-    nv.put(vt[buf], a.D, whole);
+    nk.put(kt[buf], a.D, kb, k1, mask, left);
+    nv.put(vt[buf], a.D, kb, k1, mask, left);
   };
   load(k0);
-  const int r = r0 + (lane & 31);
-  const bool in = r < a.rows;
-  const RowAt ra = row_at(a, in ? r : 0, hk);
-  const int64_t rid = row_id(a, b, ra);
   Frag<T> qf[NK], gf[NK];
-  load_row_frags<T, DP>(row_ptr<T>(a.q, b, ra), in, a.D, qf);
-  float delta = 0.f;
+  float delta = 0.f, shift = minus_inf();              // a row without keys: p = 2^-inf
   {
+    const int r = r0 + (lane & 31);
+    const bool in = r < a.rows;
+    const RowAt ra = row_at(a, in ? r : 0, hk);
+    load_row_frags<T, DP>(row_ptr<T>(a.q, b, ra), in, a.D, qf);
     const T* gp = row_ptr<T>(a.dout, b, ra);
     const T* op = row_ptr<T>(a.out, b, ra);
 #pragma unroll
@@ -648,11 +686,10 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dq_kernel(Attn a
       gf[s] = raw_frag<T>(g);
     }
     delta = half_swap_sum(delta, delta);
-  }
-  float shift = minus_inf();                           // a row without keys: p = 2^-inf
-  if (in) {
-    const float lse = a.lse[rid];
-    shift = lse == minus_inf() ? minus_inf() : Terms<T>::BIAS - lse * LOG2E;
+    if (in) {
+      const float lse = a.lse[row_id(a, b, ra)];
+      shift = lse == minus_inf() ? minus_inf() : Terms<T>::BIAS - lse * LOG2E;
+    }
   }
   f32x16 acc[ND], keys[KEYS ? ND : 1];
 #pragma unroll
@@ -732,7 +769,10 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dq_kernel(Attn a
 #pragma unroll
     for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
   }
-  if (!in) return;
+  const int r = row_again(r0);
+  if (r >= a.rows) return;
+  const RowAt ra = row_at(a, r, hk);
+  const int64_t rid = row_id(a, b, ra);
   if (a.splits == 1) {
     if (lane < 32) a.delta[rid] = delta + rest;
     T* dst = const_cast<T*>(row_ptr<T>(a.dq, b, ra));
@@ -766,9 +806,11 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dkv_kernel(Attn 
   __shared__ Tile<T, QB, DP> qt[2], gt[2];
   __shared__ float4 shift_s[2][QB / 4], delta_s[2][QB / 4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int id = die_order(blockIdx.x, gridDim.x);
-  const int tile = id % a.key_tiles, bh = id / a.key_tiles, b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const BlockAt ba = block_at(a, a.key_tiles * a.row_splits);
+  if (ba.pair >= a.B * a.Hkv) return;
+  const int split = ba.part % a.row_splits, tile = ba.part / a.row_splits, b = ba.pair / a.Hkv, hk = ba.pair - b * a.Hkv;
   const int len = key_count(a, b);
+  const int row0 = split * a.rows_per, row1 = min(a.rows, row0 + a.rows_per);
   const int key0 = tile * NW * 32, key = key0 + wave * 32 + (lane & 31);
   const bool on = key < len && (!a.mask || a.mask[(int64_t)b * a.mask_ld + key]);
   const bool busy = __any(on);
@@ -776,13 +818,13 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dkv_kernel(Attn 
 #pragma unroll
   for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{};
   float factor = F16 ? F16_FACTOR0 : 1.f;
-  if (key0 < len && a.rows > 0) {
+  if (key0 < len && row0 < row1) {
     Stage<T, QB, DP, NW * 64> nq, ng;
     nq.list_init(a, a.q);
     ng.list_init(a, a.dout);
     float lse_n = 0.f, delta_n = 0.f;
     auto load = [&](int r0) {
-      if (r0 >= a.rows) return;
+      if (r0 >= row1) return;
       nq.list(a, a.q, b, hk, r0);
       ng.list(a, a.dout, b, hk, r0);
       if (threadIdx.x < QB) {
@@ -797,15 +839,15 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dkv_kernel(Attn 
       }
     };
     auto put = [&](int buf, int r0) {
-      if (r0 >= a.rows) return;
-      nq.put(qt[buf], a.D, r0 + QB <= a.rows);
-      ng.put(gt[buf], a.D, r0 + QB <= a.rows);
+      if (r0 >= row1) return;
+      nq.put(qt[buf], a.D, r0, a.rows);
+      ng.put(gt[buf], a.D, r0, a.rows);
       if (threadIdx.x < QB) {
         reinterpret_cast<float*>(shift_s[buf])[threadIdx.x] = lse_n == minus_inf() ? minus_inf() : Terms<T>::BIAS - lse_n * LOG2E;
         reinterpret_cast<float*>(delta_s[buf])[threadIdx.x] = delta_n;
       }
     };
-    load(0);
+    load(row0);
     Frag<T> kf[NK], vf[NK];
     load_row_frags<T, DP>((const T*)a.k.p + (int64_t)b * a.k.b + (int64_t)hk * a.k.h + (int64_t)(on ? key : 0) * a.k.t, on, a.D, kf);
     load_row_frags<T, DP>((const T*)a.v.p + (int64_t)b * a.v.b + (int64_t)hk * a.v.h + (int64_t)(on ? key : 0) * a.v.t, on, a.D, vf);
@@ -857,10 +899,10 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dkv_kernel(Attn 
         }
       }
     };
-    put(0, 0);
-    load(QB);
+    put(0, row0);
+    load(row0 + QB);
     int at = 0;
-    for (int r0 = 0; r0 < a.rows; r0 += QB, at ^= 1) {
+    for (int r0 = row0; r0 < row1; r0 += QB, at ^= 1) {
       __syncthreads();
       put(at ^ 1, r0 + QB);
       load(r0 + 2 * QB);
@@ -871,6 +913,17 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dkv_kernel(Attn 
   if (key >= a.Tk) return;
   if (!on) factor = 1.f;
   constexpr float one = 1.f / (1 << (int)Terms<T>::BIAS);   // ds carries p's factor too
+  if (a.row_splits > 1) {                              // fp32, both of a key side by side; attn_key_sum_kernel follows
+    float* to = a.part + ((int64_t)(split * a.B + b) * a.Hkv + hk) * a.Tk * 2 * a.D + (int64_t)key * 2 * a.D;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      if (lone) dk[d] = f32x16{};
+      if (!on) dk[d] = dv[d] = f32x16{};
+      store_strip<float>(to, d * 32, a.D, dk[d], a.scale * one / factor);
+      store_strip<float>(to + a.D, d * 32, a.D, dv[d], one);
+    }
+    return;
+  }
   T* kd = (T*)a.dk.p + (int64_t)b * a.dk.b + (int64_t)key * a.dk.t + (int64_t)hk * a.dk.h;
   T* vd = (T*)a.dv.p + (int64_t)b * a.dv.b + (int64_t)key * a.dv.t + (int64_t)hk * a.dv.h;
 #pragma unroll
@@ -880,6 +933,29 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dkv_kernel(Attn 
     store_strip<T>(kd, d * 32, a.D, dk[d], a.scale * one / factor);
     store_strip<T>(vd, d * 32, a.D, dv[d], one);
   }
+}
+
+// dk and dv from the row splits, in split order: a thread per four columns of a key
+template <class T>
+__global__ __launch_bounds__(256) void attn_key_sum_kernel(Attn a) {
+  const int quads = a.D / 4;
+  const int64_t n_keys = (int64_t)a.B * a.Hkv * a.Tk, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= n_keys * 2 * quads) return;
+  const int64_t at = id / (2 * quads);                 // (b, hk, key)
+  const int w = (int)(id - at * 2 * quads), d = w % quads * 4;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < a.row_splits; ++i) {
+    const float4 v = *reinterpret_cast<const float4*>(a.part + ((int64_t)i * n_keys + at) * 2 * a.D + w * 4);
+    acc[0] += v.x;
+    acc[1] += v.y;
+    acc[2] += v.z;
+    acc[3] += v.w;
+  }
+  const int64_t pair = at / a.Tk;
+  const RowAt ra = {(int)(at - pair * a.Tk), (int)(pair % a.Hkv)};
+  T* dst = const_cast<T*>(row_ptr<T>(w < quads ? a.dk : a.dv, (int)(pair / a.Hkv), ra)) + d;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) dst[j] = (T)acc[j];
 }
 
 // Joins the splits of dq as attn_join_kernel does the forward's; KEYS: also what delta was off by (attn_dq_kernel)
@@ -967,14 +1043,15 @@ __device__ static inline void packet_floats(const T* p, bool ok, float* f) {
   Packet<T>::unpack(ok ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0), f);
 }
 
-struct PairAt { int split, b, hk, k0, k1; };
+struct PairAt { int split, b, hk, k0, k1; bool live; };
 __device__ static inline PairAt pair_at(const Attn& a) {
   PairAt p;
-  const int id = die_order(blockIdx.x, gridDim.x);
-  p.split = id % a.splits;
-  const int pair = id / a.splits;
-  p.b = pair / a.Hkv;
-  p.hk = pair - p.b * a.Hkv;
+  const BlockAt ba = block_at(a, a.splits);
+  p.split = ba.part;
+  p.b = ba.pair / a.Hkv;
+  p.hk = ba.pair - p.b * a.Hkv;
+  p.live = ba.pair < a.B * a.Hkv;
+  if (!p.live) p.b = 0;
   p.k0 = p.split * a.per_split;
   p.k1 = min(key_count(a, p.b), p.k0 + a.per_split);
   return p;
@@ -986,6 +1063,7 @@ __global__ __launch_bounds__(NW * 64) void attn_rows_fwd_kernel(Attn a) {
   __shared__ float sm[NW > 1 ? NW * R * (LPK * V + 2) : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LPK, slot = lane / LPK, d = sub * V;
   const PairAt pa = pair_at(a);
+  if (!pa.live) return;
   const bool in_d = d < a.D;
   const T* kp = (const T*)a.k.p + (int64_t)pa.b * a.k.b + (int64_t)pa.hk * a.k.h + d;
   const T* vp = (const T*)a.v.p + (int64_t)pa.b * a.v.b + (int64_t)pa.hk * a.v.h + d;
@@ -1163,6 +1241,7 @@ __global__ __launch_bounds__(NW * 64) void attn_rows_bwd_kernel(Attn a) {
   extern __shared__ float dyn[];                       // joins [NW][R][W], then (FUSED) p, dp [per_split * R] each
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LPK, slot = lane / LPK, d = sub * V;
   const PairAt pa = pair_at(a);
+  if (!pa.live) return;
   const bool in_d = d < a.D;
   const T* kp = (const T*)a.k.p + (int64_t)pa.b * a.k.b + (int64_t)pa.hk * a.k.h + d;
   const T* vp = (const T*)a.v.p + (int64_t)pa.b * a.v.b + (int64_t)pa.hk * a.v.h + d;
@@ -1339,12 +1418,20 @@ static int rows_lanes(int D, int dtype) {
 }
 static int rows_step_keys(int D, int dtype) { return 64 / rows_lanes(D, dtype); }
 static int padded_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
-static int pass_rows(int rows) { return rows <= 32 ? 32 : 128; }          // query rows of a block: one wave or four
+// Waves of a block: as many as there are strips of 32 rows (or keys), one, two or four
+static int strip_waves(int n) { return n <= 32 ? 1 : n <= 64 ? 2 : 4; }
 
-// Splits of the key axis: only where the row tiles alone leave part of the chip without a block (every split writes its
-// share of the result as fp32, which is read again), and never below 256 keys each.
-static int key_splits(int64_t blocks, int Tk) {
-  const int64_t want = blocks < 1 ? 1 : 512 / blocks, most = Tk / 256;
+// Splits of the key axis: only where the row tiles alone leave part of the chip without waves (every split writes its
+// share of the result as fp32, which is read again), and never below 256 keys each.  One block of four waves per CU is
+// enough for tiles that are computed; one wave alone is bound by what it has in flight, and eight per CU are.
+static int key_splits(int64_t blocks, int waves, int Tk) {
+  const int64_t want = (waves == 1 ? 2048 : 512) / (blocks < 1 ? 1 : blocks), most = Tk / 256;
+  const int64_t n = want < most ? want : most;
+  return (int)(n < 1 ? 1 : n);
+}
+// Splits of the row list for dk / dv, on the same grounds: at least 256 rows each.
+static int list_splits(int64_t blocks, int rows) {
+  const int64_t want = 512 / (blocks < 1 ? 1 : blocks), most = rows / 256;
   const int64_t n = want < most ? want : most;
   return (int)(n < 1 ? 1 : n);
 }
@@ -1370,11 +1457,16 @@ static void attn_plan(Attn* a, int dtype) {
     return;
   }
   a->few = 0;
-  a->row_tiles = (int)cdiv(a->rows, pass_rows(a->rows));
-  a->splits = key_splits((int64_t)a->row_tiles * a->B * a->Hkv, a->Tk);
+  a->row_waves = strip_waves(a->rows);
+  a->row_tiles = (int)cdiv(a->rows, 32 * a->row_waves);
+  a->splits = key_splits((int64_t)a->row_tiles * a->B * a->Hkv, a->row_waves, a->Tk);
   a->per_split = (int)align_up(cdiv(a->Tk, a->splits), 64);
   a->splits = a->Tk > 0 ? (int)cdiv(a->Tk, a->per_split) : 1;
-  a->key_tiles = (int)cdiv(a->Tk, 128);
+  a->key_waves = strip_waves(a->Tk);
+  a->key_tiles = (int)cdiv(a->Tk, 32 * a->key_waves);
+  a->row_splits = list_splits((int64_t)a->key_tiles * a->B * a->Hkv, a->rows);
+  a->rows_per = (int)align_up(cdiv(a->rows, a->row_splits), 64);
+  a->row_splits = a->rows > 0 ? (int)cdiv(a->rows, a->rows_per) : 1;
 }
 static int64_t total_rows(const Attn& a) { return (int64_t)a.B * a.Hkv * a.rows; }
 static bool rows_fused(const Attn& a) { return a.splits == 1 && (int64_t)a.per_split * a.few <= ROWS_LDS; }
@@ -1386,7 +1478,9 @@ static size_t bwd_ws_first(const Attn& a) {
 }
 static size_t bwd_ws(const Attn& a) {
   if (a.few) return rows_fused(a) ? 256 : bwd_ws_first(a) + (size_t)a.B * a.Hkv * a.Tk * a.few * 8 + 256;
-  return bwd_ws_first(a) + (a.splits > 1 ? (size_t)a.splits * total_rows(a) * (2 * a.D + 1) * 4 : 0) + 256;
+  const size_t rows = a.splits > 1 ? (size_t)a.splits * total_rows(a) * (2 * a.D + 1) * 4 : 0;
+  const size_t keys = a.row_splits > 1 ? (size_t)a.row_splits * a.B * a.Hkv * a.Tk * 2 * a.D * 4 : 0;
+  return bwd_ws_first(a) + (rows > keys ? rows : keys) + 256;           // one after the other
 }
 
 static int attn_shape(const char* what, const ctr_attn_t* s, Attn* a) {
@@ -1405,8 +1499,9 @@ static int attn_shape(const char* what, const ctr_attn_t* s, Attn* a) {
   a->scale2 = s->scale * LOG2E;
   a->sl = s->sl; a->mask = s->mask; a->mask_ld = s->mask_ld;
   attn_plan(a, s->dtype);
-  CTR_REQUIRE((a->few ? 1 : (int64_t)a->row_tiles) * a->B * a->Hkv * a->splits < (1ll << 31) &&
-              cdiv(a->Tk, 128) * a->B * a->Hkv < (1ll << 31), "%s: too many tiles", what);
+  const int64_t pairs = ((int64_t)a->B * a->Hkv + 7) / 8 * 8;
+  CTR_REQUIRE((a->few ? 1 : (int64_t)a->row_tiles) * pairs * a->splits < (1ll << 31) &&
+              cdiv(a->Tk, 32) * pairs < (1ll << 31) / 4, "%s: too many tiles", what);
   return CTR_OK;
 }
 
@@ -1459,7 +1554,7 @@ static int attn_view(const char* what, const char* name, const ctr_heads_t* v, i
 
 template <class T, int R>
 static void rows_fwd_launch(const Attn& a, hipStream_t st) {
-  const unsigned blocks = (unsigned)((int64_t)a.B * a.Hkv * a.splits);
+  const unsigned blocks = pair_blocks(a, a.splits);
 #define ROWS_FWD(T_, LPK_)                                                           \
   if (a.waves == 1) attn_rows_fwd_kernel<T_, R, LPK_, 1><<<blocks, 64, 0, st>>>(a);  \
   else attn_rows_fwd_kernel<T_, R, LPK_, 4><<<blocks, 256, 0, st>>>(a)
@@ -1469,7 +1564,7 @@ static void rows_fwd_launch(const Attn& a, hipStream_t st) {
 
 template <class T, int R>
 static void rows_bwd_launch(const Attn& a, hipStream_t st) {
-  const unsigned blocks = (unsigned)((int64_t)a.B * a.Hkv * a.splits);
+  const unsigned blocks = pair_blocks(a, a.splits);
   const size_t joins = (size_t)a.waves * R * (2 * a.lanes * Packet<T>::V + 1) * 4;
   if (rows_fused(a)) {
     const size_t lds = joins + (size_t)a.per_split * R * 8;
@@ -1511,12 +1606,12 @@ static void attn_fwd_launch(const Attn& a, hipStream_t st) {
     join_launch<T>(a, st);
     return;
   }
-  constexpr int KT = sizeof(T) == 4 ? 32 : 64;
-  const unsigned blocks = (unsigned)((int64_t)a.row_tiles * a.B * a.Hkv * a.splits);
-  const bool one = pass_rows(a.rows) == 32;
-#define ATTN_FWD(T_, DP_)                                                         \
-  if (one) attn_fwd_kernel<T_, DP_, 1, 32><<<blocks, 64, 0, st>>>(a);          \
-  else attn_fwd_kernel<T_, DP_, 4, (DP_ > 64 ? 32 : KT)><<<blocks, 256, 0, st>>>(a)
+  const unsigned blocks = pair_blocks(a, (int64_t)a.row_tiles * a.splits);
+#define ATTN_FWD(T_, DP_)                                                                                        \
+  constexpr int KT = sizeof(T_) == 4 || DP_ > 64 ? 32 : 64;                                                      \
+  if (a.row_waves == 1) attn_fwd_kernel<T_, DP_, 1, 32><<<blocks, 64, 0, st>>>(a);                               \
+  else if (a.row_waves == 2) attn_fwd_kernel<T_, DP_, 2, KT><<<blocks, 128, 0, st>>>(a);                         \
+  else attn_fwd_kernel<T_, DP_, 4, KT><<<blocks, 256, 0, st>>>(a)
   ATTN_DIM(T, a.D, ATTN_FWD);
 #undef ATTN_FWD
   join_launch<T>(a, st);
@@ -1530,13 +1625,13 @@ static void attn_bwd_launch(const Attn& a, hipStream_t st) {
     else rows_bwd_launch<T, 4>(a, st);
     return;
   }
-  constexpr int KT = sizeof(T) == 4 ? 32 : 64;
-  const unsigned blocks = (unsigned)((int64_t)a.row_tiles * a.B * a.Hkv * a.splits);
-  const bool one = pass_rows(a.rows) == 32;
+  const unsigned blocks = pair_blocks(a, (int64_t)a.row_tiles * a.splits);
   if (blocks) {
-#define ATTN_DQ(T_, DP_)                                                          \
-  if (one) attn_dq_kernel<T_, DP_, 1, 32><<<blocks, 64, 0, st>>>(a);              \
-  else attn_dq_kernel<T_, DP_, 4, (DP_ > 64 ? 32 : KT)><<<blocks, 256, 0, st>>>(a)
+#define ATTN_DQ(T_, DP_)                                                                                         \
+  constexpr int KT = sizeof(T_) == 4 || DP_ > 64 ? 32 : 64;                                                      \
+  if (a.row_waves == 1) attn_dq_kernel<T_, DP_, 1, 32><<<blocks, 64, 0, st>>>(a);                                \
+  else if (a.row_waves == 2) attn_dq_kernel<T_, DP_, 2, KT><<<blocks, 128, 0, st>>>(a);                          \
+  else attn_dq_kernel<T_, DP_, 4, KT><<<blocks, 256, 0, st>>>(a)
     ATTN_DIM(T, a.D, ATTN_DQ);
 #undef ATTN_DQ
     if (a.splits > 1) {
@@ -1545,11 +1640,17 @@ static void attn_bwd_launch(const Attn& a, hipStream_t st) {
       else attn_sum_kernel<T, false><<<(unsigned)cdiv(n * (a.D / 4), 256), 256, 0, st>>>(a, n);
     }
   }
-  const unsigned kblocks = (unsigned)((int64_t)a.key_tiles * a.B * a.Hkv);
+  const unsigned kblocks = pair_blocks(a, (int64_t)a.key_tiles * a.row_splits);
   if (kblocks) {
-#define ATTN_DKV(T_, DP_) attn_dkv_kernel<T_, DP_, 4, (sizeof(T_) == 2 && DP_ <= 64 ? 64 : 32)><<<kblocks, 256, 0, st>>>(a)
+#define ATTN_DKV(T_, DP_)                                                                                        \
+  constexpr int QB = sizeof(T_) == 2 && DP_ <= 64 ? 64 : 32;                                                     \
+  if (a.key_waves == 1) attn_dkv_kernel<T_, DP_, 1, 32><<<kblocks, 64, 0, st>>>(a);                              \
+  else if (a.key_waves == 2) attn_dkv_kernel<T_, DP_, 2, QB><<<kblocks, 128, 0, st>>>(a);                        \
+  else attn_dkv_kernel<T_, DP_, 4, QB><<<kblocks, 256, 0, st>>>(a)
     ATTN_DIM(T, a.D, ATTN_DKV);
 #undef ATTN_DKV
+    if (a.row_splits > 1)
+      attn_key_sum_kernel<T><<<(unsigned)cdiv((int64_t)a.B * a.Hkv * a.Tk * (a.D / 2), 256), 256, 0, st>>>(a);
   }
 }
 
