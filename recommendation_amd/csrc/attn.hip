@@ -572,6 +572,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(Attn a, int64_t n_rows) 
   }
   const float base = top == minus_inf() ? 0.f : top;
   float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
   for (int i = first; i < a.splits; i += every) {
     const float w = expf(a.part_lse[i * n_rows + rid] - base);
     sum += w;
@@ -982,6 +983,7 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(Attn a, int64_t n_rows) {
 #pragma unroll
   for (int j = 0; j < N; ++j) acc[j] = 0.f;
   if (quad < quads)
+#pragma unroll 4
     for (int i = first; i < a.splits; i += every) {
       const float* from = a.part + (i * n_rows + rid) * width + d;
       const float4 v = *reinterpret_cast<const float4*>(from);
@@ -1043,26 +1045,41 @@ __device__ static inline void packet_floats(const T* p, bool ok, float* f) {
   Packet<T>::unpack(ok ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0), f);
 }
 
+// NW waves work on one pair.  A wave alone on its pair shares a block with the three next ones: they are the neighbouring
+// heads of the same sample, whose rows lie side by side in memory, and are read at the same time.
 struct PairAt { int split, b, hk, k0, k1; bool live; };
+template <int NW>
 __device__ static inline PairAt pair_at(const Attn& a) {
   PairAt p;
-  const BlockAt ba = block_at(a, a.splits);
-  p.split = ba.part;
-  p.b = ba.pair / a.Hkv;
-  p.hk = ba.pair - p.b * a.Hkv;
-  p.live = ba.pair < a.B * a.Hkv;
-  if (!p.live) p.b = 0;
+  int pair;
+  if constexpr (NW == 1) {
+    pair = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    p.split = 0;
+  } else {
+    const BlockAt ba = block_at(a, a.splits);
+    pair = ba.pair;
+    p.split = ba.part;
+  }
+  p.live = pair < a.B * a.Hkv;
+  if (!p.live) pair = 0;
+  p.b = pair / a.Hkv;
+  p.hk = pair - p.b * a.Hkv;
   p.k0 = p.split * a.per_split;
   p.k1 = min(key_count(a, p.b), p.k0 + a.per_split);
   return p;
 }
+// LDS written by a wave's lanes before, read by its other lanes after
+__device__ static inline void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
 
 template <class T, int R, int LPK, int NW>
-__global__ __launch_bounds__(NW * 64) void attn_rows_fwd_kernel(Attn a) {
+__global__ __launch_bounds__(256) void attn_rows_fwd_kernel(Attn a) {
   constexpr int V = Packet<T>::V, KPW = 64 / LPK, U = ROW_STEP;
   __shared__ float sm[NW > 1 ? NW * R * (LPK * V + 2) : 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LPK, slot = lane / LPK, d = sub * V;
-  const PairAt pa = pair_at(a);
+  const int lane = threadIdx.x & 63, wave = NW == 1 ? 0 : threadIdx.x >> 6, sub = lane % LPK, slot = lane / LPK, d = sub * V;
+  const PairAt pa = pair_at<NW>(a);
   if (!pa.live) return;
   const bool in_d = d < a.D;
   const T* kp = (const T*)a.k.p + (int64_t)pa.b * a.k.b + (int64_t)pa.hk * a.k.h + d;
@@ -1236,11 +1253,13 @@ __device__ static inline void rows_write_kv(const Attn& a, int b, int hk, int k0
 
 // FUSED: one block holds all keys of its pair in LDS; else p and dp go to a.kept and the sums to a.part
 template <class T, int R, int LPK, int NW, bool FUSED>
-__global__ __launch_bounds__(NW * 64) void attn_rows_bwd_kernel(Attn a) {
+__global__ __launch_bounds__(256) void attn_rows_bwd_kernel(Attn a) {
   constexpr int V = Packet<T>::V, KPW = 64 / LPK, U = ROW_STEP, W = 2 * LPK * V + 1;
-  extern __shared__ float dyn[];                       // joins [NW][R][W], then (FUSED) p, dp [per_split * R] each
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LPK, slot = lane / LPK, d = sub * V;
-  const PairAt pa = pair_at(a);
+  extern __shared__ float lds[];                       // joins [NW][R][W], then (FUSED) p, dp [per_split * R] each
+  float* dyn = lds;
+  if (NW == 1) dyn += (threadIdx.x >> 6) * a.per_split * R * 2;          // one per pair, nothing to join
+  const int lane = threadIdx.x & 63, wave = NW == 1 ? 0 : threadIdx.x >> 6, sub = lane % LPK, slot = lane / LPK, d = sub * V;
+  const PairAt pa = pair_at<NW>(a);
   if (!pa.live) return;
   const bool in_d = d < a.D;
   const T* kp = (const T*)a.k.p + (int64_t)pa.b * a.k.b + (int64_t)pa.hk * a.k.h + d;
@@ -1249,7 +1268,7 @@ __global__ __launch_bounds__(NW * 64) void attn_rows_bwd_kernel(Attn a) {
   float* kept;
   int64_t apart;
   if constexpr (FUSED) {
-    kept = dyn + NW * R * W;
+    kept = dyn + (NW == 1 ? 0 : NW * R * W);
     apart = (int64_t)a.per_split * R;
   } else {
     kept = a.kept + ((int64_t)(pa.b * a.Hkv + pa.hk) * a.Tk + pa.k0) * R;
@@ -1343,7 +1362,7 @@ __global__ __launch_bounds__(NW * 64) void attn_rows_bwd_kernel(Attn a) {
       }
     }
   } else if constexpr (FUSED) {
-    __syncthreads();                                   // p and dp of this wave's other lanes
+    wave_fence();                                      // p and dp of this wave's other lanes
   }
   const bool lone = FUSED && lone_key(a, pa.b);
   if (wave == 0 && slot == 0)
@@ -1423,9 +1442,10 @@ static int strip_waves(int n) { return n <= 32 ? 1 : n <= 64 ? 2 : 4; }
 
 // Splits of the key axis: only where the row tiles alone leave part of the chip without waves (every split writes its
 // share of the result as fp32, which is read again), and never below 256 keys each.  One block of four waves per CU is
-// enough for tiles that are computed; one wave alone is bound by what it has in flight, and eight per CU are.
+// enough for tiles that are computed; single waves want four per CU (16 rows against 32768 keys of 128: 48 us with 1024,
+// 56 with 2048, 70 with 512).
 static int key_splits(int64_t blocks, int waves, int Tk) {
-  const int64_t want = (waves == 1 ? 2048 : 512) / (blocks < 1 ? 1 : blocks), most = Tk / 256;
+  const int64_t want = (waves == 1 ? 1024 : 512) / (blocks < 1 ? 1 : blocks), most = Tk / 256;
   const int64_t n = want < most ? want : most;
   return (int)(n < 1 ? 1 : n);
 }
@@ -1469,7 +1489,9 @@ static void attn_plan(Attn* a, int dtype) {
   a->row_splits = a->rows > 0 ? (int)cdiv(a->rows, a->rows_per) : 1;
 }
 static int64_t total_rows(const Attn& a) { return (int64_t)a.B * a.Hkv * a.rows; }
-static bool rows_fused(const Attn& a) { return a.splits == 1 && (int64_t)a.per_split * a.few <= ROWS_LDS; }
+static bool rows_fused(const Attn& a) {
+  return a.splits == 1 && (int64_t)a.per_split * a.few <= (a.waves == 1 ? ROWS_LDS / 4 : ROWS_LDS);
+}
 static size_t fwd_ws(const Attn& a) { return a.splits > 1 ? (size_t)a.splits * total_rows(a) * (a.D + 1) * 4 + 256 : 0; }
 // tiled: delta, then the splits' dq; few rows: the splits' sums, then p and dp of every key
 static size_t bwd_ws_first(const Attn& a) {
@@ -1554,9 +1576,9 @@ static int attn_view(const char* what, const char* name, const ctr_heads_t* v, i
 
 template <class T, int R>
 static void rows_fwd_launch(const Attn& a, hipStream_t st) {
-  const unsigned blocks = pair_blocks(a, a.splits);
+  const unsigned blocks = a.waves == 1 ? (unsigned)cdiv((int64_t)a.B * a.Hkv, 4) : pair_blocks(a, a.splits);
 #define ROWS_FWD(T_, LPK_)                                                           \
-  if (a.waves == 1) attn_rows_fwd_kernel<T_, R, LPK_, 1><<<blocks, 64, 0, st>>>(a);  \
+  if (a.waves == 1) attn_rows_fwd_kernel<T_, R, LPK_, 1><<<blocks, 256, 0, st>>>(a); \
   else attn_rows_fwd_kernel<T_, R, LPK_, 4><<<blocks, 256, 0, st>>>(a)
   ROWS_LANES(T, a.lanes, ROWS_FWD);
 #undef ROWS_FWD
@@ -1564,12 +1586,13 @@ static void rows_fwd_launch(const Attn& a, hipStream_t st) {
 
 template <class T, int R>
 static void rows_bwd_launch(const Attn& a, hipStream_t st) {
-  const unsigned blocks = pair_blocks(a, a.splits);
-  const size_t joins = (size_t)a.waves * R * (2 * a.lanes * Packet<T>::V + 1) * 4;
-  if (rows_fused(a)) {
-    const size_t lds = joins + (size_t)a.per_split * R * 8;
+  const bool fused = rows_fused(a), alone = a.waves == 1 && fused;
+  const unsigned blocks = alone ? (unsigned)cdiv((int64_t)a.B * a.Hkv, 4) : pair_blocks(a, a.splits);
+  const size_t joins = (size_t)4 * R * (2 * a.lanes * Packet<T>::V + 1) * 4, keep = (size_t)a.per_split * R * 8;
+  if (fused) {
+    const size_t lds = alone ? 4 * keep : joins + keep;
 #define ROWS_BWD(T_, LPK_)                                                                        \
-  if (a.waves == 1) attn_rows_bwd_kernel<T_, R, LPK_, 1, true><<<blocks, 64, lds, st>>>(a);       \
+  if (alone) attn_rows_bwd_kernel<T_, R, LPK_, 1, true><<<blocks, 256, lds, st>>>(a);      \
   else attn_rows_bwd_kernel<T_, R, LPK_, 4, true><<<blocks, 256, lds, st>>>(a)
     ROWS_LANES(T, a.lanes, ROWS_BWD);
 #undef ROWS_BWD
