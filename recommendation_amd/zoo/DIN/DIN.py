@@ -56,6 +56,11 @@ class DIN(GraphOwner):
         # the attention scoring network as three fused launches (H = 16 or 32, the reference's default); any other
         # width, or fused_attention=False, goes layer by layer through the materialised [B*T, 4H]
         self.fused_attention = bool(getattr(args, 'fused_attention', True)) and ops.din_attn_mlp_supported(H)
+        # clip_norm (not a reference flag; None: off): the gradients of a step are scaled as tf.clip_by_global_norm
+        # scales them, lookups by their slices' values; grad_norm then holds the norm before clipping (a device word)
+        self.clip_norm = getattr(args, 'clip_norm', None)
+        if self.clip_norm is not None and not 0.0 < float(self.clip_norm) < float('inf'):
+            raise ValueError('clip_norm must be positive and finite')
         self._train_graphs = {}            # (B, T) -> captured training step
         self._lr_dev = None                # the device word a captured step reads its learning rate from
         self._ready = False
@@ -90,6 +95,7 @@ class DIN(GraphOwner):
         self._loss_dev = self._scalars[:1]
         self._oor = self._scalars[1:].view(torch.int32)
         self._auc_dev = torch.zeros(1, dtype=torch.float32, device=dev)
+        self.grad_norm = torch.zeros(1, dtype=torch.float32, device=dev)
         rng = np.random.Generator(np.random.PCG64(seed))
         init = OrderedDict()
         for k, s in self.variable_shapes().items():
@@ -184,6 +190,8 @@ class DIN(GraphOwner):
                  src=torch.zeros(2 * n, dtype=torch.int32, device=dev),
                  bkeys=torch.zeros(B, dtype=torch.int32, device=dev),
                  bsrc=torch.zeros(B, dtype=torch.int32, device=dev))
+        if self.clip_norm is not None:     # dense variables, item and category slices, item_b slices
+            b['grads'] = ops.GradList([self.dense.grad, b['demb'], b['dlogit']])
         b['u_emb'] = b['din'][:, :H]        # the dense layer writes the user vector straight into the FCN's input
         return b
 
@@ -349,6 +357,8 @@ class DIN(GraphOwner):
         else:
             self._attention_mlp_backward_unfused(b, ds, i_emb, h_emb, dq, dk, B, T)
         ops.copy2d(b['ddin'][:, H:], dq, accumulate=True)                                # i_emb also feeds the FCN
+        if self.clip_norm is not None:
+            ops.clip_grads(b['grads'], self.clip_norm, self.grad_norm, ws=ws)
         # sparse updates (SGD) on item/category tables and on item_b
         sgd = ops.make_opt(OPT_SGD, lr=float(l), lr_dev=self._lr_dev)      # a captured step reads l from a device word
         n = B + B * T

@@ -62,6 +62,8 @@ def make_parser():
     p.add_argument('--epoch', help='number of epochs', type=int, default=10)
     p.add_argument('--learning_rate', help='learning rate', type=float, default=0.1)
     p.add_argument('--eval_every', type=int, default=1000)
+    p.add_argument('--clip_norm', help='bound on the global gradient norm (not a reference flag; default: none)',
+                   type=float, default=None)
     p.add_argument('--device', default='cuda:0')
     return p
 
