@@ -369,14 +369,14 @@ __device__ static inline uint64_t key_bits(const uint8_t* mask, int k0, int k1, 
   const int lane = threadIdx.x & 63, key = k0 + lane;
   return __ballot(lane < n && key < k1 && (!mask || mask[key]));
 }
-// -infinity to the scores of the keys that strip i of a tile leaves out.  They were staged as zeros, so their scores are
-// zeros, and the bits of -infinity are simply or-ed in: two instructions per score.
+// -infinity for the scores of the keys that strip i of a tile leaves out: a bit as a word of ones or zeros, and a select
+// by it, two instructions per score.
 __device__ static inline void leave_out(f32x16& s, uint64_t bits, int i) {
   const unsigned off = ~(unsigned)(bits >> (32 * i)) >> (4 * ((threadIdx.x & 63) >> 5));
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
     const unsigned all = (unsigned)__builtin_amdgcn_sbfe((int)off, acc_row(e), 1);
-    s[e] = __uint_as_float(__float_as_uint(s[e]) | (all & 0xff800000u));
+    s[e] = __uint_as_float((all & 0xff800000u) | (~all & __float_as_uint(s[e])));
   }
 }
 
@@ -841,8 +841,8 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dkv_kernel(Attn 
     };
     auto put = [&](int buf, int r0) {
       if (r0 >= row1) return;
-      nq.put(qt[buf], a.D, r0, a.rows);
-      ng.put(gt[buf], a.D, r0, a.rows);
+      nq.put(qt[buf], a.D, 0, QB);                      // rows behind the list repeat its last one: their p is 2^-inf
+      ng.put(gt[buf], a.D, 0, QB);
       if (threadIdx.x < QB) {
         reinterpret_cast<float*>(shift_s[buf])[threadIdx.x] = lse_n == minus_inf() ? minus_inf() : Terms<T>::BIAS - lse_n * LOG2E;
         reinterpret_cast<float*>(delta_s[buf])[threadIdx.x] = delta_n;
@@ -1352,15 +1352,21 @@ __global__ __launch_bounds__(256) void attn_rows_bwd_kernel(Attn a) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       delta[r] = 0.f;
-#pragma unroll
-      for (int j = 0; j < V; ++j) A[r][j] = S[r][j] = 0.f;
-      for (int w = 0; w < NW; ++w) {
-        const float* from = dyn + (w * R + r) * W;
-        delta[r] += from[2 * LPK * V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) { A[r][j] += from[d + j]; S[r][j] += from[LPK * V + d + j]; }
-      }
+      for (int w = 0; w < NW; ++w) delta[r] += dyn[(w * R + r) * W + 2 * LPK * V];
     }
+    if (wave == 0)                                     // only this one writes dq
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          float x = 0.f, y = 0.f;
+          for (int w = 0; w < NW; ++w) {
+            x += dyn[(w * R + r) * W + d + j];
+            y += dyn[(w * R + r) * W + LPK * V + d + j];
+          }
+          A[r][j] = x;
+          S[r][j] = y;
+        }
   } else if constexpr (FUSED) {
     wave_fence();                                      // p and dp of this wave's other lanes
   }
@@ -1398,6 +1404,7 @@ __global__ __launch_bounds__(256) void attn_rows_kv_kernel(Attn a, int chunks, i
   const bool lone = lone_key(a, b);
   float q[R][V], g[R][V], delta[R];
   const int64_t n_rows = (int64_t)a.B * a.Hkv * a.rows;
+  const int width = 2 * a.D + 1;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const bool in = r < a.rows;
@@ -1407,21 +1414,27 @@ __global__ __launch_bounds__(256) void attn_rows_kv_kernel(Attn a, int chunks, i
     delta[r] = 0.f;
     if (in) {
       const int64_t rid = row_id(a, b, ra);
-      for (int s = 0; s < a.splits; ++s) delta[r] += a.part[(s * n_rows + rid) * (2 * a.D + 1) + 2 * a.D];
-      if (chunk == 0 && wave == 0 && slot == 0 && in_d) {
-        float dq[V];
+      for (int i = lane; i < a.splits; i += 64) delta[r] += a.part[(i * n_rows + rid) * width + 2 * a.D];
+    }
+    delta[r] = wave_sum(delta[r]);
+  }
+  if (chunk == 0) {                                    // a thread per element of dq
+    __shared__ float delta_s[R];
+    if (threadIdx.x == 0)
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          float A = 0.f, S = 0.f;
-          for (int s = 0; s < a.splits; ++s) {
-            const float* part = a.part + (s * n_rows + rid) * (2 * a.D + 1);
-            A += part[d + j];
-            S += part[a.D + d + j];
-          }
-          dq[j] = lone ? 0.f : a.scale * (A - delta[r] * S);
-        }
-        *reinterpret_cast<uint4*>((T*)a.dq.p + (int64_t)b * a.dq.b + (int64_t)ra.t * a.dq.t + (int64_t)ra.h * a.dq.h + d) = Packet<T>::pack(dq);
+      for (int r = 0; r < R; ++r) delta_s[r] = delta[r];
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.rows * a.D; i += 256) {
+      const int r = i / a.D, at = i - r * a.D;
+      const RowAt ra = row_at(a, r, hk);
+      const float* part = a.part + row_id(a, b, ra) * width + at;
+      float A = 0.f, S = 0.f;
+#pragma unroll 4
+      for (int k = 0; k < a.splits; ++k) {
+        A += part[k * n_rows * width];
+        S += part[k * n_rows * width + a.D];
       }
+      const_cast<T*>(row_ptr<T>(a.dq, b, ra))[at] = (T)(lone ? 0.f : a.scale * (A - delta_s[r] * S));
     }
   }
   const int k0 = chunk * per_chunk, k1 = min(a.Tk, k0 + per_chunk);
@@ -1441,17 +1454,17 @@ static int padded_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96
 static int strip_waves(int n) { return n <= 32 ? 1 : n <= 64 ? 2 : 4; }
 
 // Splits of the key axis: only where the row tiles alone leave part of the chip without waves (every split writes its
-// share of the result as fp32, which is read again), and never below 256 keys each.  One block of four waves per CU is
+// share of the result as fp32, which is read again), and never below 64 keys each.  One block of four waves per CU is
 // enough for tiles that are computed; single waves want four per CU (16 rows against 32768 keys of 128: 48 us with 1024,
 // 56 with 2048, 70 with 512).
 static int key_splits(int64_t blocks, int waves, int Tk) {
-  const int64_t want = (waves == 1 ? 1024 : 512) / (blocks < 1 ? 1 : blocks), most = Tk / 256;
+  const int64_t want = (waves == 1 ? 1024 : 512) / (blocks < 1 ? 1 : blocks), most = Tk / 64;
   const int64_t n = want < most ? want : most;
   return (int)(n < 1 ? 1 : n);
 }
-// Splits of the row list for dk / dv, on the same grounds: at least 256 rows each.
+// Splits of the row list for dk / dv, on the same grounds: at least 64 rows each.
 static int list_splits(int64_t blocks, int rows) {
-  const int64_t want = 512 / (blocks < 1 ? 1 : blocks), most = rows / 256;
+  const int64_t want = 512 / (blocks < 1 ? 1 : blocks), most = rows / 64;
   const int64_t n = want < most ? want : most;
   return (int)(n < 1 ? 1 : n);
 }
@@ -1463,7 +1476,7 @@ static void rows_plan(Attn* a, int dtype) {
   const int64_t pairs = (int64_t)a->B * a->Hkv, step = rows_step_keys(a->D, dtype) * ROW_STEP;
   const int64_t most = cdiv(a->Tk < 1 ? 1 : a->Tk, step), want = pairs < 1 ? 1 : 8192 / pairs;
   const int64_t waves = want < 1 ? 1 : want < most ? want : most;
-  a->waves = waves >= 2 ? 4 : 1;
+  a->waves = waves >= 4 ? 4 : 1;
   int64_t splits = waves / 8;                          // below eight waves one block holds the pair
   a->splits = (int)(splits < 1 ? 1 : splits > 128 ? 128 : splits);
   a->per_split = (int)align_up(cdiv(a->Tk, a->splits), step);
@@ -1472,6 +1485,8 @@ static void rows_plan(Attn* a, int dtype) {
 
 static void attn_plan(Attn* a, int dtype) {
   a->rows = a->Tq * a->G;
+  // Up to four rows the vector units keep up with memory.  Eight were tried in the backward and lost (8 rows against 8757
+  // keys of 128: 430 us for the two passes, 280 for the tiles').
   if (a->rows >= 1 && a->rows <= 4) {
     rows_plan(a, dtype);
     return;
