@@ -1450,8 +1450,13 @@ static int rows_lanes(int D, int dtype) {
 }
 static int rows_step_keys(int D, int dtype) { return 64 / rows_lanes(D, dtype); }
 static int padded_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
-// Waves of a block: as many as there are strips of 32 rows (or keys), one, two or four
-static int strip_waves(int n) { return n <= 32 ? 1 : n <= 64 ? 2 : 4; }
+// Waves of a block: as many as there are strips of 32 rows (or keys), one, two or four.  Where even walks of 64 along the
+// other axis would not give every CU eight blocks, four in any case: the idle ones help to stage the tiles (6 rows of 22
+// keys, fp32, D 104, the three passes: 39 us for 60; 16 rows against 32768 keys, in walks enough: 48 us alone, 58 by four).
+static int strip_waves(int n, int64_t pairs, int other) {
+  if (pairs * cdiv(other, 64) < 2048) return 4;
+  return n <= 32 ? 1 : n <= 64 ? 2 : 4;
+}
 
 // Splits of the key axis: only where the row tiles alone leave part of the chip without waves (every split writes its
 // share of the result as fp32, which is read again), and never below 64 keys each.  One block of four waves per CU is
@@ -1492,12 +1497,12 @@ static void attn_plan(Attn* a, int dtype) {
     return;
   }
   a->few = 0;
-  a->row_waves = strip_waves(a->rows);
+  a->row_waves = strip_waves(a->rows, (int64_t)a->B * a->Hkv, a->Tk);
   a->row_tiles = (int)cdiv(a->rows, 32 * a->row_waves);
   a->splits = key_splits((int64_t)a->row_tiles * a->B * a->Hkv, a->row_waves, a->Tk);
   a->per_split = (int)align_up(cdiv(a->Tk, a->splits), 64);
   a->splits = a->Tk > 0 ? (int)cdiv(a->Tk, a->per_split) : 1;
-  a->key_waves = strip_waves(a->Tk);
+  a->key_waves = strip_waves(a->Tk, (int64_t)a->B * a->Hkv, a->rows);
   a->key_tiles = (int)cdiv(a->Tk, 32 * a->key_waves);
   a->row_splits = list_splits((int64_t)a->key_tiles * a->B * a->Hkv, a->rows);
   a->rows_per = (int)align_up(cdiv(a->rows, a->row_splits), 64);
