@@ -8,7 +8,7 @@
 // All products run on 32x32x16 matrix instructions.  The forward and the dq pass keep scores transposed (keys down,
 // query rows across): a lane owns one query row, so the running maximum, the sum and the rescaling are per-lane
 // scalars, and its 16 scores of a 32-key strip are already the second operand of the product with V (or K) once that
-// operand's rows are taken in the same order (kf_key below), which the transposing LDS read delivers.  The dk / dv pass
+// operand's rows are taken in the same order (Tile::cols), which the transposing LDS read delivers.  The dk / dv pass
 // is the mirror image: a lane owns one key, the strip runs over query rows.
 // fp32 tensors are split into three bf16 terms (24 significant bits) and every product is the six largest of the nine
 // term products; the sums are fp32 in all types.  For 16-bit tensors p and ds are rounded to the tensors' type before
@@ -21,7 +21,6 @@
 namespace ctr {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x4v __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));

@@ -267,3 +267,74 @@ def test_another_stream_and_replays(dtype):
             want = _run(q, k, v, dout, sl)
             for n in want:
                 assert torch.equal(bufs[n], want[n]), (rep, n)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('B,Tq,Tk,H,Hkv,D', [(2, 100, 70, 6, 2, 64), (2, 33, 130, 5, 1, 32), (1, 3, 200, 64, 1, 16),
+                                             (2, 70, 90, 14, 2, 96), (1, 1, 300, 40, 1, 128), (2, 9, 40, 33, 1, 24)])
+def test_groups_of_any_size(B, Tq, Tk, H, Hkv, D, dtype):
+    """3, 5, 7, 33, 40 and 64 query heads to a key head: groups that no tile of rows holds whole."""
+    q, k, v, dout = _make(B, Tq, Tk, H, Hkv, D, dtype, seed=25)
+    _check(_run(q, k, v, dout), attention(q, k, v, dout=dout))
+
+
+@pytest.mark.parametrize('Tq', [1, 40])
+def test_lengths_out_of_range_and_masks_of_other_forms(Tq):
+    """Lengths below zero and beyond Tk are taken as none and all; masks as bytes, one row for all samples, strided rows."""
+    q, k, v, dout = _make(3, Tq, 50, 2, 2, 32, torch.bfloat16, seed=27)
+    sl = torch.tensor([-3, 70, 2 ** 31 - 1], dtype=torch.int32, device=DEV)
+    _check(_run(q, k, v, dout, sl), attention(q, k, v, torch.tensor([0, 50, 50]), dout=dout))
+    keep = torch.rand(3, 90, generator=torch.Generator().manual_seed(1)) < 0.5
+    for mask in ((keep * 255).to(torch.uint8).to(DEV)[:, 7:57], keep.to(DEV)[:1, :50].expand(3, 50), keep.to(DEV)[:, 1:51]):
+        _check(_run(q, k, v, dout, None, mask), attention(q, k, v, None, mask, dout=dout))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('Tq', [1, 45])
+def test_time_before_batch(dtype, Tq):
+    q, k, v, dout = (t.transpose(0, 1).contiguous().transpose(0, 1) for t in _make(3, Tq, 70, 4, 2, 64, dtype, seed=29))
+    _check(_run(q, k, v, dout), attention(q, k, v, dout=dout))
+
+
+@pytest.mark.parametrize('Tq', [1, 40])
+def test_offsets_beyond_32_bits(Tq):
+    """Rows of a cache 64 MiB apart: the last ones lie beyond 2^31 bytes, a tile's rows beyond 2^31 of its first."""
+    Tk, D, far = 40, 32, 1 << 24
+    q, k, v, dout = _make(1, Tq, Tk, 1, 1, D, torch.float32, seed=31)
+    want = attention(q, k, v, dout=dout)
+    cache = torch.empty(Tk * far, device=DEV)
+    view = lambda at: cache.as_strided((1, Tk, 1, D), (Tk * far, far, D, 1), at)
+    kf, vf = view(0), view(64)
+    kf.copy_(k)
+    vf.copy_(v)
+    got = _run(q, kf, vf)
+    _check(got, {n: want[n] for n in ('out', 'lse')})
+    from recommendation_amd import ops
+    dq, dk, dv = torch.empty_like(q), view(128), view(192)
+    ops.cross_attn_bwd(dout, q, kf, vf, got['out'], got['lse'], dq, dk, dv, ws=_ws())
+    _check(dict(dq=dq, dk=dk, dv=dv), {n: want[n] for n in ('dq', 'dk', 'dv')})
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('B,Tq,Tk,D', [(70001, 1, 3, 8), (20003, 6, 2, 16)])
+def test_very_many_samples(B, Tq, Tk, D, dtype):
+    q, k, v, dout = _make(B, Tq, Tk, 1, 1, D, dtype, seed=33)
+    sl = (torch.arange(B) % (Tk + 1)).to(torch.int32).to(DEV)
+    _check(_run(q, k, v, dout, sl), attention(q, k, v, sl, dout=dout))
+
+
+def test_two_streams_at_once():
+    """Two calls in flight on two streams, each with its own workspace."""
+    cases = [_make(2, 1, 3000, 4, 2, 64, torch.bfloat16, seed=35), _make(2, 90, 400, 4, 2, 64, torch.bfloat16, seed=36)]
+    want = [_run(*c) for c in cases]
+    streams, ws = [torch.cuda.Stream() for _ in cases], [_ws() for _ in cases]
+    for rep in range(3):
+        got = []
+        for s, c, w in zip(streams, cases, ws):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(_run(*c, ws=w))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            for n in b:
+                assert torch.equal(a[n], b[n]), n

@@ -38,7 +38,7 @@ def _run(x, dy, gamma, beta, eps=1e-5, into=None, ws=None):
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('rows,cols', [(1, 1), (3, 2), (70, 5), (200, 8), (33, 16), (500, 17), (129, 33), (65, 64), (257, 100),
                                        (40, 128), (50, 257), (31, 512), (9, 1001), (21, 1024), (7, 2049), (13, 4096),
-                                       (5, 4097), (3, 16384), (2, 16385), (70, 20000), (5000, 24), (1, 1000), (300, 1536)])
+                                       (5, 4097), (3, 16384), (2, 16385), (70, 20000), (5000, 24), (1, 1000), (300, 1536), (300000, 20)])
 def test_forward_and_gradients(rows, cols, dtype):
     x, dy, gamma, beta = _make(rows, cols, dtype)
     got, want = _run(x, dy, gamma, beta), layer_norm(x, gamma, beta, dy=dy)
