@@ -1466,10 +1466,16 @@ static int key_splits(int64_t blocks, int waves, int Tk) {
   const int64_t n = want < most ? want : most;
   return (int)(n < 1 ? 1 : n);
 }
-// Splits of the row list for dk / dv, on the same grounds: at least 64 rows each.
-static int list_splits(int64_t blocks, int rows) {
+// Splits of the row list for dk / dv, on the same grounds: at least 64 rows each.  fp32: at most 1024, since one
+// accumulator that takes every row of a long list rounds after each 16 of them (4592 rows: 1.1e-6 off, in five splits
+// 0.5e-6) - as far as the splits stay small beside the rows themselves.
+static int list_splits(int64_t blocks, int rows, int keys, int dtype) {
   const int64_t want = 512 / (blocks < 1 ? 1 : blocks), most = rows / 64;
-  const int64_t n = want < most ? want : most;
+  int64_t n = want < most ? want : most;
+  if (dtype == CTR_F32) {
+    const int64_t fine = cdiv(rows, 1024), small = rows / (4 * (int64_t)(keys < 1 ? 1 : keys));
+    n = n > fine ? n : fine < small ? fine : n > small ? n : small;
+  }
   return (int)(n < 1 ? 1 : n);
 }
 
@@ -1503,7 +1509,7 @@ static void attn_plan(Attn* a, int dtype) {
   a->splits = a->Tk > 0 ? (int)cdiv(a->Tk, a->per_split) : 1;
   a->key_waves = strip_waves(a->Tk, (int64_t)a->B * a->Hkv, a->rows);
   a->key_tiles = (int)cdiv(a->Tk, 32 * a->key_waves);
-  a->row_splits = list_splits((int64_t)a->key_tiles * a->B * a->Hkv, a->rows);
+  a->row_splits = list_splits((int64_t)a->key_tiles * a->B * a->Hkv, a->rows, a->Tk, dtype);
   a->rows_per = (int)align_up(cdiv(a->rows, a->row_splits), 64);
   a->row_splits = a->rows > 0 ? (int)cdiv(a->rows, a->rows_per) : 1;
 }
@@ -1542,7 +1548,7 @@ static int attn_shape(const char* what, const ctr_attn_t* s, Attn* a) {
   attn_plan(a, s->dtype);
   const int64_t pairs = ((int64_t)a->B * a->Hkv + 7) / 8 * 8;
   CTR_REQUIRE((a->few ? 1 : (int64_t)a->row_tiles) * pairs * a->splits < (1ll << 31) &&
-              cdiv(a->Tk, 32) * pairs < (1ll << 31) / 4, "%s: too many tiles", what);
+              cdiv(a->Tk, 32) * pairs * (a->few ? 1 : a->row_splits) < (1ll << 31), "%s: too many tiles", what);
   return CTR_OK;
 }
 
