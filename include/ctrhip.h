@@ -800,7 +800,7 @@ int ctr_all2allv(ctr_comm_t* comm, const void* send, const int64_t* send_offset,
  * ---------------------------------------------------------------------------------- */
 typedef struct {
   int B, Tq, Tk, H, Hkv, D, dtype;
-  float scale;             /* > 0 */
+  float scale;             /* 1e-30 to 1e30 */
   const int32_t* sl;       /* [B], optional */
   const uint8_t* mask;     /* rows of mask_ld bytes, optional */
   int64_t mask_ld;

@@ -220,7 +220,13 @@ __device__ static inline bool lone_key(const Attn& a, int b) {
   if (!a.mask) return false;
   const uint8_t* mask = a.mask + (int64_t)b * a.mask_ld;
   int n = 0;
-  for (int base = 0; base < len && n < 2; base += 64) n += __popcll(__ballot(base + lane < len && mask[min(base + lane, len - 1)]));
+  for (int base = 0; base < len && n < 2; base += 512) {               // eight loads in flight: the first keys may all be off
+    bool on[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) on[i] = mask[min(base + i * 64 + lane, len - 1)] != 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) n += __popcll(__ballot(on[i] && base + i * 64 + lane < len));
+  }
   return n < 2;
 }
 
@@ -460,6 +466,9 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? WAVES<T, DP> : FWD_WAVES<T, DP>
     const auto& vs = vt[at];
     if constexpr (NBUF == 2) at ^= 1;
     if (!busy) continue;
+    const bool whole = !mask && kb + KT <= k1;
+    const uint64_t bits = whole ? 0 : key_bits(mask, kb, k1, KT);
+    if (!whole && !bits) continue;                     // the mask leaves nothing of this tile
     f32x16 s[NS];
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
@@ -467,8 +476,7 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? WAVES<T, DP> : FWD_WAVES<T, DP>
 #pragma unroll
       for (int c = 0; c < NK; ++c) s[i] = mfma<T>(ks.rows(i * 32, c * 16), qf[c], s[i]);
     }
-    if (mask || kb + KT > k1) {
-      const uint64_t bits = key_bits(mask, kb, k1, KT);
+    if (!whole) {
 #pragma unroll
       for (int i = 0; i < NS; ++i) leave_out(s[i], bits, i);
     }
@@ -700,6 +708,7 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dq_kernel(Attn a
 
   auto tile_work = [&](int buf, bool whole, int kb) {
     const uint64_t bits = whole ? 0 : key_bits(mask, kb, k1, KT);
+    if (!whole && !bits) return;                       // the mask leaves nothing of this tile
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       f32x16 s = f32x16{}, dp = f32x16{};
@@ -1536,7 +1545,7 @@ static int attn_shape(const char* what, const ctr_attn_t* s, Attn* a) {
   CTR_REQUIRE(s->B >= 0 && s->Tq >= 0 && s->Tk >= 0 && s->H >= 1 && s->Hkv >= 1 && s->H % s->Hkv == 0,
               "%s: B %d Tq %d Tk %d H %d Hkv %d (Hkv must divide H)", what, s->B, s->Tq, s->Tk, s->H, s->Hkv);
   CTR_REQUIRE(s->D >= 8 && s->D <= 128 && s->D % 8 == 0, "%s: head size %d is not a multiple of 8 up to 128", what, s->D);
-  CTR_REQUIRE(s->scale > 0.f && s->scale <= 3.0e38f, "%s: scale must be positive and finite", what);
+  CTR_REQUIRE(s->scale >= 1e-30f && s->scale <= 1e30f, "%s: scale must lie between 1e-30 and 1e30", what);
   CTR_REQUIRE((int64_t)s->Tq * (s->H / s->Hkv) < (1 << 30) && s->Tk < (1 << 30) && (int64_t)s->B * s->H < (1 << 30),
               "%s: more than 2^30 rows, keys or heads", what);
   CTR_REQUIRE(!s->mask || s->mask_ld >= 0, "%s: the mask has a negative stride", what);

@@ -1255,8 +1255,8 @@ def _attn_args(q, k, sl, mask, scale):
     if Tq * (H // Hkv) >= 1 << 30 or Tk >= 1 << 30 or B * H >= 1 << 30:
         raise ValueError('more than 2^30 query rows, keys or heads')
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not 0.0 < scale <= 3e38:
-        raise ValueError('scale must be positive and finite')
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError('scale must lie between 1e-30 and 1e30')
     mp = mld = sp = 0
     if mask is not None:
         if mask.dtype not in (torch.bool, torch.uint8):

@@ -290,6 +290,24 @@ def test_lengths_out_of_range_and_masks_of_other_forms(Tq):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('Tq,Tk', [(1, 700), (40, 700), (150, 1600), (20, 9000)])
+def test_padding_before_the_keys(dtype, Tq, Tk):
+    """Whole tiles and whole splits that the mask leaves nothing of, before, between and behind the keys of a sample; one
+    sample has its only key at the end."""
+    q, k, v, dout = _make(4, Tq, Tk, 2, 1, 64, dtype)
+    mask = torch.zeros(4, Tk, dtype=torch.bool)
+    mask[0, Tk - 300:] = True
+    mask[1, Tk - 1] = True
+    mask[2, 5], mask[2, Tk - 2] = True, True
+    mask[3, 130:131 + Tk // 3] = True
+    mask = mask.to(DEV)
+    want = attention(q, k, v, None, mask, dout=dout)
+    k2, v2 = k.clone(), v.clone()
+    k2[~mask], v2[~mask] = math.nan, math.inf
+    _check(_run(q, k2, v2, dout, None, mask), want)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('Tq', [1, 45])
 def test_time_before_batch(dtype, Tq):
     q, k, v, dout = (t.transpose(0, 1).contiguous().transpose(0, 1) for t in _make(3, Tq, 70, 4, 2, 64, dtype, seed=29))

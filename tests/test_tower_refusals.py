@@ -52,6 +52,14 @@ def test_cross_attention_refuses(kw, error):
         _fwd(**kw)
 
 
+@pytest.mark.parametrize('scale', [1e-40, 2.4e38])
+def test_cross_attention_refuses_scales_that_leave_fp32(scale):
+    """scale / ln 2 has to be an ordinary fp32 number."""
+    with pytest.raises(ValueError, match='1e-30'):
+        _fwd(scale=scale)
+    assert _abi_fwd(shape=_shape(scale=scale)) == -1 and b'1e-30' in _lib.load().ctr_last_error()
+
+
 @pytest.mark.parametrize('D', [4, 12, 20, 136, 256])
 def test_cross_attention_refuses_head_sizes(D):
     a, z = _attn(D=D)
