@@ -47,6 +47,13 @@ def test_forward_and_gradients(rows, cols, dtype):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('rows,cols', [(600, 2048), (37, 1025), (9, 4104), (530, 8192), (3, 8193), (1, 6001)])
+def test_rows_at_the_limits_of_the_kernels(rows, cols, dtype):
+    """Rows that just fill half or all of a block's registers, or pass that by an element; more rows than blocks."""
+    test_forward_and_gradients(rows, cols, dtype)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('rows,cols,pad', [(40, 24, 3), (33, 128, 1), (17, 999, 25), (6, 5000, 7), (4, 17000, 5)])
 def test_rows_of_a_wider_buffer(rows, cols, pad, dtype):
     """Rows that start at any element, results into a wider buffer whose other columns stay."""
