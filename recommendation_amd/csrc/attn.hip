@@ -16,6 +16,10 @@
 // themselves); fp16's narrow exponent is met by a power of two on p (2^14) and a running one per row on ds.
 // A key behind sl[b] or off in the mask is staged as zeros and its p is set to zero, so nothing that its memory holds
 // reaches a result.  A row without keys gives zeros, lse = -inf and no gradient.  No float atomics: same bits every run.
+// Bound: matrix and vector instructions of a SIMD hardly overlap here (per wave, two to a SIMD: 4 products 63 ns, 32 fma
+// 38, 8 exp 31, all three 107), so the time of a tile is their sum.  16 heads of 2048 x 4096 of 64, batch 8, bf16: forward
+// 365 us, 750 TFLOP/s counting its two products; dq 600 us, dk / dv 715 us, 687 and 769 TFLOP/s counting three and four
+// (a large bf16 matrix product reaches 1200 on this card).
 #include "types.h"
 
 namespace ctr {
@@ -390,9 +394,10 @@ __device__ static inline void leave_out(f32x16& s, uint64_t bits, int i) {
 // the register file and moves every value over and back (a third of the instructions of the forward's loop).
 template <class T, int DP>
 constexpr int WAVES = Terms<T>::NP == 3 && DP > 64 ? 1 : 2;
-// The forward needs fewer registers: four waves at head sizes up to 64 (tiles of 64 keys), three above (32 keys).
-template <class T, int DP>
-constexpr int FWD_WAVES = Terms<T>::NP == 3 ? (DP > 64 ? 1 : DP > 32 ? 2 : 3) : DP > 64 ? 3 : 4;
+// The forward of 16-bit tensors needs fewer registers: at head sizes up to 64, blocks of four waves run four to a SIMD
+// (16 heads of 2048 x 4096 of 64, batch 8, bf16: 369 us; 410 with three).  Above that, and for fp32, more change nothing.
+template <class T, int DP, int NW>
+constexpr int FWD_WAVES = NW == 4 && Terms<T>::NP == 1 && DP <= 64 ? 4 : WAVES<T, DP>;
 
 // ---- forward -------------------------------------------------------------------------------------------------------
 // A wave owns 32 query rows; the NW waves of a block share each tile of KT keys.  Two tiles of LDS and one barrier per
@@ -400,8 +405,11 @@ constexpr int FWD_WAVES = Terms<T>::NP == 3 ? (DP > 64 ? 1 : DP > 32 ? 2 : 3) : 
 // tile i is computed.  One wave alone needs neither.
 // The running maximum is a reference, not the maximum itself: accumulators and sum are rescaled only when a score passes
 // it by more than LIMIT (a power of two), so p stays below 2^(BIAS + LIMIT) and after the first tiles that is rare.
+// (fp16: 2^15, the largest power it holds.)  Tiles of 64 keys where two buffers of them leave room for the waves: 16-bit
+// types up to head size 64 (369 us for the shape above; 416 with 32), 32 keys otherwise (head size 128, 4 x 16 heads of
+// 1025 x 2047: 121 us; 206 with 64; fp32, head size 32, 2048 pairs of 100 x 200: 41 us; 50 with 64).
 template <class T, int DP, int NW, int KT>
-__global__ __launch_bounds__(NW * 64, (NW == 1 ? WAVES<T, DP> : FWD_WAVES<T, DP>)) void attn_fwd_kernel(Attn a) {
+__global__ __launch_bounds__(NW * 64, (FWD_WAVES<T, DP, NW>)) void attn_fwd_kernel(Attn a) {
   constexpr int NS = KT / 32, NK = DP / 16, ND = DP / 32, NBUF = NW > 1 ? 2 : 1;
   constexpr float BIAS = __is_same(T, f16_t) ? 8.f : 0.f, LIMIT = 7.f;
   __shared__ Tile<T, KT, DP> kt[NBUF];
@@ -807,7 +815,9 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dq_kernel(Attn a
   }
 }
 
-// dk and dv.  A wave owns 32 keys and walks the query rows in tiles of QB.
+// dk and dv.  A wave owns 32 keys and walks the query rows in tiles of QB: 64 where registers allow (16-bit types up to
+// head size 64: 715 us for the shape above, 830 with 32; fp32 up to 32: 100 us for 2048 pairs of 100 x 200, 113 with 32),
+// else 32 (head size 128: 138 us for 4 x 16 heads of 1024 x 1024, the same with 64).
 template <class T, int DP, int NW, int QB>
 __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dkv_kernel(Attn a) {
   constexpr int NS = QB / 32, NK = DP / 16, ND = DP / 32;
@@ -1033,8 +1043,11 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(Attn a, int64_t n_rows) {
 //   delta = sum p dp,  A = sum p dp k,  S = sum p k   (dq = scale (A - delta S)),
 // pass two writes dk = scale p (dp - delta) q and dv = p dout from the kept numbers: k and v are read once, delta is
 // the exact row sum.  While p and dp fit the LDS of one block the two passes are one launch.
-constexpr int ROW_STEP = 4;
-constexpr int ROWS_LDS = 4096;                         // (key, row) pairs whose p and dp a block keeps in LDS
+// Measured: 8192 pairs of one row and up to 200 keys of 32, fp32: 43 us forward (5 TB/s), 104 backward (6 TB/s).  128 pairs
+// of one row and 32768 keys of 64, bf16, 1.07 GB of keys and values: 240 us forward (4.5 TB/s), 256 + 287 backward.
+constexpr int ROW_STEP = 4;                            // 2: 3 % slower on those shapes; 8: within 3 % either way
+constexpr int ROWS_LDS = 4096;                         // (key, row) pairs whose p and dp a block keeps in LDS: 104 us in one
+                                                       // launch, 132 in two
 
 template <int LPK>
 __device__ static inline float slot_sum(float v) {
@@ -1488,7 +1501,9 @@ static int list_splits(int64_t blocks, int rows, int keys, int dtype) {
   return (int)(n < 1 ? 1 : n);
 }
 
-// Few rows: waves for about eight per SIMD, each with at least ROW_STEP steps of keys; four to a block, more as splits.
+// Few rows: waves for about eight per SIMD (four or sixteen: within 3 %), each with at least ROW_STEP steps of keys; four to
+// a block, more as splits.  A wave alone where there are pairs enough: nothing to join (32768 pairs of 50 keys, fp32: 78 and
+// 141 us, 85 and 148 by four; of four rows 100 and 176, 183 and 378).
 static void rows_plan(Attn* a, int dtype) {
   a->lanes = rows_lanes(a->D, dtype);
   a->few = a->rows <= 1 ? 1 : a->rows <= 2 ? 2 : 4;
@@ -1700,10 +1715,10 @@ static void attn_bwd_launch(const Attn& a, hipStream_t st) {
   const unsigned kblocks = pair_blocks(a, (int64_t)a.key_tiles * a.row_splits);
   if (kblocks) {
 #define ATTN_DKV(T_, DP_)                                                                                        \
-  constexpr int QB = sizeof(T_) == 2 && DP_ <= 64 ? 64 : 32;                                                     \
+  constexpr int QB = sizeof(T_) == 2 && DP_ <= 64 ? 64 : 32, QB4 = DP_ <= 32 ? 64 : QB;                          \
   if (a.key_waves == 1) attn_dkv_kernel<T_, DP_, 1, 32><<<kblocks, 64, 0, st>>>(a);                              \
   else if (a.key_waves == 2) attn_dkv_kernel<T_, DP_, 2, QB><<<kblocks, 128, 0, st>>>(a);                        \
-  else attn_dkv_kernel<T_, DP_, 4, QB><<<kblocks, 256, 0, st>>>(a)
+  else attn_dkv_kernel<T_, DP_, 4, QB4><<<kblocks, 256, 0, st>>>(a)
     ATTN_DIM(T, a.D, ATTN_DKV);
 #undef ATTN_DKV
     if (a.row_splits > 1)
