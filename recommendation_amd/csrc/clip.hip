@@ -6,14 +6,19 @@
 // a captured graph owns its list.  Squares are summed in fp64: no element of any of the three types overflows or
 // vanishes there, and the fp64 pipe (half the fp32 rate) is far from the bound.  One partial per block, added in block
 // order by every block of the second launch: results are the same bits on every run, and there is no third launch.
+// Measured (60 tensors of fp32 and bf16, 815 MB in all, into other tensors): the squares 165 us, 4.9 TB/s, the scaling
+// 290 us, 5.6 TB/s; a large copy reaches 4.9.  24 small tensors: 4.3 us and 1.5 for the norm, launches.
 #include "types.h"
 #include <math.h>
 
 namespace ctr {
 
 constexpr int CLIP_TENSORS = 96;                     // per launch: 96 * (8 + 8 + 8 + 4) bytes of kernel arguments
-constexpr int CLIP_BLOCKS = 1024;                    // partials per launch at most
-constexpr int CLIP_CHUNK = 32768;                    // bytes of one tensor a block takes at a time (the wider type's)
+// Partials per launch at most; the scaling takes twice as many blocks.  815 MB of squares: 165 us (171 with 512 or 2048).
+constexpr int CLIP_BLOCKS = 1024;
+// Bytes of one tensor that a block takes at a time, eight packets per thread: 165 and 290 us (171 and 291 with twice as
+// much, 165 and 295 with half).
+constexpr int CLIP_CHUNK = 32768;
 
 struct ClipList {
   const void* src[CLIP_TENSORS];
