@@ -391,7 +391,8 @@ __device__ static inline void leave_out(f32x16& s, uint64_t bits, int i) {
 
 // Waves per SIMD the tiled kernels are built for.  Two keep a wave within 256 registers, and only then does the compiler
 // leave the accumulators where the vector units reach them: at one (512 registers) it keeps them in the other half of
-// the register file and moves every value over and back (a third of the instructions of the forward's loop).
+// the register file and moves every value over and back (a third of the instructions of the forward's loop).  Three spill
+// in the backward (head size 64: 940 and 1000 us for 600 and 715).
 template <class T, int DP>
 constexpr int WAVES = Terms<T>::NP == 3 && DP > 64 ? 1 : 2;
 // The forward of 16-bit tensors needs fewer registers: at head sizes up to 64, blocks of four waves run four to a SIMD
