@@ -18,7 +18,7 @@
 // reaches a result.  A row without keys gives zeros, lse = -inf and no gradient.  No float atomics: same bits every run.
 // Bound: matrix and vector instructions of a SIMD hardly overlap here (per wave, two to a SIMD: 4 products 63 ns, 32 fma
 // 38, 8 exp 31, all three 107), so the time of a tile is their sum.  16 heads of 2048 x 4096 of 64, batch 8, bf16: forward
-// 365 us, 750 TFLOP/s counting its two products; dq 600 us, dk / dv 715 us, 687 and 769 TFLOP/s counting three and four
+// 365 us, 750 TFLOP/s counting its two products; dq 600 us, dk / dv 660 us, 687 and 830 TFLOP/s counting three and four
 // (a large bf16 matrix product reaches 1200 on this card).
 #include "types.h"
 
@@ -392,13 +392,26 @@ __device__ static inline void leave_out(f32x16& s, uint64_t bits, int i) {
 // Waves per SIMD the tiled kernels are built for.  Two keep a wave within 256 registers, and only then does the compiler
 // leave the accumulators where the vector units reach them: at one (512 registers) it keeps them in the other half of
 // the register file and moves every value over and back (a third of the instructions of the forward's loop).  Three spill
-// in the backward (head size 64: 940 and 1000 us for 600 and 715).
+// in the backward (head size 64: 940 and 1000 us for 600 and 710).
 template <class T, int DP>
 constexpr int WAVES = Terms<T>::NP == 3 && DP > 64 ? 1 : 2;
 // The forward of 16-bit tensors needs fewer registers: at head sizes up to 64, blocks of four waves run four to a SIMD
 // (16 heads of 2048 x 4096 of 64, batch 8, bf16: 369 us; 410 with three).  Above that, and for fp32, more change nothing.
 template <class T, int DP, int NW>
 constexpr int FWD_WAVES = NW == 4 && Terms<T>::NP == 1 && DP <= 64 ? 4 : WAVES<T, DP>;
+
+// A wave of the backward has two operands of its own (rows of q and dout, or keys of k and v).  16-bit types above head
+// size 64: the second stays in LDS, in registers it spills (4 x 16 heads of 1024 x 1024 of 128, bf16: dq 89 us and dk / dv
+// 97 for 123 and 137) - but not with single waves on keys of 128, which LDS then limits (4096 pairs of 500 rows and 30
+// keys: 304 us for 358).  Head size 64, dk / dv: with that operand in LDS and tiles of 32 rows three waves fit a SIMD (660 us
+// for the shape above, 710 with two), and in blocks of two waves fp16 spills no more (4096 pairs of 500 rows and 60 keys:
+// 199 us for 244; bf16 192 for 178).  dq gains nothing from it (600 either way).
+template <class T, int DP, int NW>
+constexpr int DKV_WAVES = NW == 4 && Terms<T>::NP == 1 && DP == 64 ? 3 : WAVES<T, DP>;
+template <class T, int DP, int NW>
+constexpr bool DKV_ASIDE = Terms<T>::NP == 1 && (NW == 1 ? DP == 96 : DP >= 64);
+template <class T, int DP>
+constexpr bool DQ_ASIDE = Terms<T>::NP == 1 && DP > 64;
 
 // ---- forward -------------------------------------------------------------------------------------------------------
 // A wave owns 32 query rows; the NW waves of a block share each tile of KT keys.  Two tiles of LDS and one barrier per
@@ -652,7 +665,9 @@ template <class T, int DP, int NW, int KT>
 __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dq_kernel(Attn a) {
   constexpr int NS = KT / 32, NK = DP / 16, ND = DP / 32, NBUF = NW > 1 ? 2 : 1;
   constexpr bool F16 = __is_same(T, f16_t), KEYS = Terms<T>::NP == 1;
+  constexpr bool ASIDE = DQ_ASIDE<T, DP>;
   __shared__ Tile<T, KT, DP> kt[NBUF], vt[NBUF];
+  __shared__ Tile<T, ASIDE ? 32 : 1, DP> mine[ASIDE ? NW : 1];         // a wave's own rows of dout
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const BlockAt ba = block_at(a, a.row_tiles * a.splits);
   if (ba.pair >= a.B * a.Hkv) return;
@@ -681,7 +696,7 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dq_kernel(Attn a
     nv.put(vt[buf], a.D, kb, k1, mask, left);
   };
   load(k0);
-  Frag<T> qf[NK], gf[NK];
+  Frag<T> qf[NK], gf[ASIDE ? 1 : NK];
   float delta = 0.f, shift = minus_inf();              // a row without keys: p = 2^-inf
   {
     const int r = r0 + (lane & 31);
@@ -700,7 +715,8 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dq_kernel(Attn a
       raw_floats<T>(w, wv);
 #pragma unroll
       for (int j = 0; j < 8; ++j) delta = fmaf(gv[j], wv[j], delta);
-      gf[s] = raw_frag<T>(g);
+      if constexpr (ASIDE) mine[wave].put(lane & 31, d, raw_frag<T>(g));
+      else gf[s] = raw_frag<T>(g);
     }
     delta = half_swap_sum(delta, delta);
     if (in) {
@@ -724,7 +740,8 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dq_kernel(Attn a
 #pragma unroll
       for (int c = 0; c < NK; ++c) {
         s = mfma<T>(kt[buf].rows(i * 32, c * 16), qf[c], s);
-        dp = mfma<T>(vt[buf].rows(i * 32, c * 16), gf[c], dp);
+        if constexpr (ASIDE) dp = mfma<T>(vt[buf].rows(i * 32, c * 16), mine[wave].rows(0, c * 16), dp);
+        else dp = mfma<T>(vt[buf].rows(i * 32, c * 16), gf[c], dp);
       }
       if (!whole) leave_out(s, bits, i);
 #pragma unroll
@@ -816,14 +833,15 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dq_kernel(Attn a
   }
 }
 
-// dk and dv.  A wave owns 32 keys and walks the query rows in tiles of QB: 64 where registers allow (16-bit types up to
-// head size 64: 715 us for the shape above, 830 with 32; fp32 up to 32: 100 us for 2048 pairs of 100 x 200, 113 with 32),
-// else 32 (head size 128: 138 us for 4 x 16 heads of 1024 x 1024, the same with 64).
+// dk and dv.  A wave owns 32 keys and walks the query rows in tiles of QB: 64 where registers allow (head size 32: fp32
+// 100 us for 2048 pairs of 100 x 200, 113 with 32; bf16 209 us for 8 x 16 heads of 2048 x 2048, 225 with 32), else 32.
 template <class T, int DP, int NW, int QB>
-__global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dkv_kernel(Attn a) {
+__global__ __launch_bounds__(NW * 64, (DKV_WAVES<T, DP, NW>)) void attn_dkv_kernel(Attn a) {
   constexpr int NS = QB / 32, NK = DP / 16, ND = DP / 32;
   constexpr bool F16 = __is_same(T, f16_t);
+  constexpr bool ASIDE = DKV_ASIDE<T, DP, NW>;
   __shared__ Tile<T, QB, DP> qt[2], gt[2];
+  __shared__ Tile<T, ASIDE ? 32 : 1, DP> mine[ASIDE ? NW : 1];         // a wave's own rows of v
   __shared__ float4 shift_s[2][QB / 4], delta_s[2][QB / 4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const BlockAt ba = block_at(a, a.key_tiles * a.row_splits);
@@ -868,9 +886,18 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dkv_kernel(Attn 
       }
     };
     load(row0);
-    Frag<T> kf[NK], vf[NK];
+    Frag<T> kf[NK], vf[ASIDE ? 1 : NK];
     load_row_frags<T, DP>((const T*)a.k.p + (int64_t)b * a.k.b + (int64_t)hk * a.k.h + (int64_t)(on ? key : 0) * a.k.t, on, a.D, kf);
-    load_row_frags<T, DP>((const T*)a.v.p + (int64_t)b * a.v.b + (int64_t)hk * a.v.h + (int64_t)(on ? key : 0) * a.v.t, on, a.D, vf);
+    const T* vp = (const T*)a.v.p + (int64_t)b * a.v.b + (int64_t)hk * a.v.h + (int64_t)(on ? key : 0) * a.v.t;
+    if constexpr (ASIDE) {
+#pragma unroll
+      for (int s = 0; s < NK; ++s) {
+        const int d = s * 16 + (lane >> 5) * 8;
+        mine[wave].put(lane & 31, d, raw_frag<T>(on && d < a.D ? raw_load(vp + d) : raw_zero<T>()));
+      }
+    } else {
+      load_row_frags<T, DP>(vp, on, a.D, vf);
+    }
     if (a.D < DP) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -886,7 +913,8 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dkv_kernel(Attn 
 #pragma unroll
         for (int c = 0; c < NK; ++c) {
           s = mfma<T>(qt[buf].rows(i * 32, c * 16), kf[c], s);
-          dp = mfma<T>(gt[buf].rows(i * 32, c * 16), vf[c], dp);
+          if constexpr (ASIDE) dp = mfma<T>(gt[buf].rows(i * 32, c * 16), mine[wave].rows(0, c * 16), dp);
+          else dp = mfma<T>(gt[buf].rows(i * 32, c * 16), vf[c], dp);
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -1716,7 +1744,7 @@ static void attn_bwd_launch(const Attn& a, hipStream_t st) {
   const unsigned kblocks = pair_blocks(a, (int64_t)a.key_tiles * a.row_splits);
   if (kblocks) {
 #define ATTN_DKV(T_, DP_)                                                                                        \
-  constexpr int QB = sizeof(T_) == 2 && DP_ <= 64 ? 64 : 32, QB4 = DP_ <= 32 ? 64 : QB;                          \
+  constexpr int QB = sizeof(T_) == 2 && DP_ <= 32 ? 64 : 32, QB4 = DP_ <= 32 ? 64 : 32;                          \
   if (a.key_waves == 1) attn_dkv_kernel<T_, DP_, 1, 32><<<kblocks, 64, 0, st>>>(a);                              \
   else if (a.key_waves == 2) attn_dkv_kernel<T_, DP_, 2, QB><<<kblocks, 128, 0, st>>>(a);                        \
   else attn_dkv_kernel<T_, DP_, 4, QB4><<<kblocks, 256, 0, st>>>(a)
