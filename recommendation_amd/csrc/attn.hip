@@ -835,14 +835,16 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dq_kernel(Attn a
 
 // dk and dv.  A wave owns 32 keys and walks the query rows in tiles of QB: 64 where registers allow (head size 32: fp32
 // 100 us for 2048 pairs of 100 x 200, 113 with 32; bf16 209 us for 8 x 16 heads of 2048 x 2048, 225 with 32), else 32.
+// Single waves of fp32 do with one buffer, for two leave LDS for two waves per CU (2048 pairs of 200 rows and 30 keys of 96:
+// 302 us for 453); for 16-bit types the registers bound that number.
 template <class T, int DP, int NW, int QB>
 __global__ __launch_bounds__(NW * 64, (DKV_WAVES<T, DP, NW>)) void attn_dkv_kernel(Attn a) {
-  constexpr int NS = QB / 32, NK = DP / 16, ND = DP / 32;
+  constexpr int NS = QB / 32, NK = DP / 16, ND = DP / 32, NBUF = NW > 1 || Terms<T>::NP == 1 ? 2 : 1;
   constexpr bool F16 = __is_same(T, f16_t);
   constexpr bool ASIDE = DKV_ASIDE<T, DP, NW>;
-  __shared__ Tile<T, QB, DP> qt[2], gt[2];
+  __shared__ Tile<T, QB, DP> qt[NBUF], gt[NBUF];
   __shared__ Tile<T, ASIDE ? 32 : 1, DP> mine[ASIDE ? NW : 1];         // a wave's own rows of v
-  __shared__ float4 shift_s[2][QB / 4], delta_s[2][QB / 4];
+  __shared__ float4 shift_s[NBUF][QB / 4], delta_s[NBUF][QB / 4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const BlockAt ba = block_at(a, a.key_tiles * a.row_splits);
   if (ba.pair >= a.B * a.Hkv) return;
@@ -900,7 +902,7 @@ __global__ __launch_bounds__(NW * 64, (DKV_WAVES<T, DP, NW>)) void attn_dkv_kern
     }
     if (a.D < DP) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < NBUF; ++i) {
         clear_tile(qt[i]);
         clear_tile(gt[i]);
       }
@@ -947,14 +949,23 @@ __global__ __launch_bounds__(NW * 64, (DKV_WAVES<T, DP, NW>)) void attn_dkv_kern
         }
       }
     };
-    put(0, row0);
-    load(row0 + QB);
+    if constexpr (NBUF == 2) {
+      put(0, row0);
+      load(row0 + QB);
+    }
     int at = 0;
-    for (int r0 = row0; r0 < row1; r0 += QB, at ^= 1) {
+    for (int r0 = row0; r0 < row1; r0 += QB) {
       __syncthreads();
-      put(at ^ 1, r0 + QB);
-      load(r0 + 2 * QB);
+      if constexpr (NBUF == 2) {
+        put(at ^ 1, r0 + QB);
+        load(r0 + 2 * QB);
+      } else {
+        put(0, r0);
+        load(r0 + QB);
+        __syncthreads();
+      }
       if (busy) tile_work(at);
+      if constexpr (NBUF == 2) at ^= 1;
     }
   }
   const bool lone = lone_key(a, b);
@@ -1448,7 +1459,7 @@ __global__ __launch_bounds__(256) void attn_rows_bwd_kernel(Attn a) {
 template <class T, int R, int LPK>
 __global__ __launch_bounds__(256) void attn_rows_kv_kernel(Attn a, int chunks, int per_chunk) {
   constexpr int V = Packet<T>::V;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LPK, slot = lane / LPK, d = sub * V;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LPK, d = sub * V;
   const int chunk = blockIdx.x % chunks, pair = blockIdx.x / chunks, b = pair / a.Hkv, hk = pair - b * a.Hkv;
   const bool in_d = d < a.D;
   const bool lone = lone_key(a, b);
@@ -1503,7 +1514,10 @@ static int padded_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96
 // Waves of a block: as many as there are strips of 32 rows (or keys), one, two or four.  Where even walks of 64 along the
 // other axis would not give every CU eight blocks, four in any case: the idle ones help to stage the tiles (6 rows of 22
 // keys, fp32, D 104, the three passes: 39 us for 60; 16 rows against 32768 keys, in walks enough: 48 us alone, 58 by four).
-static int strip_waves(int n, int64_t pairs, int other) {
+// fp32 above 96: four, since one wave's tiles alone fill a third of the LDS (2048 pairs of 20 rows and 200 keys of 128,
+// forward 225 us, dq 309; 284 and 466 by single waves; at 96 single waves still win, 43 and 60 us for 53 and 73).
+static int strip_waves(int n, int64_t pairs, int other, int dtype, int D) {
+  if (dtype == CTR_F32 && D > 96) return 4;
   if (pairs * cdiv(other, 64) < 2048) return 4;
   return n <= 32 ? 1 : n <= 64 ? 2 : 4;
 }
@@ -1555,12 +1569,12 @@ static void attn_plan(Attn* a, int dtype) {
     return;
   }
   a->few = 0;
-  a->row_waves = strip_waves(a->rows, (int64_t)a->B * a->Hkv, a->Tk);
+  a->row_waves = strip_waves(a->rows, (int64_t)a->B * a->Hkv, a->Tk, dtype, a->D);
   a->row_tiles = (int)cdiv(a->rows, 32 * a->row_waves);
   a->splits = key_splits((int64_t)a->row_tiles * a->B * a->Hkv, a->row_waves, a->Tk);
   a->per_split = (int)align_up(cdiv(a->Tk, a->splits), 64);
   a->splits = a->Tk > 0 ? (int)cdiv(a->Tk, a->per_split) : 1;
-  a->key_waves = strip_waves(a->Tk, (int64_t)a->B * a->Hkv, a->rows);
+  a->key_waves = strip_waves(a->Tk, (int64_t)a->B * a->Hkv, a->rows, dtype, a->D);
   a->key_tiles = (int)cdiv(a->Tk, 32 * a->key_waves);
   a->row_splits = list_splits((int64_t)a->key_tiles * a->B * a->Hkv, a->rows, a->Tk, dtype);
   a->rows_per = (int)align_up(cdiv(a->rows, a->row_splits), 64);
@@ -1629,6 +1643,10 @@ static int attn_view(const char* what, const char* name, const ctr_heads_t* v, i
   }
   return CTR_OK;
 }
+
+// Whether strip_waves gives blocks of one or two waves
+template <class T, int DP>
+constexpr bool SMALL_BLOCKS = sizeof(T) == 2 || DP <= 96;
 
 #define ATTN_DIM(T, D, CALL)                    \
   do {                                          \
@@ -1710,9 +1728,11 @@ static void attn_fwd_launch(const Attn& a, hipStream_t st) {
   const unsigned blocks = pair_blocks(a, (int64_t)a.row_tiles * a.splits);
 #define ATTN_FWD(T_, DP_)                                                                                        \
   constexpr int KT = sizeof(T_) == 4 || DP_ > 64 ? 32 : 64;                                                      \
-  if (a.row_waves == 1) attn_fwd_kernel<T_, DP_, 1, 32><<<blocks, 64, 0, st>>>(a);                               \
-  else if (a.row_waves == 2) attn_fwd_kernel<T_, DP_, 2, KT><<<blocks, 128, 0, st>>>(a);                         \
-  else attn_fwd_kernel<T_, DP_, 4, KT><<<blocks, 256, 0, st>>>(a)
+  if (a.row_waves == 4) attn_fwd_kernel<T_, DP_, 4, KT><<<blocks, 256, 0, st>>>(a);                              \
+  else if constexpr (SMALL_BLOCKS<T_, DP_>) {                                                                    \
+    if (a.row_waves == 1) attn_fwd_kernel<T_, DP_, 1, 32><<<blocks, 64, 0, st>>>(a);                             \
+    else attn_fwd_kernel<T_, DP_, 2, KT><<<blocks, 128, 0, st>>>(a);                                             \
+  }
   ATTN_DIM(T, a.D, ATTN_FWD);
 #undef ATTN_FWD
   join_launch<T>(a, st);
@@ -1730,9 +1750,11 @@ static void attn_bwd_launch(const Attn& a, hipStream_t st) {
   if (blocks) {
 #define ATTN_DQ(T_, DP_)                                                                                         \
   constexpr int KT = sizeof(T_) == 4 || DP_ > 64 ? 32 : 64;                                                      \
-  if (a.row_waves == 1) attn_dq_kernel<T_, DP_, 1, 32><<<blocks, 64, 0, st>>>(a);                                \
-  else if (a.row_waves == 2) attn_dq_kernel<T_, DP_, 2, KT><<<blocks, 128, 0, st>>>(a);                          \
-  else attn_dq_kernel<T_, DP_, 4, KT><<<blocks, 256, 0, st>>>(a)
+  if (a.row_waves == 4) attn_dq_kernel<T_, DP_, 4, KT><<<blocks, 256, 0, st>>>(a);                               \
+  else if constexpr (SMALL_BLOCKS<T_, DP_>) {                                                                    \
+    if (a.row_waves == 1) attn_dq_kernel<T_, DP_, 1, 32><<<blocks, 64, 0, st>>>(a);                              \
+    else attn_dq_kernel<T_, DP_, 2, KT><<<blocks, 128, 0, st>>>(a);                                              \
+  }
     ATTN_DIM(T, a.D, ATTN_DQ);
 #undef ATTN_DQ
     if (a.splits > 1) {
@@ -1745,9 +1767,11 @@ static void attn_bwd_launch(const Attn& a, hipStream_t st) {
   if (kblocks) {
 #define ATTN_DKV(T_, DP_)                                                                                        \
   constexpr int QB = sizeof(T_) == 2 && DP_ <= 32 ? 64 : 32, QB4 = DP_ <= 32 ? 64 : 32;                          \
-  if (a.key_waves == 1) attn_dkv_kernel<T_, DP_, 1, 32><<<kblocks, 64, 0, st>>>(a);                              \
-  else if (a.key_waves == 2) attn_dkv_kernel<T_, DP_, 2, QB><<<kblocks, 128, 0, st>>>(a);                        \
-  else attn_dkv_kernel<T_, DP_, 4, QB4><<<kblocks, 256, 0, st>>>(a)
+  if (a.key_waves == 4) attn_dkv_kernel<T_, DP_, 4, QB4><<<kblocks, 256, 0, st>>>(a);                            \
+  else if constexpr (SMALL_BLOCKS<T_, DP_>) {                                                                    \
+    if (a.key_waves == 1) attn_dkv_kernel<T_, DP_, 1, 32><<<kblocks, 64, 0, st>>>(a);                            \
+    else attn_dkv_kernel<T_, DP_, 2, QB><<<kblocks, 128, 0, st>>>(a);                                            \
+  }
     ATTN_DIM(T, a.D, ATTN_DKV);
 #undef ATTN_DKV
     if (a.row_splits > 1)

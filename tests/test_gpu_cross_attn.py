@@ -308,6 +308,17 @@ def test_padding_before_the_keys(dtype, Tq, Tk):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('D', [24, 32, 64, 72, 96, 128])
+@pytest.mark.parametrize('Tq,Tk', [(20, 70), (50, 30), (33, 64), (5, 33), (130, 20)])
+def test_many_pairs_of_few_strips(dtype, D, Tq, Tk):
+    """Enough (sample, key head) pairs for blocks of one and two waves, over rows, over keys and over both."""
+    B = 260
+    q, k, v, dout = _make(B, Tq, Tk, 8, 8, D, dtype)
+    sl = _lengths(B, Tk)
+    _check(_run(q, k, v, dout, sl), attention(q, k, v, sl, dout=dout))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('Tq', [1, 45])
 def test_time_before_batch(dtype, Tq):
     q, k, v, dout = (t.transpose(0, 1).contiguous().transpose(0, 1) for t in _make(3, Tq, 70, 4, 2, 64, dtype, seed=29))
