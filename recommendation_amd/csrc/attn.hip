@@ -18,7 +18,7 @@
 // reaches a result.  A row without keys gives zeros, lse = -inf and no gradient.  No float atomics: same bits every run.
 // Bound: matrix and vector instructions of a SIMD hardly overlap here (per wave, two to a SIMD: 4 products 63 ns, 32 fma
 // 38, 8 exp 31, all three 107), so the time of a tile is their sum.  16 heads of 2048 x 4096 of 64, batch 8, bf16: forward
-// 365 us, 750 TFLOP/s counting its two products; dq 600 us, dk / dv 660 us, 687 and 830 TFLOP/s counting three and four
+// 365 us, 750 TFLOP/s counting its two products; dq 635 us, dk / dv 660 us, 650 and 830 TFLOP/s counting three and four
 // (a large bf16 matrix product reaches 1200 on this card).
 #include "types.h"
 
@@ -405,7 +405,7 @@ constexpr int FWD_WAVES = NW == 4 && Terms<T>::NP == 1 && DP <= 64 ? 4 : WAVES<T
 // 97 for 123 and 137) - but not with single waves on keys of 128, which LDS then limits (4096 pairs of 500 rows and 30
 // keys: 304 us for 358).  Head size 64, dk / dv: with that operand in LDS and tiles of 32 rows three waves fit a SIMD (660 us
 // for the shape above, 710 with two), and in blocks of two waves fp16 spills no more (4096 pairs of 500 rows and 60 keys:
-// 199 us for 244; bf16 192 for 178).  dq gains nothing from it (600 either way).
+// 199 us for 244; bf16 192 for 178).  dq gains nothing from it.
 template <class T, int DP, int NW>
 constexpr int DKV_WAVES = NW == 4 && Terms<T>::NP == 1 && DP == 64 ? 3 : WAVES<T, DP>;
 template <class T, int DP, int NW>
@@ -634,9 +634,10 @@ __global__ __launch_bounds__(256) void attn_join_kernel(Attn a, int64_t n_rows) 
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------
-// fp16: keeps ds * factor below 2^15 with a power of two per lane that only ever shrinks; the accumulators follow it
+// fp16: keeps ds * factor below 2^15 with a power of two per lane that only ever shrinks; the accumulators and the sum
+// follow it
 template <int ND>
-__device__ static inline float fit_f16(const f32x16& ds, float factor, f32x16* acc) {
+__device__ static inline float fit_f16(const f32x16& ds, float factor, f32x16* acc, float& sum) {
   float top = 0.f;
 #pragma unroll
   for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(ds[r]));
@@ -646,12 +647,30 @@ __device__ static inline float fit_f16(const f32x16& ds, float factor, f32x16* a
     const float next = over ? ldexpf(1.f, 13 - ilogbf(fminf(top, 3.0e38f))) : factor;
     const float by = next / factor;
     factor = next;
+    sum *= by;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[d][r] *= by;
   }
   return factor;
+}
+// sum + the eight 16-bit values of an operand, in fp32
+template <class T>
+__device__ static inline float add_frag(const Frag<T>& f, float sum) {
+  const uint4 w = __builtin_bit_cast(uint4, f.t[0]);
+  const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (__is_same(T, f16_t)) {
+      const f16x2 one = {(f16_t)1.f, (f16_t)1.f};
+      sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, u[i]), one, sum, false);
+    } else {
+      const bf16x2 one = {(bf16_t)1.f, (bf16_t)1.f};
+      sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, u[i]), one, sum, false);
+    }
+  }
+  return sum;
 }
 constexpr float F16_FACTOR0 = 1.2676506e30f;           // 2^100: the first strip with a gradient sets the factor
 
@@ -660,7 +679,10 @@ constexpr float F16_FACTOR0 = 1.2676506e30f;           // 2^100: the first strip
 // For 16-bit tensors delta = sum_d dout out carries the rounding of out, the same error e for every key of a row: dq
 // would be off by e times the row's mean key, dk alike.  The sum of ds over all keys is exactly that error (it is zero
 // otherwise), so it is summed in fp32, put into delta for the dk / dv pass, and taken out of dq with the row's mean key
-// (KEYS: sum p k, a second product per strip over operands that are there already).
+// (KEYS: sum p k, a second product per strip over operands that are there already).  For dq it is the sum of the rounded
+// ds that is taken out: what their roundings have in common over the keys goes with it (8 rows against 14000 keys, bf16:
+// dq 0.26 % off instead of 0.27; 40 against 3: 0.21 instead of 0.25; 0.17 to 0.2 are the last rounding's; 635 us for
+// the shape above, 600 without).
 template <class T, int DP, int NW, int KT>
 __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dq_kernel(Attn a) {
   constexpr int NS = KT / 32, NK = DP / 16, ND = DP / 32, NBUF = NW > 1 ? 2 : 1;
@@ -729,7 +751,7 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dq_kernel(Attn a
   for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
 #pragma unroll
   for (int d = 0; d < (KEYS ? ND : 1); ++d) keys[d] = f32x16{};
-  float factor = F16 ? F16_FACTOR0 : 1.f, rest = 0.f;
+  float factor = F16 ? F16_FACTOR0 : 1.f, rest = 0.f, drop = 0.f;    // sums of ds and of the rounded ds * factor
 
   auto tile_work = [&](int buf, bool whole, int kb) {
     const uint64_t bits = whole ? 0 : key_bits(mask, kb, k1, KT);
@@ -750,7 +772,7 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dq_kernel(Attn a
         dp[e] = s[e] * (dp[e] - delta);
         if (KEYS) rest += dp[e];
       }
-      if constexpr (F16) factor = fit_f16<ND>(dp, factor, acc);
+      if constexpr (F16) factor = fit_f16<ND>(dp, factor, acc, drop);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float f[8], e[8];
@@ -761,7 +783,10 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dq_kernel(Attn a
         }
         const Frag<T> df = make_frag<T>(f);
         Frag<T> pf;
-        if constexpr (KEYS) pf = make_frag<T>(e);
+        if constexpr (KEYS) {
+          pf = make_frag<T>(e);
+          drop = add_frag<T>(df, drop);
+        }
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
           const Frag<T> kf = kt[buf].cols(i * 32 + c * 16, d * 32);
@@ -799,8 +824,9 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dq_kernel(Attn a
   }
   constexpr float unbias = 1.f / (1 << (int)Terms<T>::BIAS);
   rest = half_swap_sum(rest, rest) * unbias;
+  drop = half_swap_sum(drop, drop) * (unbias / factor);
   if (lone_key(a, b)) {
-    rest = 0.f;
+    rest = drop = 0.f;
 #pragma unroll
     for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
   }
@@ -815,10 +841,10 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dq_kernel(Attn a
     for (int d = 0; d < ND; ++d) {
       if constexpr (KEYS)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[d][e] = acc[d][e] * (unbias / factor) - rest * (keys[d][e] * unbias);
+        for (int e = 0; e < 16; ++e) acc[d][e] = acc[d][e] * (unbias / factor) - drop * (keys[d][e] * unbias);
       store_strip<T>(dst, d * 32, a.D, acc[d], a.scale);
     }
-  } else {                                             // sum ds k, then sum p k, then sum ds; the join follows
+  } else {                                             // sum ds k, then sum p k; both sums of ds; the join follows
     const int64_t n_rows = (int64_t)a.B * a.Hkv * a.rows;
     float* dst = a.part + ((int64_t)split * n_rows + rid) * (KEYS ? 2 * a.D : a.D);
 #pragma unroll
@@ -827,7 +853,8 @@ __global__ __launch_bounds__(NW * 64, (WAVES<T, DP>)) void attn_dq_kernel(Attn a
       if constexpr (KEYS) store_strip<float>(dst + a.D, d * 32, a.D, keys[d], unbias);
     }
     if (lane < 32) {
-      if constexpr (KEYS) a.part_lse[(int64_t)split * n_rows + rid] = rest;
+      if constexpr (KEYS)
+        *reinterpret_cast<float2*>(a.part_lse + 2 * ((int64_t)split * n_rows + rid)) = make_float2(rest, drop);
       if (split == 0) a.delta[rid] = delta;
     }
   }
@@ -857,7 +884,7 @@ __global__ __launch_bounds__(NW * 64, (DKV_WAVES<T, DP, NW>)) void attn_dkv_kern
   f32x16 dk[ND], dv[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{};
-  float factor = F16 ? F16_FACTOR0 : 1.f;
+  float factor = F16 ? F16_FACTOR0 : 1.f, none = 0.f;
   if (key0 < len && row0 < row1) {
     Stage<T, QB, DP, NW * 64> nq, ng;
     nq.list_init(a, a.q);
@@ -931,7 +958,7 @@ __global__ __launch_bounds__(NW * 64, (DKV_WAVES<T, DP, NW>)) void attn_dkv_kern
             dp[4 * g + j] = ds;
           }
         }
-        if constexpr (F16) factor = fit_f16<ND>(dp, factor, dk);
+        if constexpr (F16) factor = fit_f16<ND>(dp, factor, dk, none);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float f[8], e[8];
@@ -1021,7 +1048,7 @@ __global__ __launch_bounds__(256) void attn_key_sum_kernel(Attn a) {
 template <class T, bool WIDE>
 __global__ __launch_bounds__(256) void attn_sum_kernel(Attn a, int64_t n_rows) {
   constexpr bool KEYS = Terms<T>::NP == 1;
-  constexpr int N = KEYS ? 9 : 4;                      // four columns of sum ds k, of sum p k, and sum ds
+  constexpr int N = KEYS ? 10 : 4;                     // four columns of sum ds k, of sum p k, sum ds, sum of the rounded
   const int quads = a.D / 4, width = KEYS ? 2 * a.D : a.D;
   int64_t rid;
   int quad, first = 0, every = 1;
@@ -1055,7 +1082,9 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(Attn a, int64_t n_rows) {
         acc[5] += k.y;
         acc[6] += k.z;
         acc[7] += k.w;
-        acc[8] += a.part_lse[i * n_rows + rid];
+        const float2 both = *reinterpret_cast<const float2*>(a.part_lse + 2 * (i * n_rows + rid));
+        acc[8] += both.x;
+        acc[9] += both.y;
       }
     }
   if constexpr (WIDE) {
@@ -1068,7 +1097,7 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(Attn a, int64_t n_rows) {
 #pragma unroll
       for (int j = 0; j < N; ++j) acc[j] += red[g][quad][j];
   }
-  if (KEYS && d == 0) a.delta[rid] += acc[N - 1];
+  if (KEYS && d == 0) a.delta[rid] += acc[N - 2];
   T* dst = row_of<T>(a, a.dq, rid) + d;
 #pragma unroll
   for (int j = 0; j < 4; ++j) dst[j] = (T)(a.scale * (KEYS ? acc[j] - acc[N - 1] * acc[KEYS ? 4 + j : 0] : acc[j]));
@@ -1592,7 +1621,7 @@ static size_t bwd_ws_first(const Attn& a) {
 }
 static size_t bwd_ws(const Attn& a) {
   if (a.few) return rows_fused(a) ? 256 : bwd_ws_first(a) + (size_t)a.B * a.Hkv * a.Tk * a.few * 8 + 256;
-  const size_t rows = a.splits > 1 ? (size_t)a.splits * total_rows(a) * (2 * a.D + 1) * 4 : 0;
+  const size_t rows = a.splits > 1 ? (size_t)a.splits * total_rows(a) * (2 * a.D + 2) * 4 : 0;
   const size_t keys = a.row_splits > 1 ? (size_t)a.row_splits * a.B * a.Hkv * a.Tk * 2 * a.D * 4 : 0;
   return bwd_ws_first(a) + (rows > keys ? rows : keys) + 256;           // one after the other
 }
