@@ -182,7 +182,7 @@ struct Attn {
   float scale, scale2;                                 // scale2 = scale * log2(e)
   int rows, row_tiles, key_tiles, splits, per_split;
   int row_waves, key_waves, row_splits, rows_per;      // waves per block; splits of the row list in the dk / dv pass
-  float *part, *part_lse;                              // [splits][B H Tq][D], [splits][B H Tq]
+  float *part, *part_lse;                              // forward: [splits][B H Tq][D], [splits][B H Tq]; dq: attn_dq_kernel
   float* kept;                                         // few rows: p, then dp, [B Hkv][Tk][R]
   bool near;                                           // a tile's rows lie within 2^31 bytes of its first
   int few, waves, lanes;                               // rows padded to 1, 2 or 4 (0: the tiled kernels); waves per
