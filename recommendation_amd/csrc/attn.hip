@@ -1308,7 +1308,8 @@ __global__ __launch_bounds__(256) void attn_rows_fwd_kernel(Attn a) {
 }
 
 // dk and dv of the keys [k0, k1) of a pair, KPW keys per wave and step; kept: p and dp of key k, row r at
-// kept[(k - from) * R + r] and `apart` floats behind
+// kept[(k - from) * R + r] and `apart` floats behind.  A key that is left out carries p = -1: its zeros do not depend on
+// what q and dout hold (0 * infinity).
 template <class T, int R, int LPK>
 __device__ static inline void rows_write_kv(const Attn& a, int b, int hk, int k0, int k1, int live, int from,
                                             const float* kept, int64_t apart, const float (&q)[R][Packet<T>::V],
@@ -1326,6 +1327,7 @@ __device__ static inline void rows_write_kv(const Attn& a, int b, int hk, int k0
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const float p = kept[(int64_t)(key - from) * R + r], dp = kept[apart + (int64_t)(key - from) * R + r];
+        if (p < 0.f) continue;
         const float ds = p == 0.f || lone ? 0.f : p * (dp - delta[r]) * a.scale;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -1414,7 +1416,7 @@ __global__ __launch_bounds__(256) void attn_rows_bwd_kernel(Attn a) {
           S[r][j] = fmaf(p, f[j], S[r][j]);
         }
         if (sub == 0 && key < pa.k1) {
-          kept[(int64_t)(key - pa.k0) * R + r] = p;
+          kept[(int64_t)(key - pa.k0) * R + r] = ok[u] ? p : -1.f;
           kept[apart + (int64_t)(key - pa.k0) * R + r] = dp;
         }
       }
