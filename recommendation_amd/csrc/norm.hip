@@ -1,5 +1,8 @@
 // Layer norm over the last axis of a [rows, cols] view, forward and backward.
 //   mean = sum x / n,  var = sum (x - mean)^2 / n,  rstd = 1 / sqrt(var + eps),  xh = (x - mean) rstd
+// The mean's own rounding would be a common offset of its row, large beside a spread that is small against the mean, so
+// the second pass sums the residuals d = x - mean too: c = sum d / n is what the mean is off by, and is taken out of
+// it, of d and of the variance (sum d^2 / n - c^2).
 //   y = xh gamma + beta
 //   g = dy gamma;  dx = rstd (g - sum g / n - xh sum(g xh) / n);  dgamma = sum_rows dy xh;  dbeta = sum_rows dy
 // Memory bound: the forward reads x and writes y once, the backward reads x and dy and writes dx once.  A row lives in
@@ -36,6 +39,42 @@ __device__ static inline float row_sum(float v, float* red) {
     return s;
   }
 }
+// two sums behind one barrier; red: one array for each
+template <int LPR>
+__device__ static inline float2 row_sum2(float v, float w, float (*red)[16]) {
+  if constexpr (LPR <= 64) {
+    return make_float2(group_sum<LPR>(v), group_sum<LPR>(w));
+  } else {
+    constexpr int W = LPR / 64;
+    v = wave_sum(v);
+    w = wave_sum(w);
+    const int wave = threadIdx.x >> 6, first = wave / W * W;
+    if ((threadIdx.x & 63) == 0) {
+      red[0][wave] = v;
+      red[1][wave] = w;
+    }
+    __syncthreads();
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      s.x += red[0][first + i];
+      s.y += red[1][first + i];
+    }
+    return s;
+  }
+}
+// sum / n as one rounded number: left to itself the compiler fuses the product into the subtraction from some entries of
+// the row and not from others, and equal entries differ
+__device__ static inline float row_mean(float sum, float inv_n) {
+#pragma clang fp contract(off)
+  return sum * inv_n;
+}
+// What the residuals d of a row around `mean` say: mean corrected, rstd, and what is left to take out of d
+struct RowStat { float mean, rstd, c; };
+__device__ static inline RowStat row_stat(float mean, float sum_d, float sum_d2, float inv_n, float eps) {
+  const float c = row_mean(sum_d, inv_n);
+  return {mean + c, 1.f / sqrtf(fmaxf(sum_d2 * inv_n - c * c, 0.f) + eps), c};
+}
 // a packet on its way: whole ones as they lie, the one at the end of a row element by element
 template <class T>
 __device__ static inline uint4 fetch_packet(const T* p, int have) {
@@ -68,7 +107,7 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_kernel(const T* x, int64_t x_l
                                                          const float* __restrict__ beta, float eps, T* y, int64_t y_ld,
                                                          float* __restrict__ mean_out, float* __restrict__ rstd_out) {
   constexpr int V = Packet<T>::V, GPB = THREADS / LPR;
-  __shared__ float red[2][THREADS / 64];
+  __shared__ float red[3][16];
   const int l = threadIdx.x % LPR, group = threadIdx.x / LPR;
   const float inv_n = 1.f / (float)cols;
   float ga[NV][V], be[NV][V];
@@ -100,21 +139,21 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_kernel(const T* x, int64_t x_l
       for (int j = 0; j < V; ++j) s += v[i][j];
     }
     if (base + step < rows) fetch(row + step);
-    const float mean = row_sum<LPR>(s, red[0]) * inv_n;
-    float q = 0.f;
+    const float mean = row_mean(row_sum<LPR>(s, red[0]), inv_n);
+    float q = 0.f, r = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (have[i] == V) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) { v[i][j] -= mean; q = fmaf(v[i][j], v[i][j], q); }
+        for (int j = 0; j < V; ++j) { v[i][j] -= mean; r += v[i][j]; q = fmaf(v[i][j], v[i][j], q); }
       } else {
 #pragma unroll
         for (int j = 0; j < V; ++j)
-          if (j < have[i]) { v[i][j] -= mean; q = fmaf(v[i][j], v[i][j], q); }
+          if (j < have[i]) { v[i][j] -= mean; r += v[i][j]; q = fmaf(v[i][j], v[i][j], q); }
       }
     }
-    const float var = row_sum<LPR>(q, red[1]) * inv_n;
-    const float rstd = 1.f / sqrtf(var + eps);
+    const float2 sums = row_sum2<LPR>(r, q, red + 1);
+    const RowStat st = row_stat(mean, sums.x, sums.y, inv_n, eps);
     if (active) {
       T* yr = y + row * y_ld;
 #pragma unroll
@@ -122,13 +161,13 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_kernel(const T* x, int64_t x_l
         const int c = (l + i * LPR) * V;
         float o[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = fmaf(v[i][j] * rstd, ga[i][j], be[i][j]);
+        for (int j = 0; j < V; ++j) o[j] = fmaf((v[i][j] - st.c) * st.rstd, ga[i][j], be[i][j]);
         if (have[i] == V) packet_store(yr + c, Packet<T>::pack(o));
         else store_part(yr + c, have[i], o);
       }
       if (l == 0) {
-        if (mean_out) mean_out[row] = mean;
-        if (rstd_out) rstd_out[row] = rstd;
+        if (mean_out) mean_out[row] = st.mean;
+        if (rstd_out) rstd_out[row] = st.rstd;
       }
     }
   }
@@ -285,36 +324,40 @@ __global__ __launch_bounds__(1024) void ln_fwd_wide_kernel(const T* x, int64_t x
                                                            int64_t y_ld, float* __restrict__ mean_out,
                                                            float* __restrict__ rstd_out) {
   constexpr int V = Packet<T>::V, STEP = 1024 * V;
-  __shared__ float red[2][16];
+  __shared__ float red[3][16];
   const float inv_n = 1.f / (float)cols;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* xr = x + row * x_ld;
     T* yr = y + row * y_ld;
-    float f[V], s = 0.f, q = 0.f;
+    float f[V], s = 0.f, q = 0.f, r = 0.f;
     for (int c = threadIdx.x * V; c < cols; c += STEP) {
       wide_load(xr, c, cols, 0.f, f);
 #pragma unroll
       for (int j = 0; j < V; ++j) s += f[j];
     }
-    const float mean = row_sum<1024>(s, red[0]) * inv_n;
+    const float mean = row_mean(row_sum<1024>(s, red[0]), inv_n);
     for (int c = threadIdx.x * V; c < cols; c += STEP) {
       wide_load(xr, c, cols, mean, f);
 #pragma unroll
-      for (int j = 0; j < V; ++j) q = fmaf(f[j] - mean, f[j] - mean, q);
+      for (int j = 0; j < V; ++j) {
+        r += f[j] - mean;
+        q = fmaf(f[j] - mean, f[j] - mean, q);
+      }
     }
-    const float rstd = 1.f / sqrtf(row_sum<1024>(q, red[1]) * inv_n + eps);
+    const float2 sums = row_sum2<1024>(r, q, red + 1);
+    const RowStat st = row_stat(mean, sums.x, sums.y, inv_n, eps);
     for (int c = threadIdx.x * V; c < cols; c += STEP) {
       wide_load(xr, c, cols, 0.f, f);
       const int n = min(V, cols - c);
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        if (j < n) f[j] = fmaf((f[j] - mean) * rstd, gamma ? gamma[c + j] : 1.f, beta ? beta[c + j] : 0.f);
+        if (j < n) f[j] = fmaf((f[j] - mean - st.c) * st.rstd, gamma ? gamma[c + j] : 1.f, beta ? beta[c + j] : 0.f);
       if (n == V) packet_store(yr + c, Packet<T>::pack(f));
       else store_part(yr + c, n, f);
     }
     if (threadIdx.x == 0) {
-      if (mean_out) mean_out[row] = mean;
-      if (rstd_out) rstd_out[row] = rstd;
+      if (mean_out) mean_out[row] = st.mean;
+      if (rstd_out) rstd_out[row] = st.rstd;
     }
   }
 }
