@@ -1230,7 +1230,7 @@ def _here(names, *tensors):
 
 
 def _heads(t, shape, dtype, name):
-    """ctr_heads_t of a [B, T, heads, D] view (the stride of an axis of one plays no part)."""
+    """(ctr_heads_t, span) of a [B, T, heads, D] view (the stride of an axis of one plays no part)."""
     if t.shape != shape:
         raise ValueError('%s must be %s, got %s' % (name, list(shape), list(t.shape)))
     if t.dtype != dtype:
@@ -1238,11 +1238,15 @@ def _heads(t, shape, dtype, name):
     sb, st, sh, sd = t.stride()
     if sd != 1:
         raise ValueError('%s must have a contiguous last dimension' % name)
-    return _lib.HEADS.pack(t.data_ptr(), sb if shape[0] > 1 else 0, st if shape[1] > 1 else 0, sh if shape[2] > 1 else 0)
+    B, T, H, D = shape
+    p = t.data_ptr()
+    sb, st, sh = sb if B > 1 else 0, st if T > 1 else 0, sh if H > 1 else 0
+    end = p + ((B - 1) * sb + (T - 1) * st + (H - 1) * sh + D) * (4 if dtype is torch.float32 else 2) if B and T else 0
+    return _lib.HEADS.pack(p, sb, st, sh), (p if end else 0, end, t, name)
 
 
 def _attn_args(q, k, sl, mask, scale):
-    """(ctr_attn_t, q's shape, k's shape) of a cross-attention call, checked."""
+    """(ctr_attn_t, q's shape, k's shape, spans of sl and mask) of a cross-attention call, checked."""
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError('q must be [B, Tq, H, D] and k [B, Tk, Hkv, D]')
     qs, ks = q.shape, k.shape
@@ -1258,35 +1262,94 @@ def _attn_args(q, k, sl, mask, scale):
     if not 1e-30 <= scale <= 1e30:
         raise ValueError('scale must lie between 1e-30 and 1e30')
     mp = mld = sp = 0
+    spans = ()
     if mask is not None:
         if mask.dtype not in (torch.bool, torch.uint8):
             raise TypeError('mask: expected bool or uint8, got %s' % mask.dtype)
         if mask.shape != (B, Tk) or (Tk > 1 and mask.stride(1) != 1):
             raise ValueError('mask must be [B, Tk] with a contiguous last dimension')
         mp, mld = mask.data_ptr(), mask.stride(0) if B > 1 else 0
+        if B and Tk:
+            spans = ((mp, mp + (B - 1) * mld + Tk, mask, 'mask'),)
     if sl is not None:
         if sl.dtype != torch.int32 or sl.shape != (B,) or not sl.is_contiguous():
             raise ValueError('sl must be a contiguous int32 [B] tensor')
         sp = sl.data_ptr()
-    return _lib.ATTN.pack(B, Tq, Tk, H, Hkv, D, _dtype(q, 'q'), scale, sp, mp, mld), qs, ks
+        if B:
+            spans += ((sp, sp + 4 * B, sl, 'sl'),)
+    return _lib.ATTN.pack(B, Tq, Tk, H, Hkv, D, _dtype(q, 'q'), scale, sp, mp, mld), qs, ks, spans
 
 
 def _lse(lse, qs):
+    """(address, span)"""
     if lse.dtype != torch.float32 or lse.shape != (qs[0], qs[2], qs[1]) or not lse.is_contiguous():
         raise ValueError('lse must be contiguous float32 [B, H, Tq]')
-    return lse.data_ptr()
+    p = lse.data_ptr()
+    end = p + 4 * lse.numel()
+    return p, (p if end > p else 0, end if end > p else 0, lse, 'lse')
 
 
-def _apart(names, outs, ins):
-    """No output starts where another tensor of the call does (views that merely share a buffer are fine)."""
-    seen = [t.data_ptr() for t in outs + ins if t.numel()]
-    if len(set(seen[:len(outs)])) == len(outs) and not set(seen[:len(outs)]) & set(seen[len(outs):]):
-        return
-    ptrs = [(t.data_ptr() if t.numel() else None) for t in outs + ins]
-    for i in range(len(outs)):
-        for j in range(len(ptrs)):
-            if j != i and ptrs[i] is not None and ptrs[i] == ptrs[j]:
-                raise ValueError('%s shares its memory with %s' % (names.split()[i], names.split()[j]))
+def _runs(t):
+    """(bytes of a contiguous run of t, [(runs, bytes apart)] of its other axes)."""
+    size = run = t.element_size()
+    axes = []
+    for stride, n in sorted(zip(t.stride(), t.shape)):
+        if n == 1 or stride == 0:
+            continue
+        if not axes and stride * size == run:
+            run *= n
+        else:
+            axes.append((n, stride * size))
+    return run, axes
+
+
+def _share(a, b):
+    """Whether two tensors of strides >= 0 have a byte in common: whether run i of a and run j of b meet for some indices,
+    searched from the widest stride down (axes of one stride together, by the difference of their indices).  Views of the
+    same strides, such as the parts of a packed projection, take a step or two per axis; a search that takes more than
+    2000 (views of one buffer with strides of their own) counts as a meeting."""
+    ra, axes_a = _runs(a)
+    rb, axes_b = _runs(b)
+    ends = {}                                          # stride -> (least, greatest) difference of the indices
+    for n, s in axes_a:
+        lo, hi = ends.get(s, (0, 0))
+        ends[s] = (lo, hi + n - 1)
+    for n, s in axes_b:
+        lo, hi = ends.get(s, (0, 0))
+        ends[s] = (lo - n + 1, hi)
+    axes = sorted(((s, lo, hi) for s, (lo, hi) in ends.items()), reverse=True)
+    below = [(0, 0)]                                   # what the axes behind each one can still add
+    for s, lo, hi in reversed(axes):
+        below.append((below[-1][0] + s * lo, below[-1][1] + s * hi))
+    below.reverse()
+    steps = 0
+    todo = [(0, a.data_ptr() - b.data_ptr())]          # a's run begins `at` behind b's: they meet where -ra < at < rb
+    while todo:
+        i, at = todo.pop()
+        steps += 1
+        if i == len(axes):
+            if -ra < at < rb:
+                return True
+            continue
+        if steps > 2000:
+            return True
+        s, lo, hi = axes[i]
+        least, most = below[i + 1]
+        first, last = max(lo, -((at + most + ra - 1) // s)), min(hi, (rb - 1 - at - least) // s)
+        todo.extend((i + 1, at + d * s) for d in range(first, min(last, first + 2000) + 1))
+    return False
+
+
+def _apart(outs, ins):
+    """outs are written: none of them may share memory with another tensor of the call.  (begin, end, tensor, name) each;
+    the spans settle nearly every call."""
+    for i, (b0, e0, t0, name) in enumerate(outs):
+        for b1, e1, t1, other in ins:
+            if b0 < e1 and b1 < e0 and _share(t0, t1):
+                raise ValueError('%s shares its memory with %s' % (name, other))
+        for b1, e1, t1, other in outs[i + 1:]:
+            if b0 < e1 and b1 < e0 and _share(t0, t1):
+                raise ValueError('%s shares its memory with %s' % (name, other))
 
 
 @_timed
@@ -1295,12 +1358,13 @@ def cross_attn_fwd(q, k, v, out, *, lse=None, sl=None, mask=None, scale=None, ws
     states of another sequence.  q, out [B,Tq,H,D], k, v [B,Tk,Hkv,D] in float32, bfloat16 or float16 (D a multiple of 8
     up to 128, rows on 16-byte boundaries, other strides free).  sl (int32 [B]): only the first sl[b] keys; mask (bool or
     uint8 [B,Tk]): only the keys that are set.  A row without keys gives zeros.  scale: 1 / sqrt(D) by default.
-    lse (float32 [B,H,Tq]): the logarithm of every softmax's sum, kept for cross_attn_bwd."""
-    sh, qs, ks = _attn_args(q, k, sl, mask, scale)
+    lse (float32 [B,H,Tq]): the logarithm of every softmax's sum, kept for cross_attn_bwd.  out and lse share no memory
+    with each other or an input (views that interleave in one buffer are apart)."""
+    sh, qs, ks, keys = _attn_args(q, k, sl, mask, scale)
     t = q.dtype
-    hq, hk, hv, ho = _heads(q, qs, t, 'q'), _heads(k, ks, t, 'k'), _heads(v, ks, t, 'v'), _heads(out, qs, t, 'out')
-    lp = None if lse is None else _lse(lse, qs)
-    _apart('out q k v', (out,), (q, k, v))
+    (hq, mq), (hk, mk), (hv, mv), (ho, mo) = _heads(q, qs, t, 'q'), _heads(k, ks, t, 'k'), _heads(v, ks, t, 'v'), _heads(out, qs, t, 'out')
+    lp, ml = (None, None) if lse is None else _lse(lse, qs)
+    _apart((mo,) if ml is None else (mo, ml), (mq, mk, mv) + keys)
     stream = _here('q k v out lse sl mask', q, k, v, out, lse, sl, mask)
     L = lib()
     wp, wn = ws.get(L.ctr_cross_attn_fwd_workspace_bytes(sh))
@@ -1310,13 +1374,14 @@ def cross_attn_fwd(q, k, v, out, *, lse=None, sl=None, mask=None, scale=None, ws
 @_timed
 def cross_attn_bwd(dout, q, k, v, out, lse, dq, dk, dv, *, sl=None, mask=None, scale=None, ws):
     """Gradients of cross_attn_fwd from its own inputs, out and lse (the same sl, mask and scale).  dq, dk and dv are
-    overwritten; keys that no row attends to get zeros; heads that share keys add up in dk and dv."""
-    sh, qs, ks = _attn_args(q, k, sl, mask, scale)
+    overwritten; keys that no row attends to get zeros; heads that share keys add up in dk and dv.  They share no memory
+    with each other or an input (the parts of one packed gradient are apart)."""
+    sh, qs, ks, keys = _attn_args(q, k, sl, mask, scale)
     t = q.dtype
-    hg, hq, hk, hv = _heads(dout, qs, t, 'dout'), _heads(q, qs, t, 'q'), _heads(k, ks, t, 'k'), _heads(v, ks, t, 'v')
-    ho, gq, gk, gv = _heads(out, qs, t, 'out'), _heads(dq, qs, t, 'dq'), _heads(dk, ks, t, 'dk'), _heads(dv, ks, t, 'dv')
-    lp = _lse(lse, qs)
-    _apart('dq dk dv dout q k v out', (dq, dk, dv), (dout, q, k, v, out))
+    (hg, mg), (hq, mq), (hk, mk), (hv, mv) = _heads(dout, qs, t, 'dout'), _heads(q, qs, t, 'q'), _heads(k, ks, t, 'k'), _heads(v, ks, t, 'v')
+    (ho, mo), (gq, nq), (gk, nk), (gv, nv) = _heads(out, qs, t, 'out'), _heads(dq, qs, t, 'dq'), _heads(dk, ks, t, 'dk'), _heads(dv, ks, t, 'dv')
+    lp, ml = _lse(lse, qs)
+    _apart((nq, nk, nv), (mg, mq, mk, mv, mo, ml) + keys)
     stream = _here('dout q k v out lse dq dk dv sl mask', dout, q, k, v, out, lse, dq, dk, dv, sl, mask)
     L = lib()
     wp, wn = ws.get(L.ctr_cross_attn_bwd_workspace_bytes(sh))

@@ -1,0 +1,139 @@
+"""Outputs of cross attention that share memory with another tensor of the call are refused, views that only interleave in
+one buffer are not (CPU tensors: a call that is well formed ends at the check of the device)."""
+import random
+
+import pytest
+import torch
+
+from recommendation_amd import ops
+
+
+class Ws:
+    def get(self, n):
+        return None, 0
+
+
+def _elements(t):
+    at = torch.tensor([t.storage_offset()])
+    for n, stride in zip(t.shape, t.stride()):
+        at = (at[:, None] + torch.arange(n)[None] * stride).reshape(-1)
+    return set(at.tolist())
+
+
+@pytest.mark.parametrize('seed', range(8))
+def test_share_is_exact(seed):
+    """Against the sets of elements, over views of any strides (overlapping and broadcast ones too)."""
+    rng = random.Random(seed)
+    buf = torch.zeros(4096)
+
+    def view():
+        shape = [rng.randint(1, 4) for _ in range(3)] + [rng.choice([1, 2, 4, 8])]
+        strides = [rng.choice([0, 4, 8, 12, 16, 24, 32, 48, 64, 96, 128, 200]) for _ in range(3)] + [1]
+        return torch.as_strided(buf, shape, strides, rng.choice([0, 4, 8, 16, 32, 64, 100, 300]))
+
+    seen = set()
+    for _ in range(400):
+        a, b = view(), view()
+        want = bool(_elements(a) & _elements(b))
+        assert ops._share(a, b) == want, (a.shape, a.stride(), a.storage_offset(), b.shape, b.stride(), b.storage_offset())
+        seen.add(want)
+    assert seen == {True, False}
+
+
+def test_share_of_other_types_and_of_no_elements():
+    raw = torch.zeros(1024, dtype=torch.uint8)
+    a = raw[:64].view(torch.float32)
+    assert ops._share(a, raw[63:70]) and not ops._share(a, raw[64:70]) and ops._share(raw[60:62].view(torch.bfloat16), a)
+
+
+def _t(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+B, TQ, TK, H, HKV, D = 3, 6, 5, 4, 2, 16
+
+
+def _fwd(**kw):
+    a = dict(q=_t(B, TQ, H, D), k=_t(B, TK, HKV, D), v=_t(B, TK, HKV, D), out=_t(B, TQ, H, D))
+    a.update(kw)
+    ops.cross_attn_fwd(**a, ws=Ws())
+
+
+def _bwd(**kw):
+    a = dict(dout=_t(B, TQ, H, D), q=_t(B, TQ, H, D), k=_t(B, TK, HKV, D), v=_t(B, TK, HKV, D), out=_t(B, TQ, H, D),
+             lse=_t(B, H, TQ), dq=_t(B, TQ, H, D), dk=_t(B, TK, HKV, D), dv=_t(B, TK, HKV, D))
+    a.update(kw)
+    ops.cross_attn_bwd(**a, ws=Ws())
+
+
+def _shifted(shape, by):
+    """Two tensors of `shape` in one buffer, the second `by` elements behind the first."""
+    n = 1
+    for s in shape:
+        n *= s
+    buf = _t(n + by)
+    return buf[:n].view(shape), buf[by:].view(shape)
+
+
+def test_forward_refuses_shifted_outputs():
+    for by in (0, 4, 64, B * TQ * H * D - 4):
+        for a, b in (_shifted((B, TQ, H, D), by), _shifted((B, TQ, H, D), by)[::-1]):
+            with pytest.raises(ValueError, match='out shares its memory with q'):
+                _fwd(q=a, out=b)
+    wide = _t(B, TK + 1, HKV, D)
+    with pytest.raises(ValueError, match='out shares its memory with v'):
+        ops.cross_attn_fwd(_t(B, TK, HKV, D), _t(B, TK, HKV, D), wide[:, :TK], wide[:, 1:], ws=Ws())
+    buf = _t(B * H * TQ + B * TQ * H * D)
+    lse, out = buf[:B * H * TQ].view(B, H, TQ), buf[B * H * TQ - 4:-4].view(B, TQ, H, D)
+    with pytest.raises(ValueError, match='out shares its memory with lse'):
+        _fwd(lse=lse, out=out)
+    with pytest.raises(ValueError, match='lse shares its memory with q'):
+        _fwd(lse=lse, q=out)
+    rows = _t(B * TQ * H * D)
+    with pytest.raises(ValueError, match='out shares its memory with mask'):
+        _fwd(out=rows.view(B, TQ, H, D), mask=rows.view(torch.uint8)[64:64 + B * TK].view(B, TK))
+    with pytest.raises(ValueError, match='out shares its memory with sl'):
+        _fwd(out=rows.view(B, TQ, H, D), sl=rows.view(torch.int32)[-B:])
+
+
+def test_backward_refuses_shifted_gradients():
+    buf = _t(B, TK + 1, HKV, D)
+    with pytest.raises(ValueError, match='dk shares its memory with dv'):
+        _bwd(dk=buf[:, :TK], dv=buf[:, 1:])
+    for name in ('dout', 'q', 'out'):
+        a, b = _shifted((B, TQ, H, D), 64)
+        with pytest.raises(ValueError, match='dq shares its memory with ' + name):
+            _bwd(**{'dq': b, name: a})
+    for name in ('k', 'v'):
+        a, b = _shifted((B, TK, HKV, D), 4)
+        with pytest.raises(ValueError, match='dk shares its memory with ' + name):
+            _bwd(**{'dk': a, name: b})
+    rows = _t(B * TQ * H * D)
+    with pytest.raises(ValueError, match='dq shares its memory with lse'):
+        _bwd(dq=rows.view(B, TQ, H, D), lse=rows[-B * H * TQ:].view(B, H, TQ))
+
+
+def test_views_that_interleave_are_taken():
+    """Parts of a packed projection and of its gradient, columns of a wider buffer, neighbours in one arena."""
+    pack = lambda T: _t(B, T, H + 2 * HKV, D).split([H, HKV, HKV], dim=2)
+    (q, k, v), (dq, dk, dv) = pack(TK), pack(TK)
+    both = _t(B, TK, H, 2 * D)
+    out, dout = both[..., :D], both[..., D:]
+    lse = _t(B, H, TK)
+    with pytest.raises(ValueError, match='must live on the GPU'):
+        ops.cross_attn_fwd(q, k, v, out, lse=lse, ws=Ws())
+    with pytest.raises(ValueError, match='must live on the GPU'):
+        ops.cross_attn_bwd(dout, q, k, v, out, lse, dq, dk, dv, ws=Ws())
+    kv = _t(2, B, TK, HKV, D).permute(1, 2, 0, 3, 4)
+    with pytest.raises(ValueError, match='must live on the GPU'):
+        _bwd(dk=kv[:, :, 0], dv=kv[:, :, 1])
+    time_first = _t(TK, B, 2, HKV, D).transpose(0, 1)
+    with pytest.raises(ValueError, match='must live on the GPU'):
+        _bwd(dk=time_first[:, :, 0], dv=time_first[:, :, 1])
+    arena = _t(4 * B * TQ * H * D)
+    parts = [arena[i * B * TQ * H * D:(i + 1) * B * TQ * H * D].view(B, TQ, H, D) for i in range(4)]
+    with pytest.raises(ValueError, match='must live on the GPU'):
+        _bwd(dout=parts[0], q=parts[1], out=parts[2], dq=parts[3])
+    shared = _t(1, TQ, H, D).expand(B, TQ, H, D)                       # inputs may be one another
+    with pytest.raises(ValueError, match='must live on the GPU'):
+        _bwd(dout=shared, q=shared, out=shared)
