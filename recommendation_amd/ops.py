@@ -1389,7 +1389,7 @@ def cross_attn_bwd(dout, q, k, v, out, lse, dq, dk, dv, *, sl=None, mask=None, s
 
 
 def _ln_rows(t, shape, dtype, name):
-    """(address, leading dimension)"""
+    """(address, leading dimension, span)"""
     if t.shape != shape:
         raise ValueError('%s must be %s, got %s' % (name, list(shape), list(t.shape)))
     if t.dtype != dtype:
@@ -1398,17 +1398,23 @@ def _ln_rows(t, shape, dtype, name):
     rows, cols = shape
     if (one != 1 and cols > 1) or (rows > 1 and ld < cols):
         raise ValueError('%s must have a contiguous last dimension and rows that do not overlap' % name)
-    return t.data_ptr(), ld if rows > 1 else cols
+    p, ld = t.data_ptr(), ld if rows > 1 else cols
+    end = p + ((rows - 1) * ld + cols) * (4 if dtype is torch.float32 else 2) if rows else 0
+    return p, ld, (p if end else 0, end, t, name)
 
 
-def _ln_vec(t, n, name):
+def _ln_vec(t, n, name, spans):
+    """address; its span goes to `spans`"""
     if t is None:
         return None
     if t.dtype != torch.float32:
         raise TypeError('%s: expected torch.float32, got %s' % (name, t.dtype))
     if t.numel() != n or not t.is_contiguous():
         raise ValueError('%s must be contiguous with %d entries' % (name, n))
-    return t.data_ptr()
+    p = t.data_ptr()
+    if n:
+        spans.append((p, p + 4 * n, t, name))
+    return p
 
 
 def _ln_shape(x):
@@ -1420,14 +1426,19 @@ def _ln_shape(x):
 @_timed
 def layer_norm_fwd(x, y, *, gamma=None, beta=None, eps=1e-5, mean=None, rstd=None):
     """y = (x - mean) rstd gamma + beta over the columns of x [rows, cols] (float32, bfloat16 or float16; any row
-    stride).  gamma, beta: float32 [cols] or None; mean, rstd: float32 [rows], kept for layer_norm_bwd.  y may be x."""
+    stride).  gamma, beta: float32 [cols] or None; mean, rstd: float32 [rows], kept for layer_norm_bwd.  y may be x; no
+    output shares memory with another tensor otherwise."""
     rows, cols = shape = _ln_shape(x)
     dt = _dtype(x, 'x')
     if not 0.0 <= eps < math.inf:
         raise ValueError('eps must be finite and not negative')
-    (xp, xld), (yp, yld) = _ln_rows(x, shape, x.dtype, 'x'), _ln_rows(y, shape, x.dtype, 'y')
-    ga, be = _ln_vec(gamma, cols, 'gamma'), _ln_vec(beta, cols, 'beta')
-    mp, rp = _ln_vec(mean, rows, 'mean'), _ln_vec(rstd, rows, 'rstd')
+    (xp, xld, mx), (yp, yld, my) = _ln_rows(x, shape, x.dtype, 'x'), _ln_rows(y, shape, x.dtype, 'y')
+    ins, outs = [], [my]
+    ga, be = _ln_vec(gamma, cols, 'gamma', ins), _ln_vec(beta, cols, 'beta', ins)
+    mp, rp = _ln_vec(mean, rows, 'mean', outs), _ln_vec(rstd, rows, 'rstd', outs)
+    if yp != xp or yld != xld:                         # in place: x is y
+        ins.append(mx)
+    _apart(outs, ins)
     stream = _here('x y gamma beta mean rstd', x, y, gamma, beta, mean, rstd)
     check(lib().ctr_layer_norm_fwd(xp, xld, rows, cols, dt, ga, be, eps, yp, yld, mp, rp, stream), 'ctr_layer_norm_fwd')
 
@@ -1435,15 +1446,22 @@ def layer_norm_fwd(x, y, *, gamma=None, beta=None, eps=1e-5, mean=None, rstd=Non
 @_timed
 def layer_norm_bwd(dy, x, mean, rstd, dx, *, gamma=None, dgamma=None, dbeta=None, accumulate=False, ws):
     """dx, dgamma and dbeta of layer_norm_fwd from its x, mean and rstd.  accumulate: dx is added to what it holds (the
-    gradient that the residual branch left there).  dx may be dy or x."""
+    gradient that the residual branch left there).  dx may be dy or x; no output shares memory with another tensor
+    otherwise."""
     rows, cols = shape = _ln_shape(x)
     dt = _dtype(x, 'x')
-    (gp, gld), (xp, xld) = _ln_rows(dy, shape, x.dtype, 'dy'), _ln_rows(x, shape, x.dtype, 'x')
-    dp, dld = _ln_rows(dx, shape, x.dtype, 'dx')
+    (gp, gld, mg), (xp, xld, mx) = _ln_rows(dy, shape, x.dtype, 'dy'), _ln_rows(x, shape, x.dtype, 'x')
+    dp, dld, md = _ln_rows(dx, shape, x.dtype, 'dx')
     if mean is None or rstd is None:
         raise ValueError('layer_norm_bwd needs the mean and rstd that layer_norm_fwd kept')
-    mp, rp, ga = _ln_vec(mean, rows, 'mean'), _ln_vec(rstd, rows, 'rstd'), _ln_vec(gamma, cols, 'gamma')
-    dg, db = _ln_vec(dgamma, cols, 'dgamma'), _ln_vec(dbeta, cols, 'dbeta')
+    ins, outs = [], [md]
+    mp, rp, ga = _ln_vec(mean, rows, 'mean', ins), _ln_vec(rstd, rows, 'rstd', ins), _ln_vec(gamma, cols, 'gamma', ins)
+    dg, db = _ln_vec(dgamma, cols, 'dgamma', outs), _ln_vec(dbeta, cols, 'dbeta', outs)
+    if dp != gp or dld != gld:                         # in place: dy, or x, is dx
+        ins.append(mg)
+    if dp != xp or dld != xld:
+        ins.append(mx)
+    _apart(outs, ins)
     stream = _here('dy x mean rstd dx gamma dgamma dbeta', dy, x, mean, rstd, dx, gamma, dgamma, dbeta)
     L = lib()
     wp, wn = (None, 0) if dg is None and db is None else ws.get(L.ctr_layer_norm_bwd_workspace_bytes(rows, cols))

@@ -1,4 +1,4 @@
-"""Outputs of cross attention that share memory with another tensor of the call are refused, views that only interleave in
+"""Outputs of cross attention and layer norm that share memory with another tensor of the call are refused, views that only interleave in
 one buffer are not (CPU tensors: a call that is well formed ends at the check of the device)."""
 import random
 
@@ -137,3 +137,72 @@ def test_views_that_interleave_are_taken():
     shared = _t(1, TQ, H, D).expand(B, TQ, H, D)                       # inputs may be one another
     with pytest.raises(ValueError, match='must live on the GPU'):
         _bwd(dout=shared, q=shared, out=shared)
+
+
+ROWS, COLS = 4, 6
+
+
+def _norm_fwd(**kw):
+    a = dict(x=_t(ROWS, COLS), y=_t(ROWS, COLS), gamma=_t(COLS), beta=_t(COLS), mean=_t(ROWS), rstd=_t(ROWS))
+    a.update(kw)
+    ops.layer_norm_fwd(**a)
+
+
+def _norm_bwd(**kw):
+    a = dict(dy=_t(ROWS, COLS), x=_t(ROWS, COLS), mean=_t(ROWS), rstd=_t(ROWS), dx=_t(ROWS, COLS), gamma=_t(COLS),
+             dgamma=_t(COLS), dbeta=_t(COLS))
+    a.update(kw)
+    ops.layer_norm_bwd(**a, ws=Ws())
+
+
+@pytest.mark.parametrize('by', [1, 3, COLS, 2 * COLS])
+def test_layer_norm_refuses_shifted_rows(by):
+    a, b = _shifted((ROWS, COLS), by)
+    with pytest.raises(ValueError, match='y shares its memory with x'):
+        _norm_fwd(x=a, y=b)
+    with pytest.raises(ValueError, match='dx shares its memory with x'):
+        _norm_bwd(x=b, dx=a)
+    with pytest.raises(ValueError, match='dx shares its memory with dy'):
+        _norm_bwd(dy=a, dx=b)
+    with pytest.raises(ValueError, match='dx shares its memory with x'):
+        _norm_bwd(dy=a, dx=a, x=b)
+
+
+def test_layer_norm_refuses_the_same_start_with_other_rows():
+    wide = _t(ROWS * 2 * COLS)
+    x, y = wide.view(ROWS, 2 * COLS)[:, :COLS], wide[:ROWS * COLS].view(ROWS, COLS)
+    with pytest.raises(ValueError, match='y shares its memory with x'):
+        _norm_fwd(x=x, y=y)
+    with pytest.raises(ValueError, match='dx shares its memory with dy'):
+        _norm_bwd(dy=x, dx=y)
+
+
+def test_layer_norm_refuses_shared_vectors():
+    rows, cols = _t(2 * ROWS), _t(2 * COLS)
+    for kw, match in ((dict(mean=rows[:ROWS], rstd=rows[:ROWS]), 'mean shares its memory with rstd'),
+                      (dict(mean=rows[:ROWS], rstd=rows[1:ROWS + 1]), 'mean shares its memory with rstd'),
+                      (dict(mean=cols[:ROWS], gamma=cols[:COLS]), 'mean shares its memory with gamma'),
+                      (dict(rstd=cols[5:5 + ROWS], beta=cols[:COLS]), 'rstd shares its memory with beta')):
+        with pytest.raises(ValueError, match=match):
+            _norm_fwd(**kw)
+    for kw, match in ((dict(dgamma=cols[:COLS], dbeta=cols[:COLS]), 'dgamma shares its memory with dbeta'),
+                      (dict(dgamma=cols[:COLS], dbeta=cols[2:COLS + 2]), 'dgamma shares its memory with dbeta'),
+                      (dict(dgamma=cols[:COLS], gamma=cols[:COLS]), 'dgamma shares its memory with gamma'),
+                      (dict(dbeta=cols[:COLS], mean=cols[:ROWS]), 'dbeta shares its memory with mean')):
+        with pytest.raises(ValueError, match=match):
+            _norm_bwd(**kw)
+    y = _t(ROWS, COLS)
+    with pytest.raises(ValueError, match='y shares its memory with mean'):
+        _norm_fwd(x=y, y=y, mean=y.view(-1)[:ROWS])
+
+
+def test_layer_norm_takes_its_rows_in_place_and_columns_side_by_side():
+    a = _t(ROWS, COLS)
+    both = _t(ROWS, 2 * COLS)
+    for call in (lambda: _norm_fwd(x=a, y=a), lambda: _norm_fwd(x=both[:, :COLS], y=both[:, COLS:]),
+                 lambda: _norm_fwd(x=both[:, :COLS], y=both[:, :COLS]), lambda: _norm_bwd(dy=a, dx=a),
+                 lambda: _norm_bwd(x=a, dx=a), lambda: _norm_bwd(x=a, dy=a, dx=a),
+                 lambda: _norm_bwd(dy=both[:, :COLS], dx=both[:, COLS:]),
+                 lambda: _norm_fwd(x=_t(1, COLS), y=_t(1, 2 * COLS)[:, :COLS], mean=_t(1), rstd=_t(1))):
+        with pytest.raises(ValueError, match='must live on the GPU'):
+            call()
