@@ -1511,12 +1511,18 @@ class GradList:
         return bool(((at > 0) & (other.ends.take(at - 1, mode='clip') > self.begins)).any()) if len(other.begins) else False
 
 
+    def holds(self, address, nbytes):
+        """Whether a tensor of this list has one of the bytes."""
+        at = self.begins.searchsorted(address + nbytes)
+        return at > 0 and self.ends[at - 1] > address
+
+
 def _grad_list(grads):
     return grads if isinstance(grads, GradList) else GradList(grads)
 
 
-def _grad_call(g, norm):
-    """(address of norm, the current stream) of a call on the list g."""
+def _grad_call(g, norm, o=None):
+    """(address of norm, the current stream) of a call on the list g, with results into the list o."""
     np_ = None
     if norm is not None:
         if norm.dtype != torch.float32 or norm.numel() != 1:
@@ -1524,6 +1530,8 @@ def _grad_call(g, norm):
         if norm.get_device() < 0:
             raise ValueError('norm must live on the GPU (libctrhip has no CPU path)')
         np_ = norm.data_ptr()
+        if g.holds(np_, 4) or (o is not None and o is not g and o.holds(np_, 4)):
+            raise ValueError('norm shares its memory with a tensor of the list')
     dev = torch.cuda.current_device()
     for d in (g.device, None if norm is None else norm.get_device()):
         if d is not None and d != dev:
@@ -1557,7 +1565,7 @@ def clip_grads(grads, max_norm, norm=None, *, out=None, ws):
             raise ValueError('out must hold tensors of the same sizes and dtypes')
         if o.places != g.places and o.overlaps(g):
             raise ValueError('out shares memory with the gradients without being them')
-    np_, stream = _grad_call(g, norm)
+    np_, stream = _grad_call(g, norm, o)
     wp, wn = ws.get(lib().ctr_grad_norm_workspace_bytes(len(g)))
     check(lib().ctr_clip_grads(g.ptrs, o.ptrs, g.counts, g.dtypes, len(g), max_norm, np_, wp, wn, stream),
           'ctr_clip_grads')

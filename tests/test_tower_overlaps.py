@@ -1,5 +1,6 @@
-"""Outputs of cross attention and layer norm that share memory with another tensor of the call are refused, views that only interleave in
-one buffer are not (CPU tensors: a call that is well formed ends at the check of the device)."""
+"""Outputs of cross attention, layer norm and gradient clipping that share memory with another tensor of the call are
+refused, views that only interleave in one buffer are not (CPU tensors: a call that is well formed ends at the check of
+the device)."""
 import random
 
 import pytest
@@ -206,3 +207,33 @@ def test_layer_norm_takes_its_rows_in_place_and_columns_side_by_side():
                  lambda: _norm_fwd(x=_t(1, COLS), y=_t(1, 2 * COLS)[:, :COLS], mean=_t(1), rstd=_t(1))):
         with pytest.raises(ValueError, match='must live on the GPU'):
             call()
+
+
+def test_a_gradient_list_knows_its_bytes():
+    buf = _t(100)
+    lst = ops.GradList.__new__(ops.GradList)
+    with pytest.raises(ValueError, match='must live on the GPU'):
+        lst.__init__([buf[10:20], buf[:0], buf[40:41], buf[30:35]])
+    inside = [i for i in range(100) if lst.holds(buf[i:].data_ptr(), 4)]
+    assert inside == [*range(10, 20), *range(30, 35), 40]
+    assert lst.holds(buf[20:].data_ptr() - 1, 4) and not lst.holds(buf[20:].data_ptr(), 4)
+    none = ops.GradList([])
+    assert not none.holds(buf.data_ptr(), 4)
+
+
+@pytest.mark.gpu
+def test_the_norm_may_not_be_a_gradient():
+    dev = 'cuda:0'
+    ws = ops.Workspace(torch.device(dev))
+    buf, out = torch.ones(50, device=dev), torch.ones(52, device=dev)
+    grads, outs = ops.GradList([buf[:20], buf[30:]]), ops.GradList([out[:20], out[32:]])
+    for norm in (buf[19:20], buf[30:31], buf[49:]):
+        with pytest.raises(ValueError, match='norm shares its memory'):
+            ops.grad_norm(grads, norm, ws=ws)
+        with pytest.raises(ValueError, match='norm shares its memory'):
+            ops.clip_grads(grads, 1.0, norm, ws=ws)
+    with pytest.raises(ValueError, match='norm shares its memory'):
+        ops.clip_grads(grads, 1.0, out[5:6], out=outs, ws=ws)
+    ops.grad_norm(grads, buf[20:21], ws=ws)
+    ops.clip_grads(grads, 1.0, out[20:21], out=outs, ws=ws)
+    assert abs(buf[20].item() - 40 ** 0.5) < 1e-6 and out[20] == buf[20] and (buf[:20] == 1).all() and out[21] == 1
