@@ -818,7 +818,8 @@ int ctr_cross_attn_bwd(const ctr_attn_t* shape, const ctr_heads_t* dout, const c
                        const ctr_heads_t* dk, const ctr_heads_t* dv, void* workspace, size_t workspace_bytes,
                        void* stream);
 
-/* Layer norm over the columns of a [rows, cols] view (any leading dimension >= cols, any alignment):
+/* Layer norm over the columns of a [rows, cols] view (1 to 2^30 - 1 columns, any leading dimension >= cols, any
+ * alignment):
  *   y = (x - mean) rstd gamma + beta,  rstd = 1 / sqrt(var + eps),  var = mean of (x - mean)^2
  * gamma / beta [cols] optional (1 and 0).  mean_out, rstd_out [rows]: kept for the backward (optional).  y may be x.
  * _bwd: with g = dy gamma and xh = (x - mean) rstd,  dx = rstd (g - mean(g) - xh mean(g xh)) (added to dx's content

@@ -535,7 +535,8 @@ using namespace ctr;
 extern "C" int ctr_layer_norm_fwd(const void* x, int64_t x_ld, int64_t rows, int cols, int dtype, const float* gamma,
                                   const float* beta, float eps, void* y, int64_t y_ld, float* mean_out, float* rstd_out,
                                   void* stream) {
-  CTR_REQUIRE(rows >= 0 && cols >= 1, "layer_norm_fwd: rows %lld cols %d", (long long)rows, cols);
+  CTR_REQUIRE(rows >= 0 && cols >= 1 && cols < (1 << 30), "layer_norm_fwd: rows %lld cols %d (1 to 2^30 - 1)",
+              (long long)rows, cols);
   CTR_REQUIRE(type_bytes(dtype) != 0, "layer_norm_fwd: unknown dtype %d", dtype);
   CTR_REQUIRE(eps >= 0.f, "layer_norm_fwd: eps must not be negative");
   if (rows == 0) return CTR_OK;
@@ -554,7 +555,8 @@ extern "C" int ctr_layer_norm_bwd(const void* dy, int64_t dy_ld, const void* x, 
                                   const float* rstd, int64_t rows, int cols, int dtype, const float* gamma, void* dx,
                                   int64_t dx_ld, int accumulate_dx, float* dgamma, float* dbeta, void* workspace,
                                   size_t workspace_bytes, void* stream) {
-  CTR_REQUIRE(rows >= 0 && cols >= 1, "layer_norm_bwd: rows %lld cols %d", (long long)rows, cols);
+  CTR_REQUIRE(rows >= 0 && cols >= 1 && cols < (1 << 30), "layer_norm_bwd: rows %lld cols %d (1 to 2^30 - 1)",
+              (long long)rows, cols);
   CTR_REQUIRE(type_bytes(dtype) != 0, "layer_norm_bwd: unknown dtype %d", dtype);
   CTR_REQUIRE(rows == 0 || (dy && x && mean && rstd && dx && dy_ld >= cols && x_ld >= cols && dx_ld >= cols),
               "layer_norm_bwd: missing tensor or a leading dimension below cols");
