@@ -796,7 +796,8 @@ int ctr_all2allv(ctr_comm_t* comm, const void* send, const int64_t* send_offset,
  * and above, infinities among them, give NaN where they enter.
  * _bwd: dq, dk, dv (all overwritten, zeros for keys that are left out) from dout and the forward's q, k, v, out, lse,
  * sl, mask; dk / dv are summed over the query heads that share a key head.  Outputs share no memory with an input or
- * with each other.  All sums in a fixed order.
+ * with each other.  All sums in a fixed order.  Refused: shapes that need 2^32 threads or more in one launch (from 2^24
+ * samples times key heads on, later for short ones).
  * ---------------------------------------------------------------------------------- */
 typedef struct {
   int B, Tq, Tk, H, Hkv, D, dtype;

@@ -207,9 +207,9 @@ __device__ static inline BlockAt block_at(const Attn& a, int per) {
   const int turn = id >> 3;
   return {turn / per * 8 + (id & 7), turn % per};
 }
-static unsigned pair_blocks(const Attn& a, int64_t per) {              // blocks of pairs beyond the last one leave at once
+static int64_t pair_blocks(const Attn& a, int64_t per) {               // blocks of pairs beyond the last one leave at once
   const int64_t pairs = (int64_t)a.B * a.Hkv;
-  return (unsigned)((by_dies(pairs) ? (pairs + 7) / 8 * 8 : pairs) * per);
+  return (by_dies(pairs) ? (pairs + 7) / 8 * 8 : pairs) * per;
 }
 
 __device__ static inline int key_count(const Attn& a, int b) {
@@ -1628,7 +1628,30 @@ static size_t bwd_ws(const Attn& a) {
   return bwd_ws_first(a) + (rows > keys ? rows : keys) + 256;           // one after the other
 }
 
-static int attn_shape(const char* what, const ctr_attn_t* s, Attn* a) {
+// Blocks of attn_rows_kv_kernel per pair, and keys for each
+static int kv_chunk_keys(const Attn& a) {
+  const int64_t want = cdiv(2048, (int64_t)a.B * a.Hkv), most = cdiv(a.Tk, 64);
+  return (int)cdiv(a.Tk, want < most ? want : most);
+}
+static int kv_chunks(const Attn& a) { return (int)cdiv(a.Tk, kv_chunk_keys(a)); }
+
+// Whether every launch of a call has fewer than 2^32 threads: the hardware counts them in 32 bits
+static bool launches_fit(const Attn& a, bool backward) {
+  auto fits = [](int64_t blocks, int threads) { return blocks < (1ll << 32) / threads; };
+  const int64_t pairs = (int64_t)a.B * a.Hkv;
+  if (a.few) {
+    const bool alone = a.waves == 1 && (!backward || rows_fused(a));
+    if (!fits(alone ? cdiv(pairs, 4) : pair_blocks(a, a.splits), 256)) return false;
+    return !backward || rows_fused(a) || pairs == 0 || fits(pairs * kv_chunks(a), 256);
+  }
+  if (!fits(pair_blocks(a, (int64_t)a.row_tiles * a.splits), 64 * a.row_waves)) return false;
+  if (a.splits > 1 && !fits(a.splits >= JOIN_WIDE ? total_rows(a) : cdiv(total_rows(a) * (a.D / 4), 256), 256)) return false;
+  if (!backward) return true;
+  return fits(pair_blocks(a, (int64_t)a.key_tiles * a.row_splits), 64 * a.key_waves) &&
+         (a.row_splits == 1 || fits(cdiv(pairs * a.Tk * (a.D / 2), 256), 256));
+}
+
+static int attn_shape(const char* what, const ctr_attn_t* s, bool backward, Attn* a) {
   CTR_REQUIRE(s, "%s: no shape", what);
   CTR_REQUIRE(type_bytes(s->dtype) != 0, "%s: unknown dtype %d", what, s->dtype);
   CTR_REQUIRE(s->B >= 0 && s->Tq >= 0 && s->Tk >= 0 && s->H >= 1 && s->Hkv >= 1 && s->H % s->Hkv == 0,
@@ -1644,9 +1667,7 @@ static int attn_shape(const char* what, const ctr_attn_t* s, Attn* a) {
   a->scale2 = s->scale * LOG2E;
   a->sl = s->sl; a->mask = s->mask; a->mask_ld = s->mask_ld;
   attn_plan(a, s->dtype);
-  const int64_t pairs = ((int64_t)a->B * a->Hkv + 7) / 8 * 8;
-  CTR_REQUIRE((a->few ? 1 : (int64_t)a->row_tiles) * pairs * a->splits < (1ll << 31) &&
-              cdiv(a->Tk, 32) * pairs * (a->few ? 1 : a->row_splits) < (1ll << 31), "%s: too many tiles", what);
+  CTR_REQUIRE(launches_fit(*a, backward), "%s: a launch of 2^32 threads or more", what);
   return CTR_OK;
 }
 
@@ -1726,8 +1747,7 @@ static void rows_bwd_launch(const Attn& a, hipStream_t st) {
     return;
   }
   const int64_t pairs = (int64_t)a.B * a.Hkv;
-  const int64_t want = cdiv(2048, pairs), most = cdiv(a.Tk, 64);
-  const int per = (int)cdiv(a.Tk, want < most ? want : most), chunks = (int)cdiv(a.Tk, per);
+  const int per = kv_chunk_keys(a), chunks = kv_chunks(a);
 #define ROWS_BWD(T_, LPK_)                                                                        \
   attn_rows_bwd_kernel<T_, R, LPK_, 4, false><<<blocks, 256, joins, st>>>(a);                     \
   attn_rows_kv_kernel<T_, R, LPK_><<<(unsigned)(pairs * chunks), 256, 0, st>>>(a, chunks, per)
@@ -1816,11 +1836,11 @@ using namespace ctr;
 
 extern "C" size_t ctr_cross_attn_fwd_workspace_bytes(const ctr_attn_t* shape) {
   Attn a;
-  return attn_shape("cross_attn_fwd", shape, &a) ? 0 : fwd_ws(a);
+  return attn_shape("cross_attn_fwd", shape, false, &a) ? 0 : fwd_ws(a);
 }
 extern "C" size_t ctr_cross_attn_bwd_workspace_bytes(const ctr_attn_t* shape) {
   Attn a;
-  return attn_shape("cross_attn_bwd", shape, &a) ? 0 : bwd_ws(a);
+  return attn_shape("cross_attn_bwd", shape, true, &a) ? 0 : bwd_ws(a);
 }
 
 extern "C" int ctr_cross_attn_fwd(const ctr_attn_t* s, const ctr_heads_t* q, const ctr_heads_t* k, const ctr_heads_t* v,
@@ -1828,7 +1848,7 @@ extern "C" int ctr_cross_attn_fwd(const ctr_attn_t* s, const ctr_heads_t* q, con
                                   void* stream) {
   const char* what = "cross_attn_fwd";
   Attn a;
-  int rc = attn_shape(what, s, &a);
+  int rc = attn_shape(what, s, false, &a);
   if (rc) return rc;
   if ((rc = attn_view(what, "q", q, s->B, s->Tq, s->H, s->D, s->dtype, false, &a.q))) return rc;
   if ((rc = attn_view(what, "k", k, s->B, s->Tk, s->Hkv, s->D, s->dtype, false, &a.k))) return rc;
@@ -1859,7 +1879,7 @@ extern "C" int ctr_cross_attn_bwd(const ctr_attn_t* s, const ctr_heads_t* dout, 
                                   size_t workspace_bytes, void* stream) {
   const char* what = "cross_attn_bwd";
   Attn a;
-  int rc = attn_shape(what, s, &a);
+  int rc = attn_shape(what, s, true, &a);
   if (rc) return rc;
   if ((rc = attn_view(what, "dout", dout, s->B, s->Tq, s->H, s->D, s->dtype, false, &a.dout))) return rc;
   if ((rc = attn_view(what, "q", q, s->B, s->Tq, s->H, s->D, s->dtype, false, &a.q))) return rc;

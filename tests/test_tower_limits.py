@@ -19,3 +19,38 @@ def test_layer_norm_columns(cols):
     assert _refused(fwd, 'layer_norm_fwd: rows 1 cols %d' % cols)
     bwd = lib.ctr_layer_norm_bwd(P, 1 << 31, P, 1 << 31, P, P, 1, cols, 0, None, 2 * P, 1 << 31, 0, None, None, None, 0, None)
     assert _refused(bwd, 'layer_norm_bwd: rows 1 cols %d' % cols)
+
+
+def _shape(B, Tq, Tk, D=128, dtype=0):
+    return _lib.ATTN.pack(B, Tq, Tk, 1, 1, D, dtype, 0.25, 0, 0, 0)
+
+
+def _calls(shape):
+    """What the forward and the backward say of a shape, without tensors: the first thing they miss."""
+    lib = _lib.load()
+    v = _lib.HEADS.pack(0, 4096, 256, 16)
+    assert lib.ctr_cross_attn_fwd(shape, v, v, v, v, None, None, 0, None) == -1
+    said = [lib.ctr_last_error().decode()]
+    assert lib.ctr_cross_attn_bwd(shape, v, v, v, v, v, None, v, v, v, None, 0, None) == -1
+    return said + [lib.ctr_last_error().decode()]
+
+
+@pytest.mark.parametrize('most,Tq,Tk,D', [
+    ((1 << 24) - 8, 5, 5, 128),          # four waves for each (sample, head)
+    ((1 << 23) - 8, 129, 40, 128),       # two strips of rows
+    ((1 << 26) - 8, 1, 5, 128),          # few rows: four pairs to a block
+    ((1 << 26) - 8, 5, 5, 32),           # blocks of one wave
+])
+def test_attention_launches(most, Tq, Tk, D):
+    """A launch holds fewer than 2^32 threads: the last shape below that is taken, the next ones are refused before
+    anything is written."""
+    assert all('is NULL' in text for text in _calls(_shape(most, Tq, Tk, D)))
+    for B in (most + 8, 2 * most):
+        assert all('2^32 threads' in text for text in _calls(_shape(B, Tq, Tk, D)))
+        assert _lib.load().ctr_cross_attn_bwd_workspace_bytes(_shape(B, Tq, Tk, D)) == 0
+
+
+def test_attention_launches_of_one_direction():
+    """Few rows whose p and dp do not fit a block's LDS: the backward needs a block per pair, the forward a quarter."""
+    fwd, bwd = _calls(_shape(1 << 24, 1, 1100))
+    assert 'is NULL' in fwd and '2^32 threads' in bwd
