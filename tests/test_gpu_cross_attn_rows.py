@@ -1,11 +1,11 @@
 """Cross attention of few query rows per key head (kernels of their own): what non-finite gradients and queries leave
-alone."""
+alone, and three rows, which the kernels for four take."""
 import math
 
 import pytest
 import torch
 
-from tests.test_gpu_cross_attn import TYPES, _check, _make, _run
+from tests.test_gpu_cross_attn import TYPES, _check, _lengths, _make, _run
 from tests.tower_reference import attention
 
 pytestmark = pytest.mark.gpu
@@ -41,3 +41,19 @@ def test_keys_left_out_get_zeros_beside_infinite_gradients_and_queries(B, Tq, Tk
     assert wrong == dict(dk=0, dv=0)
     for n in got:
         assert torch.equal(got[n][2:], clean[n][2:]), n
+
+
+# one wave to a pair in one launch, and with keys too many for its share of LDS; one block to a pair, the same two; split
+THREE = [(700, 60, 4, 32), (700, 300, 4, 16), (150, 700, 4, 40), (150, 1500, 4, 24), (3, 5000, 2, 64), (2, 2100, 1, 128),
+         (2, 1, 3, 8), (5, 37, 2, 96)]
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('Tq,G', [(3, 1), (1, 3)])
+@pytest.mark.parametrize('B,Tk,Hkv,D', THREE)
+@pytest.mark.parametrize('masked', [False, True])
+def test_three_rows(B, Tk, Hkv, D, Tq, G, masked, dtype):
+    q, k, v, dout = _make(B, Tq, Tk, Hkv * G, Hkv, D, dtype, seed=43)
+    sl = _lengths(B, Tk)
+    mask = (torch.rand(B, Tk, generator=torch.Generator().manual_seed(44)) < 0.8).to(DEV) if masked else None
+    _check(_run(q, k, v, dout, sl, mask), attention(q, k, v, sl, mask, dout=dout))
