@@ -1539,6 +1539,14 @@ def _grad_call(g, norm, o=None):
     return np_, torch._C._cuda_getCurrentRawStream(dev)
 
 
+def clip_bound(bound, name='max_norm'):
+    """A bound as clip_grads takes it: a float that is positive and finite in fp32 too."""
+    bound = float(bound)
+    if not 1.5e-45 <= bound <= 3e38:
+        raise ValueError('%s must be positive and finite (1.5e-45 to 3e38), got %s' % (name, bound))
+    return bound
+
+
 @_timed
 def grad_norm(grads, norm, *, ws):
     """norm[0] = the square root of the sum of all squares over a GradList (or a list of tensors), summed in fp64."""
@@ -1556,9 +1564,7 @@ def clip_grads(grads, max_norm, norm=None, *, out=None, ws):
     without `out`; norm (float32 [1], optional) receives the norm before clipping.  A norm that is not finite makes every
     result NaN.  In place, nothing is written when the norm is within the bound."""
     g = _grad_list(grads)
-    max_norm = float(max_norm)
-    if not 0.0 < max_norm <= 3e38:
-        raise ValueError('max_norm must be positive and finite')
+    max_norm = clip_bound(max_norm)
     o = g if out is None else _grad_list(out)
     if o is not g:
         if o.kinds != g.kinds:

@@ -58,9 +58,8 @@ class DIN(GraphOwner):
         self.fused_attention = bool(getattr(args, 'fused_attention', True)) and ops.din_attn_mlp_supported(H)
         # clip_norm (not a reference flag; None: off): the gradients of a step are scaled as tf.clip_by_global_norm
         # scales them, lookups by their slices' values; grad_norm then holds the norm before clipping (a device word)
-        self.clip_norm = getattr(args, 'clip_norm', None)
-        if self.clip_norm is not None and not 0.0 < float(self.clip_norm) < float('inf'):
-            raise ValueError('clip_norm must be positive and finite')
+        clip = getattr(args, 'clip_norm', None)
+        self.clip_norm = None if clip is None else ops.clip_bound(clip, 'clip_norm')
         self._train_graphs = {}            # (B, T) -> captured training step
         self._lr_dev = None                # the device word a captured step reads its learning rate from
         self._ready = False

@@ -1,8 +1,12 @@
 """The largest sizes of the attention-tower operators at the C ABI: what lies beyond them is refused by name, before
 anything is launched (no GPU: a call that passes its checks ends in another error)."""
+import ctypes
+import math
+
 import pytest
 
-from recommendation_amd import _lib
+from oracle import ctr_oracle as O
+from recommendation_amd import _lib, ops
 
 P = 1 << 20
 
@@ -54,3 +58,28 @@ def test_attention_launches_of_one_direction():
     """Few rows whose p and dp do not fit a block's LDS: the backward needs a block per pair, the forward a quarter."""
     fwd, bwd = _calls(_shape(1 << 24, 1, 1100))
     assert 'is NULL' in fwd and '2^32 threads' in bwd
+
+
+@pytest.mark.parametrize('bound', [0.0, -2.0, 1e-46, 3.1e38, 1e39, math.inf, math.nan])
+def test_din_refuses_the_bounds_that_clipping_refuses(bound):
+    """When the model is made, not at its first step."""
+    import recommendation_amd as ra
+    ra.enable_zoo_imports()
+    from DIN import DIN
+    cfg = O.default_cfg('DIN')
+    cfg.hidden_units, cfg.clip_norm = 32, bound
+    with pytest.raises(ValueError, match='clip_norm must be positive and finite'):
+        DIN.DIN(cfg, 5, 4, 3, [0, 1, 2, 0])
+    with pytest.raises(ValueError, match='max_norm must be positive and finite'):
+        ops.clip_grads([], bound, ws=None)
+
+
+@pytest.mark.parametrize('bound', [1.5e-45, 1e-40, 1, '0.5', 3e38])
+def test_bounds_that_fp32_holds(bound):
+    import recommendation_amd as ra
+    ra.enable_zoo_imports()
+    from DIN import DIN
+    cfg = O.default_cfg('DIN')
+    cfg.hidden_units, cfg.clip_norm = 32, bound
+    assert DIN.DIN(cfg, 5, 4, 3, [0, 1, 2, 0]).clip_norm == float(bound)
+    assert 0.0 < ctypes.c_float(float(bound)).value < math.inf
