@@ -711,6 +711,9 @@ int ctr_din_attn_mlp_wgrad_sl(const float* q, const float* k, const int32_t* sl,
                               void* workspace, size_t workspace_bytes, void* stream);
 int ctr_din_attn_pool_fwd(const float* score, const int32_t* sl, const float* K, int B, int T, int H,
                           float* att_out, float* out, void* stream);
+/* datt = dout . K;  dscore = att (datt - sum_j att_j datt_j) / sqrt(H), 0 from sl[b] on;  dK (+)= att dout.  att: the
+ * forward's weights.  A row whose weights add up to one within 2^-18 is taken for a rounded softmax and its sum for one;
+ * other rows are taken as they are. */
 int ctr_din_attn_pool_bwd(const float* dout, const float* att, const int32_t* sl, const float* K,
                           int B, int T, int H, float* dscore, float* dK, int accumulate_k, void* stream);
 int ctr_bn_infer(const float* x, int64_t x_ld, int rows, int cols,

@@ -218,6 +218,21 @@ __global__ __launch_bounds__(256) void din_attn_pool_fwd_block_kernel(const floa
   }
 }
 
+__device__ static inline double wave_sum64(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+// sum_j att[j] datt[j] for the score gradients below.  The gradients behind dscore (the scoring network's biases above all)
+// are sums over all positions of terms that nearly cancel, since the dscore of softmax weights add up to zero: an error of
+// the dot product is the same for every position and would be what is left.  So it is summed and subtracted in fp64, and
+// weights that a softmax rounded to fp32 (their sum within 2^-18 of one: up to 43 roundings of 2^-24 at 8192 positions)
+// are divided by their sum.  Weights of any other sum are taken as they are.
+__device__ static inline double pool_dot(double dot, double sum) {
+  return fabs(sum - 1.) <= 3.814697265625e-6 ? dot / sum : dot;
+}
+
 // datt[t] = dout . K[t];  dscore[t] = att[t] * (datt[t] - sum_j att[j] datt[j]) / sqrt(H)  (0 where masked)
 // dK[b,t,:] (+)= att[t] * dout
 __global__ __launch_bounds__(256) void din_attn_pool_bwd_kernel(const float* __restrict__ dout,
@@ -231,21 +246,19 @@ __global__ __launch_bounds__(256) void din_attn_pool_bwd_kernel(const float* __r
   if (b >= B) return;
   const float inv = 1.f / sqrtf((float)H);
   const int len = sl[b];
-  float dot = 0.f;
+  double dot = 0., sum = 0.;
   for (int t = lane; t < T; t += 64) {
     float da = 0.f;
     for (int h = 0; h < H; ++h) da += dout[b * H + h] * K[(b * T + t) * H + h];
     dscore[b * T + t] = da;  // staged: datt
-    dot += att[b * T + t] * da;
+    dot = fma((double)att[b * T + t], (double)da, dot);
+    sum += (double)att[b * T + t];
   }
-  dot = wave_sum(dot);
-  float rest = 0.f;                    // the weights add up to one: what is left of dot's own rounding (see the block kernel)
-  for (int t = lane; t < T; t += 64) rest += att[b * T + t] * (dscore[b * T + t] - dot);
-  dot += wave_sum(rest);
+  dot = pool_dot(wave_sum64(dot), wave_sum64(sum));
   for (int t = lane; t < T; t += 64) {
     const float a = att[b * T + t];
     const float da = dscore[b * T + t];
-    dscore[b * T + t] = t < len ? a * (da - dot) * inv : 0.f;
+    dscore[b * T + t] = t < len ? a * (float)(da - dot) * inv : 0.f;
     for (int h = 0; h < H; ++h) {
       float* o = dK + (b * T + t) * H + h;
       const float g = a * dout[b * H + h];
@@ -262,10 +275,10 @@ __global__ __launch_bounds__(256) void din_attn_pool_bwd_block_kernel(const floa
                                                                      const float* __restrict__ K, int B, int T, int H,
                                                                      float* __restrict__ dscore,
                                                                      float* __restrict__ dK, int acc_k) {
-  extern __shared__ float sm[];       // att_s[T], do_s[H], red4[4]
+  extern __shared__ float sm[];       // att_s[T], do_s[H]
+  __shared__ double red4[4], sum4[4];
   float* att_s = sm;
   float* do_s = sm + T;
-  float* red4 = do_s + H;
   const int64_t b = blockIdx.x;
   const float inv = 1.f / sqrtf((float)H);
   const int len = sl[b];
@@ -275,7 +288,7 @@ __global__ __launch_bounds__(256) void din_attn_pool_bwd_block_kernel(const floa
   // masked positions (weight exactly 0 unless the length is 0: uniform weights) add nothing to the dot product and
   // get dscore = 0: their rows of K are not read
   const int Tv = len > 0 && len < T ? len : T;
-  float dot = 0.f;
+  double dot = 0., sum = 0.;
   for (int t = threadIdx.x; t < T; t += 256) {
     float da = 0.f;
     if (t < Tv)
@@ -286,18 +299,20 @@ __global__ __launch_bounds__(256) void din_attn_pool_bwd_block_kernel(const floa
     const float a = att[b * T + t];
     att_s[t] = a;
     dscore[b * T + t] = da;   // staged: datt
-    dot += a * da;
+    dot = fma((double)a, (double)da, dot);
+    sum += (double)a;
   }
-  dot = block_sum256(dot, red4);
-  // The gradients behind dscore (the scoring network's biases above all) are sums over all positions of terms that
-  // nearly cancel, since dscore adds up to zero: dot's rounding error is the same for every position and would be what
-  // is left.  The weights add up to one, so sum_t att (datt - dot) is that error, and it is put back.
-  float rest = 0.f;
-  for (int t = threadIdx.x; t < T; t += 256) rest += att_s[t] * (dscore[b * T + t] - dot);
-  dot += block_sum256(rest, red4);
+  dot = wave_sum64(dot);
+  sum = wave_sum64(sum);
+  if ((threadIdx.x & 63) == 0) {
+    red4[threadIdx.x >> 6] = dot;
+    sum4[threadIdx.x >> 6] = sum;
+  }
+  __syncthreads();
+  dot = pool_dot((red4[0] + red4[1]) + (red4[2] + red4[3]), (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
   for (int t = threadIdx.x; t < T; t += 256) {
     const float da = dscore[b * T + t];
-    dscore[b * T + t] = t < len ? att_s[t] * (da - dot) * inv : 0.f;
+    dscore[b * T + t] = t < len ? att_s[t] * (float)(da - dot) * inv : 0.f;
   }
   const int G = 256 / H;
   const int tg = threadIdx.x / H, h = threadIdx.x - tg * H;
@@ -518,7 +533,7 @@ extern "C" int ctr_din_attn_pool_bwd(const float* dout, const float* att, const 
   CTR_REQUIRE(dout && att && sl && K && dscore && dK, "ctr_din_attn_pool_bwd: null pointer");
   if (H <= 256 && 256 % H == 0 && H % 4 == 0 && T <= 8192 && ((uintptr_t)K % 16) == 0)
     hipLaunchKernelGGL(din_attn_pool_bwd_block_kernel, dim3((unsigned)B), dim3(256),
-                       (size_t)(T + H + 4) * sizeof(float), (hipStream_t)stream, dout, att, sl, K, B, T, H, dscore, dK,
+                       (size_t)(T + H) * sizeof(float), (hipStream_t)stream, dout, att, sl, K, B, T, H, dscore, dK,
                        accumulate_k);
   else
     hipLaunchKernelGGL(din_attn_pool_bwd_kernel, dim3((unsigned)cdiv(B, 4)), dim3(256), 0, (hipStream_t)stream, dout,
