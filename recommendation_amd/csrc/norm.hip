@@ -15,6 +15,10 @@
 // barrier per sum).  fp32, 128 columns, 50 Mi elements: 76 and 124 us, 5.5 and 5.1 TB/s.
 #include "types.h"
 
+// Fused multiply-adds where the code says so and nowhere else: left to itself the compiler fuses a row's mean (sum / n)
+// or gamma into the arithmetic of some of its entries and not of others, and equal entries of a row get different results.
+#pragma clang fp contract(off)
+
 namespace ctr {
 
 constexpr int LN_LANE_ELEMS = 16;
@@ -63,17 +67,12 @@ __device__ static inline float2 row_sum2(float v, float w, float (*red)[16]) {
     return s;
   }
 }
-// sum / n as one rounded number: left to itself the compiler fuses the product into the subtraction from some entries of
-// the row and not from others, and equal entries differ
-__device__ static inline float row_mean(float sum, float inv_n) {
-#pragma clang fp contract(off)
-  return sum * inv_n;
-}
-// What the residuals d of a row around `mean` say: mean corrected, rstd, and what is left to take out of d
-struct RowStat { float mean, rstd, c; };
+// What the residuals d of a row around `mean` say: the mean corrected, and rstd and shift with xh = d rstd + shift
+struct RowStat { float mean, rstd, shift; };
 __device__ static inline RowStat row_stat(float mean, float sum_d, float sum_d2, float inv_n, float eps) {
-  const float c = row_mean(sum_d, inv_n);
-  return {mean + c, 1.f / sqrtf(fmaxf(sum_d2 * inv_n - c * c, 0.f) + eps), c};
+  const float c = sum_d * inv_n;
+  const float rstd = 1.f / sqrtf(fmaxf(fmaf(sum_d2, inv_n, -c * c), 0.f) + eps);
+  return {mean + c, rstd, -c * rstd};
 }
 // a packet on its way: whole ones as they lie, the one at the end of a row element by element
 template <class T>
@@ -139,7 +138,7 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_kernel(const T* x, int64_t x_l
       for (int j = 0; j < V; ++j) s += v[i][j];
     }
     if (base + step < rows) fetch(row + step);
-    const float mean = row_mean(row_sum<LPR>(s, red[0]), inv_n);
+    const float mean = row_sum<LPR>(s, red[0]) * inv_n;
     float q = 0.f, r = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -161,7 +160,7 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_kernel(const T* x, int64_t x_l
         const int c = (l + i * LPR) * V;
         float o[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = fmaf((v[i][j] - st.c) * st.rstd, ga[i][j], be[i][j]);
+        for (int j = 0; j < V; ++j) o[j] = fmaf(fmaf(v[i][j], st.rstd, st.shift), ga[i][j], be[i][j]);
         if (have[i] == V) packet_store(yr + c, Packet<T>::pack(o));
         else store_part(yr + c, have[i], o);
       }
@@ -246,7 +245,7 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_kernel(const T* dy, int64_t dy
         const int c = (l + i * LPR) * V;
         float o[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = rstd * ((g[i][j] - s1) - xh[i][j] * s2);
+        for (int j = 0; j < V; ++j) o[j] = rstd * fmaf(-xh[i][j], s2, g[i][j] - s1);
         if (acc) {
           float old[V];
           if (have[i] == V) Packet<T>::unpack(packet_load(dr + c), old);
@@ -335,7 +334,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_wide_kernel(const T* x, int64_t x
 #pragma unroll
       for (int j = 0; j < V; ++j) s += f[j];
     }
-    const float mean = row_mean(row_sum<1024>(s, red[0]), inv_n);
+    const float mean = row_sum<1024>(s, red[0]) * inv_n;
     for (int c = threadIdx.x * V; c < cols; c += STEP) {
       wide_load(xr, c, cols, mean, f);
 #pragma unroll
@@ -351,7 +350,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_wide_kernel(const T* x, int64_t x
       const int n = min(V, cols - c);
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        if (j < n) f[j] = fmaf((f[j] - mean - st.c) * st.rstd, gamma ? gamma[c + j] : 1.f, beta ? beta[c + j] : 0.f);
+        if (j < n) f[j] = fmaf(fmaf(f[j] - mean, st.rstd, st.shift), gamma ? gamma[c + j] : 1.f, beta ? beta[c + j] : 0.f);
       if (n == V) packet_store(yr + c, Packet<T>::pack(f));
       else store_part(yr + c, n, f);
     }
@@ -399,7 +398,7 @@ __global__ __launch_bounds__(1024) void ln_dx_wide_kernel(const T* dy, int64_t d
       for (int j = 0; j < V; ++j)
         if (j < n) {
           const float h = g[j] * (gamma ? gamma[c + j] : 1.f);
-          f[j] = rstd * ((h - s1) - (f[j] - mean) * rstd * s2) + (acc ? old[j] : 0.f);
+          f[j] = fmaf(rstd, fmaf(-(f[j] - mean) * rstd, s2, h - s1), acc ? old[j] : 0.f);
         }
       if (n == V) packet_store(dr + c, Packet<T>::pack(f));
       else store_part(dr + c, n, f);

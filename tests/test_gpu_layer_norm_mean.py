@@ -64,3 +64,16 @@ def test_backward_of_constant_rows(cols):
     want = rstd * (g - g.mean(1, keepdim=True))
     bound = rstd * ((30 + cols / 1024 + 8) * E * (g.abs() + g.abs().mean(1, keepdim=True)))
     assert ((got['dx'].double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('cols', COLS)
+def test_equal_entries_get_equal_gradients(cols, dtype):
+    """Rows of two values, dy following x: dx has two values too, whatever lane or packet an entry lies in."""
+    x = torch.where(torch.arange(cols) % 3 == 0, 3.0, -1.5).expand(4, cols).to(dtype).to(DEV).contiguous()
+    dy = torch.where(torch.arange(cols) % 3 == 0, 100.3, 99.1).expand(4, cols).to(dtype).to(DEV).contiguous()
+    got = _run(x, dy, None, None)
+    for n in ('y', 'dx'):
+        for first in range(min(cols, 2)):
+            same = got[n][:, torch.arange(cols) % 3 == 0] if first == 0 else got[n][:, torch.arange(cols) % 3 != 0]
+            assert (same == same[:, :1]).all(), (n, first, same.unique())
