@@ -6,6 +6,7 @@ before a kernel is launched.
 """
 from __future__ import annotations
 
+import bisect
 import ctypes as C
 import math
 
@@ -1491,6 +1492,7 @@ class GradList:
         for (_, end, i), (start, _, j) in zip(spans, spans[1:]):
             if start < end:
                 raise ValueError('tensors %d and %d share memory' % (i, j))
+        self.spans = spans
         self.begins = torch.tensor([s[0] for s in spans], dtype=torch.int64).numpy()
         self.ends = torch.tensor([s[1] for s in spans], dtype=torch.int64).numpy()
         self.device = None
@@ -1513,8 +1515,8 @@ class GradList:
 
     def holds(self, address, nbytes):
         """Whether a tensor of this list has one of the bytes."""
-        at = self.begins.searchsorted(address + nbytes)
-        return at > 0 and self.ends[at - 1] > address
+        at = bisect.bisect_left(self.spans, (address + nbytes,)) - 1
+        return at >= 0 and self.spans[at][1] > address
 
 
 def _grad_list(grads):
