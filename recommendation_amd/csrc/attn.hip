@@ -16,10 +16,14 @@
 // themselves); fp16's narrow exponent is met by a power of two on p (2^14) and a running one per row on ds.
 // A key behind sl[b] or off in the mask is staged as zeros and its p is set to zero, so nothing that its memory holds
 // reaches a result.  A row without keys gives zeros, lse = -inf and no gradient.  No float atomics: same bits every run.
-// Bound: matrix and vector instructions of a SIMD hardly overlap here (per wave, two to a SIMD: 4 products 63 ns, 32 fma
-// 38, 8 exp 31, all three 107), so the time of a tile is their sum.  16 heads of 2048 x 4096 of 64, batch 8, bf16: forward
-// 365 us, 750 TFLOP/s counting its two products; dq 635 us, dk / dv 660 us, 650 and 830 TFLOP/s counting three and four
-// (a large bf16 matrix product reaches 1200 on this card).
+// Bound: matrix and vector instructions, which overlap by about half, and waiting.  A loop of 4 products, 32 fma and 8 exp
+// takes a wave, two to a SIMD, 63 ns, 38 and 31 one by one; fma and exp together 80, products and exp 71, products and fma
+// 90, all three 107 (no overlap of products and the rest would be 143, a full one 80).  At head size 128 (4 x 16 heads of
+// 1025 x 2047 on 4, bf16) the waves wait for half of their cycles besides; for what, the counters taken do not say.
+// 16 heads of 2048 x 4096 of 64, batch 8, bf16: forward 336 us, 820 TFLOP/s counting its two products; dq 574 us, dk / dv
+// 600 us, 720 and 920 TFLOP/s counting three and four (a large bf16 matrix product reaches 1390 on the same card).
+// Times without a second one beside them are averages of a kernel trace over whole passes in a row on the same inputs;
+// times that are compared come from one sweep each and are to be read against each other only.
 #include "types.h"
 
 namespace ctr {
@@ -392,7 +396,10 @@ __device__ static inline void leave_out(f32x16& s, uint64_t bits, int i) {
 // Waves per SIMD the tiled kernels are built for.  Two keep a wave within 256 registers, and only then does the compiler
 // leave the accumulators where the vector units reach them: at one (512 registers) it keeps them in the other half of
 // the register file and moves every value over and back (a third of the instructions of the forward's loop).  Three spill
-// in the backward (head size 64: 940 and 1000 us for 600 and 710).
+// in the backward (head size 64: 940 and 1000 us for 600 and 710).  At two some blocks of one and two waves spill as well,
+// by the compiler's report (registers per lane, bf16 / fp16): dq of one wave 66 / 70 at head size 96 and 81 / 88 at 128, of
+// two waves 4 / 0 and 21 / 32; dk / dv of two waves 50 / 67 at 128; fp32 dk / dv 77 by one wave and 8 by four at 64, 64 by
+// four at 128.  Those are many samples of short sequences (4096 pairs of 20 rows and 500 keys of 128, bf16: dq 356 us).
 template <class T, int DP>
 constexpr int WAVES = Terms<T>::NP == 3 && DP > 64 ? 1 : 2;
 // The forward of 16-bit tensors needs fewer registers: at head sizes up to 64, blocks of four waves run four to a SIMD
@@ -1112,11 +1119,12 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(Attn a, int64_t n_rows) {
 //   delta = sum p dp,  A = sum p dp k,  S = sum p k   (dq = scale (A - delta S)),
 // pass two writes dk = scale p (dp - delta) q and dv = p dout from the kept numbers: k and v are read once, delta is
 // the exact row sum.  While p and dp fit the LDS of one block the two passes are one launch.
-// Measured: 8192 pairs of one row and up to 200 keys of 32, fp32: 43 us forward (5 TB/s), 104 backward (6 TB/s).  128 pairs
-// of one row and 32768 keys of 64, bf16, 1.07 GB of keys and values: 240 us forward (4.5 TB/s), 256 + 287 backward.
+// Measured: 8192 pairs of one row and up to 200 keys of 32, fp32: 38 us forward by itself (5.5 TB/s), 75 behind a backward,
+// whose writes are still on their way to memory; 109 backward (5.8 TB/s).  128 pairs of one row and 32768 keys of 64, bf16,
+// 1.07 GB of keys and values: 205 us forward by itself (5.2 TB/s), 263 behind a backward; 258 + 285 backward.
 constexpr int ROW_STEP = 4;                            // 2: 3 % slower on those shapes; 8: within 3 % either way
-constexpr int ROWS_LDS = 4096;                         // (key, row) pairs whose p and dp a block keeps in LDS: 104 us in one
-                                                       // launch, 132 in two
+constexpr int ROWS_LDS = 4096;                         // (key, row) pairs whose p and dp a block keeps in LDS: backward of the
+                                                       // first shape 104 us in one launch, 132 in two
 
 template <int LPK>
 __device__ static inline float slot_sum(float v) {

@@ -6,8 +6,9 @@
 // a captured graph owns its list.  Squares are summed in fp64: no element of any of the three types overflows or
 // vanishes there, and the fp64 pipe (half the fp32 rate) is far from the bound.  One partial per block, added in block
 // order by every block of the second launch: results are the same bits on every run, and there is no third launch.
-// Measured (60 tensors of fp32 and bf16, 815 MB in all, into other tensors): the squares 165 us, 4.9 TB/s, the scaling
-// 290 us, 5.6 TB/s; a large copy reaches 4.9.  24 small tensors: 4.3 us and 1.5 for the norm, launches.
+// Measured (60 tensors of fp32 and bf16, 815 MB in all, into other tensors; averages of a kernel trace over calls in a
+// row): the squares 167 us, 4.9 TB/s, the scaling 293 us, 5.6 TB/s; a large copy reaches 4.9.  24 small tensors: 4.5 us and
+// 1.7 for the norm, launches.
 #include "types.h"
 #include <math.h>
 

@@ -10,9 +10,12 @@
 // backward accumulates dgamma / dbeta of its lane's columns over all rows of its block before it writes one partial row
 // per block; a second launch adds those in block order.  Sums are fp32, in a fixed order: results are the same bits on
 // every run.  Rows above 16384 columns are walked in several passes instead.
-// Measured (32 Mi elements, bf16, 64 to 4096 columns): forward 23 - 25 us, 5.4 - 5.8 TB/s (a large copy reaches 4.9);
-// backward 33 - 36 us, 5.6 - 6.1 TB/s, and 4.6 us for the partial rows.  8192 columns: 25 and 48 (one row to a block, a
-// barrier per sum).  fp32, 128 columns, 50 Mi elements: 76 and 124 us, 5.5 and 5.1 TB/s.
+// Measured (32 Mi elements, forward and backward in turn on the same inputs, averages of a kernel trace; a large copy
+// reaches 4.9 TB/s).  bf16, 64 to 4096 columns: forward 22 - 23 us, 5.8 - 6.0 TB/s; backward 32 - 35 us, 5.7 - 6.3 TB/s, and
+// 4.7 us for the partial rows.  24 columns: 29 and 55 (three of four lanes of a row at work, and a row's arithmetic on so
+// few elements).  8192 columns: 24 and 49 + 7.5, 16384: 27 and 56 + 13 (one row to a block, two barriers in sight each).
+// fp32, 64 to 8192 columns: 43 - 48 and 76 - 80; 16384: 50 and 91 + 13; 128 columns, 50 Mi elements: 74 and 124 us, 5.7 and
+// 5.1 TB/s.  Walked rows are five times as far from memory's time: 1600 x 20000, bf16: forward 134, backward 161 + 27 + 7.
 #include "types.h"
 
 // Fused multiply-adds where the code says so and nowhere else: left to itself the compiler fuses a row's mean (sum / n)
