@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import bisect
 import ctypes as C
+import functools
 import math
 
 import torch
@@ -59,8 +60,6 @@ def set_timer(timer):
 
 
 def _timed(fn):
-    import functools
-
     @functools.wraps(fn)
     def wrap(*a, **k):
         if _TIMER is None:
@@ -1290,11 +1289,12 @@ def _lse(lse, qs):
     return p, (p if end > p else 0, end if end > p else 0, lse, 'lse')
 
 
-def _runs(t):
-    """(bytes of a contiguous run of t, [(runs, bytes apart)] of its other axes)."""
-    size = run = t.element_size()
+@functools.lru_cache(maxsize=256)
+def _runs(shape, strides, size):
+    """(bytes of a contiguous run, [(runs, bytes apart)] of the other axes) of a tensor's layout, elements of `size` bytes."""
+    run = size
     axes = []
-    for stride, n in sorted(zip(t.stride(), t.shape)):
+    for stride, n in sorted(zip(strides, shape)):
         if n == 1 or stride == 0:
             continue
         if not axes and stride * size == run:
@@ -1306,11 +1306,15 @@ def _runs(t):
 
 def _share(a, b):
     """Whether two tensors of strides >= 0 have a byte in common: whether run i of a and run j of b meet for some indices,
-    searched from the widest stride down (axes of one stride together, by the difference of their indices).  Views of the
-    same strides, such as the parts of a packed projection, take a step or two per axis; a search that takes more than
-    2000 (views of one buffer with strides of their own) counts as a meeting."""
-    ra, axes_a = _runs(a)
-    rb, axes_b = _runs(b)
+    searched from the widest stride down (axes of one stride together, by the difference of their indices).  Views whose
+    strides have a divisor that both runs fit into side by side, such as the parts of a packed projection, need no search;
+    one that takes more than 2000 steps (views of one buffer with strides of their own) counts as a meeting."""
+    ra, axes_a = _runs(a.shape, a.stride(), a.element_size())
+    rb, axes_b = _runs(b.shape, b.stride(), b.element_size())
+    behind = a.data_ptr() - b.data_ptr()
+    period = math.gcd(*[s for _, s in axes_a], *[s for _, s in axes_b])
+    if period and rb <= behind % period <= period - ra:
+        return False
     ends = {}                                          # stride -> (least, greatest) difference of the indices
     for n, s in axes_a:
         lo, hi = ends.get(s, (0, 0))
@@ -1324,7 +1328,7 @@ def _share(a, b):
         below.append((below[-1][0] + s * lo, below[-1][1] + s * hi))
     below.reverse()
     steps = 0
-    todo = [(0, a.data_ptr() - b.data_ptr())]          # a's run begins `at` behind b's: they meet where -ra < at < rb
+    todo = [(0, behind)]                               # a's run begins `at` behind b's: they meet where -ra < at < rb
     while todo:
         i, at = todo.pop()
         steps += 1
