@@ -74,7 +74,8 @@ __device__ static inline float2 row_sum2(float v, float w, float (*red)[16]) {
 struct RowStat { float mean, rstd, shift; };
 __device__ static inline RowStat row_stat(float mean, float sum_d, float sum_d2, float inv_n, float eps) {
   const float c = sum_d * inv_n;
-  const float rstd = 1.f / sqrtf(fmaxf(fmaf(sum_d2, inv_n, -c * c), 0.f) + eps);
+  const float var = fmaf(sum_d2, inv_n, -c * c);       // below zero by its rounding at most; NaN stays NaN
+  const float rstd = 1.f / sqrtf((var < 0.f ? 0.f : var) + eps);
   return {mean + c, rstd, -c * rstd};
 }
 // a packet on its way: whole ones as they lie, the one at the end of a row element by element

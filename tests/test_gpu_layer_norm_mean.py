@@ -1,4 +1,6 @@
 """Layer norm of rows whose spread is nothing or little beside their mean: the mean's rounding must not be left in the row."""
+import math
+
 import pytest
 import torch
 
@@ -77,3 +79,16 @@ def test_equal_entries_get_equal_gradients(cols, dtype):
         for first in range(min(cols, 2)):
             same = got[n][:, torch.arange(cols) % 3 == 0] if first == 0 else got[n][:, torch.arange(cols) % 3 != 0]
             assert (same == same[:, :1]).all(), (n, first, same.unique())
+
+
+@pytest.mark.parametrize('cols', [7, 40, 1000, 6001, 20001])
+@pytest.mark.parametrize('value', [math.nan, math.inf, -math.inf])
+def test_the_statistics_of_bad_rows(cols, value):
+    """A row with a NaN or an infinity keeps no rstd that looks like a number."""
+    x, dy, gamma, beta = _make(6, cols, torch.float32)
+    x[2, cols - 1] = value
+    x[4, 0] = value
+    got = _run(x, dy, gamma, beta)
+    bad = torch.tensor([False, False, True, False, True, False], device=DEV)
+    assert (got['rstd'].isnan() == bad).all() and (got['mean'].isfinite() == ~bad).all()
+    assert (got['y'].isnan().all(1) == bad).all() and (got['dx'].isnan().all(1) == bad).all()
