@@ -1331,17 +1331,17 @@ def _share(a, b):
     todo = [(0, behind)]                               # a's run begins `at` behind b's: they meet where -ra < at < rb
     while todo:
         i, at = todo.pop()
-        steps += 1
         if i == len(axes):
             if -ra < at < rb:
                 return True
             continue
-        if steps > 2000:
-            return True
         s, lo, hi = axes[i]
         least, most = below[i + 1]
         first, last = max(lo, -((at + most + ra - 1) // s)), min(hi, (rb - 1 - at - least) // s)
-        todo.extend((i + 1, at + d * s) for d in range(first, min(last, first + 2000) + 1))
+        steps += max(0, last - first + 1)
+        if steps > 2000:
+            return True
+        todo.extend((i + 1, at + d * s) for d in range(first, last + 1))
     return False
 
 
