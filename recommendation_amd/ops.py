@@ -1348,13 +1348,16 @@ def _share(a, b):
 def _apart(outs, ins):
     """outs are written: none of them may share memory with another tensor of the call.  (begin, end, tensor, name) each;
     the spans settle nearly every call."""
-    for i, (b0, e0, t0, name) in enumerate(outs):
+    n = 0
+    for b0, e0, t0, name in outs:
+        n += 1
         for b1, e1, t1, other in ins:
             if b0 < e1 and b1 < e0 and _share(t0, t1):
                 raise ValueError('%s shares its memory with %s' % (name, other))
-        for b1, e1, t1, other in outs[i + 1:]:
-            if b0 < e1 and b1 < e0 and _share(t0, t1):
-                raise ValueError('%s shares its memory with %s' % (name, other))
+        if n < len(outs):
+            for b1, e1, t1, other in outs[n:]:
+                if b0 < e1 and b1 < e0 and _share(t0, t1):
+                    raise ValueError('%s shares its memory with %s' % (name, other))
 
 
 @_timed
@@ -1397,22 +1400,23 @@ def _ln_rows(t, shape, dtype, name):
     """(address, leading dimension, span)"""
     if t.shape != shape:
         raise ValueError('%s must be %s, got %s' % (name, list(shape), list(t.shape)))
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError('%s: expected %s, got %s' % (name, dtype, t.dtype))
     ld, one = t.stride()
     rows, cols = shape
     if (one != 1 and cols > 1) or (rows > 1 and ld < cols):
         raise ValueError('%s must have a contiguous last dimension and rows that do not overlap' % name)
-    p, ld = t.data_ptr(), ld if rows > 1 else cols
-    end = p + ((rows - 1) * ld + cols) * (4 if dtype is torch.float32 else 2) if rows else 0
-    return p, ld, (p if end else 0, end, t, name)
+    p = t.data_ptr()
+    if rows <= 1:
+        return p, cols, (p, p + cols * (4 if dtype is f32 else 2), t, name) if rows else (0, 0, t, name)
+    return p, ld, (p, p + ((rows - 1) * ld + cols) * (4 if dtype is f32 else 2), t, name)
 
 
 def _ln_vec(t, n, name, spans):
     """address; its span goes to `spans`"""
     if t is None:
         return None
-    if t.dtype != torch.float32:
+    if t.dtype is not f32:
         raise TypeError('%s: expected torch.float32, got %s' % (name, t.dtype))
     if t.numel() != n or not t.is_contiguous():
         raise ValueError('%s must be contiguous with %d entries' % (name, n))
@@ -1434,10 +1438,10 @@ def layer_norm_fwd(x, y, *, gamma=None, beta=None, eps=1e-5, mean=None, rstd=Non
     stride).  gamma, beta: float32 [cols] or None; mean, rstd: float32 [rows], kept for layer_norm_bwd.  y may be x; no
     output shares memory with another tensor otherwise."""
     rows, cols = shape = _ln_shape(x)
-    dt = _dtype(x, 'x')
+    dt, kind = _dtype(x, 'x'), x.dtype
     if not 0.0 <= eps < math.inf:
         raise ValueError('eps must be finite and not negative')
-    (xp, xld, mx), (yp, yld, my) = _ln_rows(x, shape, x.dtype, 'x'), _ln_rows(y, shape, x.dtype, 'y')
+    (xp, xld, mx), (yp, yld, my) = _ln_rows(x, shape, kind, 'x'), _ln_rows(y, shape, kind, 'y')
     ins, outs = [], [my]
     ga, be = _ln_vec(gamma, cols, 'gamma', ins), _ln_vec(beta, cols, 'beta', ins)
     mp, rp = _ln_vec(mean, rows, 'mean', outs), _ln_vec(rstd, rows, 'rstd', outs)
